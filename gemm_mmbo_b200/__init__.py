@@ -14,6 +14,7 @@ _PUBLIC = (
     "MAT_C", "MmboError", "device_status", "fill", "gemm", "gemm_bcast", "gemm_mcast", "gemm_sharded", "gemm_sharded_host", "gemm_host", "set_option", "get_option", "launch_count", "last_kernel", "gemm_strided_batched", "hgemm_NN", "hgemm_NT", "hgemm_TN", "hgemm_TT",
     "kernel_name", "kernel_params", "kernel_table", "num_kernels", "select_kernel", "sgemm_NN", "sgemm_NT",
     "sgemm_TN", "sgemm_TT", "shard_columns", "status_string", "wgm_map", "workspace_bytes", "set_workspace", "tuning_set", "tuning_load", "tuning_clear",
+    "DTYPE_BF16", "w4_bytes", "w4_quantize", "w4_pack", "w4_unpack", "gemm_w4", "moe_workspace_bytes", "moe",
 )
 __all__ = list(_PUBLIC)
 

@@ -73,6 +73,16 @@ SIGNATURES = {
     "mmbo_last_kernel": (ctypes.c_int, [ctypes.c_int]),
     "mmbo_gemm_f32_noalloc": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, _sz, _sz, _sz, _fp, _vp, _sz, _vp, _sz,
                                              _fp, _vp, _sz, _vp]),
+    "mmbo_w4_bytes": (ctypes.c_int, [_sz, _sz, ctypes.c_int, ctypes.c_int, _szp]),
+    "mmbo_w4_quantize": (ctypes.c_int, [ctypes.c_int, _sz, _sz, ctypes.c_int, ctypes.c_int, _vp, _sz, _vp, _vp]),
+    "mmbo_w4_pack": (ctypes.c_int, [ctypes.c_int, _sz, _sz, ctypes.c_int, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "mmbo_w4_unpack": (ctypes.c_int, [ctypes.c_int, _sz, _sz, ctypes.c_int, ctypes.c_int, _vp, _vp, _sz, _vp]),
+    "mmbo_gemm_w4": (ctypes.c_int, [ctypes.c_int, _sz, _sz, _sz, _fp, _vp, ctypes.c_int, ctypes.c_int, _vp, _sz, _fp,
+                                    _vp, _sz, _vp]),
+    "mmbo_moe_workspace_bytes": (ctypes.c_int, [ctypes.c_int, _sz, _sz, _sz, _sz, _sz, _szp]),
+    "mmbo_moe": (ctypes.c_int, [ctypes.c_int, _sz, _sz, _sz, _sz, _sz, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp,
+                                _sz, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _fp, _vp, _sz, _vp, _vp, _vp, _sz,
+                                _vp]),
 }
 
 

@@ -1,0 +1,227 @@
+// Host side of the 4-bit and mixture-of-experts entry points: checks, launch shapes, launches.  Included by
+// mmbo_api.cu behind its own definitions, whose lock, launch counter and device queries it uses.
+#pragma once
+
+#include "moe.cuh"
+#include "w4.cuh"
+
+namespace mmbo {
+
+static bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+static int check_w4(int dtype, size_t m, size_t k, int group, int zeros) {
+  if (dtype != MMBO_DTYPE_F16 && dtype != MMBO_DTYPE_BF16) return MMBO_ERR_BAD_DTYPE;
+  if (m > 0x7fffffffull || k > 0x7fffffffull) return MMBO_ERR_BAD_DIM;
+  if (group != 32 && group != 64 && group != 128) return MMBO_ERR_BAD_GROUP;
+  if (zeros != 0 && zeros != 1) return MMBO_ERR_BAD_GROUP;
+  return MMBO_OK;
+}
+
+static size_t w4_total_bytes(size_t m, size_t k, const W4Format& f) {
+  return w4_row_blocks(m) * w4_k_tiles(k) * f.tile_bytes();
+}
+
+// One warp per tile, eight to a block.
+static int w4_tile_grid(size_t m, size_t k, unsigned* grid) {
+  const size_t blocks = (w4_row_blocks(m) * w4_k_tiles(k) + 7) / 8;
+  if (blocks > 0x7fffffffull) return MMBO_ERR_TOO_LARGE;
+  *grid = (unsigned)blocks;
+  return MMBO_OK;
+}
+
+template <typename T>
+static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* packed, W4Format f, const void* B,
+                       size_t ldb, float beta, void* C, size_t ldc, cudaStream_t st) {
+  const dim3 grid((unsigned)((m + 7) / 8), (unsigned)(n < 65535 ? n : 65535));
+  w4_gemm_simple_kernel<T><<<grid, 256, 0, st>>>(m, n, k, alpha, static_cast<const unsigned char*>(packed), f,
+                                                 static_cast<const T*>(B), ldb, beta, static_cast<T*>(C), ldc);
+  MMBO_COUNT_LAUNCH();
+  return (int)cudaGetLastError();
+}
+
+// Workspace of the expert layer: expert numbers and gates (where the caller takes none), hidden vectors.
+struct MoeWorkspace {
+  size_t ids, gates, hidden, total;
+};
+static MoeWorkspace moe_workspace(size_t tokens, size_t f, size_t topk) {
+  MoeWorkspace w;
+  w.ids = 0;
+  w.gates = align_up(tokens * topk * 4, 256);
+  w.hidden = w.gates + align_up(tokens * topk * 4, 256);
+  w.total = w.hidden + align_up(tokens * topk * f * 4, 256);
+  return w;
+}
+
+static int check_moe_sizes(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_t topk) {
+  if (dtype != MMBO_DTYPE_F16 && dtype != MMBO_DTYPE_BF16) return MMBO_ERR_BAD_DTYPE;
+  if (tokens > MMBO_MOE_MAX_TOKENS || experts == 0 || experts > MMBO_MOE_MAX_EXPERTS || topk == 0 || topk > experts ||
+      topk > MMBO_MOE_MAX_TOPK || d == 0 || f == 0 || d > MMBO_MOE_MAX_WIDTH || f > MMBO_MOE_MAX_WIDTH)
+    return MMBO_ERR_BAD_DIM;
+  return MMBO_OK;
+}
+
+template <typename T>
+static int run_moe(const MoeArgs& a, cudaStream_t st) {
+  moe_route_kernel<T><<<(unsigned)a.tokens, 256, a.experts * 4, st>>>(a);
+  MMBO_COUNT_LAUNCH();
+  const unsigned pairs = (unsigned)(a.tokens * a.topk);
+  moe_up_simple_kernel<T><<<dim3((unsigned)((a.f + 7) / 8), pairs), 256, 0, st>>>(a);
+  MMBO_COUNT_LAUNCH();
+  moe_down_simple_kernel<T><<<dim3((unsigned)((a.d + 7) / 8), (unsigned)a.tokens), 256, 0, st>>>(a);
+  MMBO_COUNT_LAUNCH();
+  return (int)cudaGetLastError();
+}
+
+}  // namespace mmbo
+
+extern "C" {
+
+int mmbo_w4_bytes(size_t m, size_t k, int group, int zeros, size_t* bytes) {
+  int rc = check_w4(MMBO_DTYPE_F16, m, k, group, zeros);
+  if (rc) return rc;
+  if (!bytes) return MMBO_ERR_NULL_POINTER;
+  *bytes = w4_total_bytes(m, k, W4Format{group, zeros});
+  return MMBO_OK;
+}
+
+int mmbo_w4_quantize(int dtype, size_t m, size_t k, int group, int zeros, const void* W, size_t ldw, void* packed,
+                     void* stream) {
+  MMBO_API_LOCK();
+  int rc = check_w4(dtype, m, k, group, zeros);
+  if (rc) return rc;
+  if (m == 0 || k == 0) return MMBO_OK;
+  if (!W || !packed) return MMBO_ERR_NULL_POINTER;
+  if (ldw < k) return MMBO_ERR_BAD_LDA;
+  if (!aligned_to(W, 2) || !aligned_to(packed, 16)) return MMBO_ERR_MISALIGNED;
+  unsigned grid = 0;
+  if ((rc = w4_tile_grid(m, k, &grid))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const W4Format f{group, zeros};
+  if (dtype == MMBO_DTYPE_F16)
+    w4_quantize_kernel<__half><<<grid, 256, 0, st>>>(m, k, f, static_cast<const __half*>(W), ldw,
+                                                     static_cast<unsigned char*>(packed));
+  else
+    w4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m, k, f, static_cast<const __nv_bfloat16*>(W), ldw,
+                                                            static_cast<unsigned char*>(packed));
+  MMBO_COUNT_LAUNCH();
+  return (int)cudaGetLastError();
+}
+
+int mmbo_w4_pack(int dtype, size_t m, size_t k, int group, const unsigned char* codes, size_t ldcodes,
+                 const void* scales, size_t ldscales, const unsigned char* zeroPoints, size_t ldzeros, void* packed,
+                 void* stream) {
+  MMBO_API_LOCK();
+  const int zeros = zeroPoints != nullptr;
+  int rc = check_w4(dtype, m, k, group, zeros);
+  if (rc) return rc;
+  if (m == 0 || k == 0) return MMBO_OK;
+  if (!codes || !scales || !packed) return MMBO_ERR_NULL_POINTER;
+  const size_t groups = (k + group - 1) / group;
+  if (ldcodes < (k + 1) / 2) return MMBO_ERR_BAD_LDA;
+  if (ldscales < groups || (zeros && ldzeros < groups)) return MMBO_ERR_BAD_LDB;
+  if (!aligned_to(scales, 2) || !aligned_to(packed, 16)) return MMBO_ERR_MISALIGNED;
+  unsigned grid = 0;
+  if ((rc = w4_tile_grid(m, k, &grid))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const W4Format f{group, zeros};
+  unsigned char* out = static_cast<unsigned char*>(packed);
+  if (dtype == MMBO_DTYPE_F16)
+    w4_pack_kernel<__half><<<grid, 256, 0, st>>>(m, k, f, codes, ldcodes, static_cast<const __half*>(scales), ldscales,
+                                                 zeroPoints, ldzeros, out);
+  else
+    w4_pack_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m, k, f, codes, ldcodes,
+                                                        static_cast<const __nv_bfloat16*>(scales), ldscales,
+                                                        zeroPoints, ldzeros, out);
+  MMBO_COUNT_LAUNCH();
+  return (int)cudaGetLastError();
+}
+
+int mmbo_w4_unpack(int dtype, size_t m, size_t k, int group, int zeros, const void* packed, void* W, size_t ldw,
+                   void* stream) {
+  MMBO_API_LOCK();
+  int rc = check_w4(dtype, m, k, group, zeros);
+  if (rc) return rc;
+  if (m == 0 || k == 0) return MMBO_OK;
+  if (!W || !packed) return MMBO_ERR_NULL_POINTER;
+  if (ldw < k) return MMBO_ERR_BAD_LDA;
+  if (!aligned_to(W, 2) || !aligned_to(packed, 16)) return MMBO_ERR_MISALIGNED;
+  unsigned grid = 0;
+  if ((rc = w4_tile_grid(m, k, &grid))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const W4Format f{group, zeros};
+  const unsigned char* in = static_cast<const unsigned char*>(packed);
+  if (dtype == MMBO_DTYPE_F16)
+    w4_unpack_kernel<__half><<<grid, 256, 0, st>>>(m, k, f, in, static_cast<__half*>(W), ldw);
+  else
+    w4_unpack_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m, k, f, in, static_cast<__nv_bfloat16*>(W), ldw);
+  MMBO_COUNT_LAUNCH();
+  return (int)cudaGetLastError();
+}
+
+int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, const float* alpha, const void* packed, int group, int zeros,
+                 const void* B, size_t ldb, const float* beta, void* C, size_t ldc, void* stream) {
+  MMBO_API_LOCK();
+  int rc = check_w4(dtype, m, k, group, zeros);
+  if (rc) return rc;
+  if (n > 0x7fffffffull) return MMBO_ERR_BAD_DIM;
+  if (!alpha || !beta) return MMBO_ERR_NULL_POINTER;
+  if (m == 0 || n == 0) return MMBO_OK;
+  if (!C || (k && (!packed || !B))) return MMBO_ERR_NULL_POINTER;
+  if (k && (ldb < k || ldb > 0x7fffffffull)) return MMBO_ERR_BAD_LDB;
+  if (ldc < m || ldc > 0x7fffffffull) return MMBO_ERR_BAD_LDC;
+  if (!aligned_to(C, 2) || (k && (!aligned_to(B, 2) || !aligned_to(packed, 16)))) return MMBO_ERR_MISALIGNED;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const W4Format f{group, zeros};
+  if (dtype == MMBO_DTYPE_F16) return run_w4_gemm<__half>(m, n, k, *alpha, packed, f, B, ldb, *beta, C, ldc, st);
+  return run_w4_gemm<__nv_bfloat16>(m, n, k, *alpha, packed, f, B, ldb, *beta, C, ldc, st);
+}
+
+int mmbo_moe_workspace_bytes(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_t topk, size_t* bytes) {
+  int rc = check_moe_sizes(dtype, tokens, d, f, experts, topk);
+  if (rc) return rc;
+  if (!bytes) return MMBO_ERR_NULL_POINTER;
+  *bytes = moe_workspace(tokens, f, topk).total;
+  return MMBO_OK;
+}
+
+int mmbo_moe(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_t topk, int renorm, int group, int zeros,
+             const void* X, size_t ldx, const void* router, size_t ldr, const void* gate, const void* up, size_t ldg,
+             size_t strideG, const void* down, size_t ldd, size_t strideD, const float* beta, void* Y, size_t ldy,
+             int* ids, float* gates, void* workspace, size_t workspaceBytes, void* stream) {
+  MMBO_API_LOCK();
+  int rc = check_moe_sizes(dtype, tokens, d, f, experts, topk);
+  if (rc) return rc;
+  if (renorm != 0 && renorm != 1) return MMBO_ERR_BAD_DIM;
+  if (group != 0 && (rc = check_w4(dtype, d, f, group, zeros))) return rc;
+  if (group == 0 && zeros != 0) return MMBO_ERR_BAD_GROUP;
+  if (!beta) return MMBO_ERR_NULL_POINTER;
+  if (tokens == 0) return MMBO_OK;
+  if (!X || !router || !gate || !up || !down || !Y || !workspace) return MMBO_ERR_NULL_POINTER;
+  if (ldx < d || ldx > 0x7fffffffull) return MMBO_ERR_BAD_LDB;
+  if (ldy < d || ldy > 0x7fffffffull) return MMBO_ERR_BAD_LDC;
+  if (ldr < d || ldr > 0x7fffffffull) return MMBO_ERR_BAD_LDA;
+  const W4Format fmt{group, zeros};
+  if (group == 0) {
+    if (ldg < d || ldd < f || ldg > 0x7fffffffull || ldd > 0x7fffffffull) return MMBO_ERR_BAD_LDA;
+    if (experts > 1 && (strideG < (f - 1) * ldg + d || strideD < (d - 1) * ldd + f)) return MMBO_ERR_BAD_LDA;
+    if (!aligned_to(gate, 2) || !aligned_to(up, 2) || !aligned_to(down, 2)) return MMBO_ERR_MISALIGNED;
+  } else {
+    if (experts > 1 && (strideG < w4_total_bytes(f, d, fmt) || strideD < w4_total_bytes(d, f, fmt)))
+      return MMBO_ERR_BAD_LDA;
+    if (!aligned_to(gate, 16) || !aligned_to(up, 16) || !aligned_to(down, 16)) return MMBO_ERR_MISALIGNED;
+    if (experts > 1 && (strideG % 16 != 0 || strideD % 16 != 0)) return MMBO_ERR_MISALIGNED;
+  }
+  if (!aligned_to(X, 2) || !aligned_to(router, 2) || !aligned_to(Y, 2) || !aligned_to(ids, 4) ||
+      !aligned_to(gates, 4) || !aligned_to(workspace, 256))
+    return MMBO_ERR_MISALIGNED;
+  const MoeWorkspace ws = moe_workspace(tokens, f, topk);
+  if (workspaceBytes < ws.total) return MMBO_ERR_WORKSPACE;
+  char* base = static_cast<char*>(workspace);
+  MoeArgs a{tokens, d, f, experts, topk, renorm, fmt, X, router, gate, up, down, ldx, ldr, ldg, strideG, ldd, strideD,
+            *beta, Y, ldy, ids ? ids : reinterpret_cast<int*>(base + ws.ids),
+            gates ? gates : reinterpret_cast<float*>(base + ws.gates), reinterpret_cast<float*>(base + ws.hidden)};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == MMBO_DTYPE_F16 ? run_moe<__half>(a, st) : run_moe<__nv_bfloat16>(a, st);
+}
+
+}  // extern "C"

@@ -1726,6 +1726,8 @@ const char* mmbo_status_string(int status) {
     case MMBO_ERR_BAD_OPTION: return "unknown option name";
     case MMBO_ERR_NCCL: return "an NCCL call on the caller's communicator failed";
     case MMBO_ERR_NO_NCCL: return "libnccl.so.2 could not be found in the process";
+    case MMBO_ERR_BAD_GROUP: return "group must be 32, 64 or 128 and zeros 0 or 1";
+    case MMBO_ERR_MISALIGNED: return "a pointer or stride is not aligned as the entry point asks";
     case MMBO_ERR_NOALLOC_TOO_LARGE:
       return "problem needs more scratch than the library's built-in MMBO_NOALLOC_SCRATCH_BYTES";
   }
@@ -1926,3 +1928,5 @@ int mmbo_gemm_f32_noalloc(int transA, int transB, size_t m, size_t n, size_t k, 
 }
 
 }  // extern "C"
+
+#include "low_bit_api.cuh"

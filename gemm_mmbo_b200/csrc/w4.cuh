@@ -1,0 +1,279 @@
+// 4-bit weights with group scales: the packed format, the kernels that write and read it, and the product of a packed
+// matrix with columns of 16-bit activations.
+//
+//   W(i, j) = (q(i, j) - z(i, g)) * s(i, g),   g = j / group,   q and z in 0..15   (z = 8 where no zero points are kept)
+//   C = alpha * W * B + beta * C               W is m x k, B is k x n, C is m x n, column-major
+//
+// Packed format.  Rows are taken in blocks of 16 and columns in tiles of 128; the tiles of one row block follow one
+// another, so that whoever walks along k reads one contiguous stream.  A tile is
+//     1024 bytes of codes          row r (0..15) at 64 r; within a row, 16 bytes for each of four "lanes" t, holding one
+//                                  32-bit word for each quarter u of the tile: the columns 32 u + 8 t .. + 7
+//     (128 / group) x 16 scales    in the activations' type, group by group, row by row
+//     (128 / group) x 16 bytes     zero points, where the matrix has them
+// In a word, column j of its eight sits in nibble (j >> 1) + 4 (j & 1): `(w >> 4 p) & 0x000f000f` is the pair
+// (2p, 2p + 1) in the two halves of a register, ready to become two 16-bit floats.  With this order the four words of
+// a lane are the four k-steps a 16-row matrix instruction wants from that lane, one 16-byte load serves a whole tile
+// row, and no k-step spans two groups (groups are 32, 64 or 128 wide).
+// Rows past m and columns past k hold the code of weight zero.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ref_kernels.cuh"
+
+namespace mmbo {
+
+constexpr int kW4Rows = 16;    // rows of a block
+constexpr int kW4Cols = 128;   // columns of a tile
+constexpr int kW4Codes = 1024; // bytes of codes in a tile
+
+struct W4Format {
+  int group, zeros;
+  __host__ __device__ int groups() const { return kW4Cols / group; }
+  __host__ __device__ uint32_t tile_bytes() const { return kW4Codes + groups() * (kW4Rows * 2 + (zeros ? kW4Rows : 0)); }
+};
+__host__ __device__ inline size_t w4_row_blocks(size_t m) { return (m + kW4Rows - 1) / kW4Rows; }
+__host__ __device__ inline size_t w4_k_tiles(size_t k) { return (k + kW4Cols - 1) / kW4Cols; }
+
+// ---------------------------------------------------------------- 16-bit types --------
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight consecutive elements as they lie in memory.  `vec`: the address is 16-byte aligned and all eight exist;
+// otherwise the `left` (possibly none) that exist are read one by one and the others are zero.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, long long left, bool vec, T (&out)[8]) {
+  if (vec && left >= 8) {
+    *reinterpret_cast<uint4*>(out) = __ldg(reinterpret_cast<const uint4*>(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = i < left ? p[i] : from_f32<T>(0.f);
+  }
+}
+
+// ---------------------------------------------------------------- writing the format --
+// One warp per tile; lane 4 r + t (r 0..7, t 0..3) owns rows r and r + 8 of the block and, in each quarter u, the
+// columns 32 u + 8 t .. + 7: its eight words are two 16-byte stores, and the loads of four lanes are 64 contiguous
+// bytes of a row.  One pass, so bound by bytes: 2 m k in, m k / 2 out.
+//
+// Symmetric: s = max|w| / 7 rounded to the weights' type, z = 8.  With zero points: lo = min(w, 0), hi = max(w, 0),
+// s = (hi - lo) / 15 rounded to the weights' type, z = rint(-lo / s).  q = rint(w / s) + z, held to 0..15; ties to
+// even.  A group whose scale rounds to zero becomes zeros; one with an infinity or a NaN becomes NaN (its scale is).
+template <typename T>
+__global__ void w4_quantize_kernel(size_t m, size_t k, W4Format f, const T* __restrict__ W, size_t ldw,
+                                   unsigned char* __restrict__ packed) {
+  const size_t tiles = w4_k_tiles(k);
+  const size_t unit = (size_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (unit >= w4_row_blocks(m) * tiles) return;
+  const size_t block = unit / tiles, tile = unit % tiles;
+  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  unsigned char* out = packed + unit * f.tile_bytes();
+  const bool vec = ldw % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15u) == 0;
+  const int per = f.group / 32;  // quarters in a group
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = r + 8 * half;
+    const size_t i = block * kW4Rows + row;
+    T w[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const size_t j = tile * kW4Cols + 32 * u + 8 * t;
+      const long long left = i < m ? (long long)k - (long long)j : 0;
+      load8(W + i * ldw + j, left, vec, w[u]);
+    }
+    float lo[4], hi[4];
+    bool bad[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      lo[u] = hi[u] = 0.f;
+      bad[u] = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = to_f32(w[u][e]);
+        lo[u] = fminf(lo[u], v);
+        hi[u] = fmaxf(hi[u], v);
+        bad[u] |= !(fabsf(v) <= 3.4e38f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1) {
+        lo[u] = fminf(lo[u], __shfl_xor_sync(0xffffffffu, lo[u], x));
+        hi[u] = fmaxf(hi[u], __shfl_xor_sync(0xffffffffu, hi[u], x));
+        bad[u] |= __shfl_xor_sync(0xffffffffu, (int)bad[u], x) != 0;
+      }
+    }
+    uint32_t word[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int first = u / per * per;
+      float l = lo[u], h = hi[u];
+      bool b = bad[u];
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (v >= first && v < first + per) {
+          l = fminf(l, lo[v]);
+          h = fmaxf(h, hi[v]);
+          b |= bad[v];
+        }
+      // halves first: the span of two bfloat16 values may pass the largest float
+      const float wide = f.zeros ? (0.5f * h - 0.5f * l) / 7.5f : fmaxf(-l, h) / 7.f;
+      float s = to_f32(from_f32<T>(wide));
+      if (b || !(s <= 3.4e38f)) s = __int_as_float(0x7fc00000);
+      const bool live = s > 0.f;
+      const float z = f.zeros ? (live ? fminf(fmaxf(rintf(-l / s), 0.f), 15.f) : 0.f) : 8.f;
+      word[u] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float q = live ? fminf(fmaxf(rintf(to_f32(w[u][e]) / s) + z, 0.f), 15.f) : z;
+        word[u] |= (uint32_t)q << (4 * ((e >> 1) + 4 * (e & 1)));
+      }
+      if (t == 0 && u % per == 0) {
+        const int g = u / per;
+        reinterpret_cast<T*>(out + kW4Codes)[g * kW4Rows + row] = from_f32<T>(s);
+        if (f.zeros) out[kW4Codes + f.groups() * kW4Rows * 2 + g * kW4Rows + row] = (unsigned char)z;
+      }
+    }
+    *reinterpret_cast<uint4*>(out + row * 64 + t * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+  }
+}
+
+// Codes, scales and zero points that exist already (a quantised checkpoint), put into the packed order.
+// codes: two a byte, the even column in the low half, rows `ldcodes` bytes apart; scales and zero points row by row.
+template <typename T>
+__global__ void w4_pack_kernel(size_t m, size_t k, W4Format f, const unsigned char* __restrict__ codes, size_t ldcodes,
+                               const T* __restrict__ scales, size_t lds, const unsigned char* __restrict__ zps,
+                               size_t ldz, unsigned char* __restrict__ packed) {
+  const size_t tiles = w4_k_tiles(k);
+  const size_t unit = (size_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (unit >= w4_row_blocks(m) * tiles) return;
+  const size_t block = unit / tiles, tile = unit % tiles;
+  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  unsigned char* out = packed + unit * f.tile_bytes();
+  const size_t total_groups = (k + f.group - 1) / f.group;
+  const int per = f.group / 32;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = r + 8 * half;
+    const size_t i = block * kW4Rows + row;
+    uint32_t word[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const size_t j0 = tile * kW4Cols + 32 * u + 8 * t;
+      const size_t g = (tile * kW4Cols + 32 * u) / f.group;
+      const bool have = i < m && g < total_groups;
+      const uint32_t z = f.zeros ? (have ? (uint32_t)(zps[i * ldz + g] & 15) : 0u) : 8u;
+      word[u] = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const size_t j = j0 + e;
+        uint32_t q = z;
+        if (i < m && j < k) {
+          const uint32_t byte = codes[i * ldcodes + j / 2];
+          q = (j & 1) ? byte >> 4 : byte & 15u;
+        }
+        word[u] |= q << (4 * ((e >> 1) + 4 * (e & 1)));
+      }
+      if (t == 0 && u % per == 0) {
+        const int gt = u / per;
+        reinterpret_cast<T*>(out + kW4Codes)[gt * kW4Rows + row] = have ? scales[i * lds + g] : from_f32<T>(0.f);
+        if (f.zeros) out[kW4Codes + f.groups() * kW4Rows * 2 + gt * kW4Rows + row] = (unsigned char)z;
+      }
+    }
+    *reinterpret_cast<uint4*>(out + row * 64 + t * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+  }
+}
+
+// The weights that a packed matrix stands for, rounded to the 16-bit type (the product of a 4-bit difference and a
+// 16-bit scale has up to 15 bits): the mirror of w4_quantize_kernel.
+template <typename T>
+__global__ void w4_unpack_kernel(size_t m, size_t k, W4Format f, const unsigned char* __restrict__ packed,
+                                 T* __restrict__ W, size_t ldw) {
+  const size_t tiles = w4_k_tiles(k);
+  const size_t unit = (size_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (unit >= w4_row_blocks(m) * tiles) return;
+  const size_t block = unit / tiles, tile = unit % tiles;
+  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const unsigned char* in = packed + unit * f.tile_bytes();
+  const bool vec = ldw % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15u) == 0;
+  const int per = f.group / 32;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = r + 8 * half;
+    const size_t i = block * kW4Rows + row;
+    if (i >= m) continue;
+    const uint4 c = __ldg(reinterpret_cast<const uint4*>(in + row * 64 + t * 16));
+    const uint32_t word[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const size_t j = tile * kW4Cols + 32 * u + 8 * t;
+      if (j >= k) continue;
+      const int g = u / per;
+      const float s = to_f32(reinterpret_cast<const T*>(in + kW4Codes)[g * kW4Rows + row]);
+      const int z = f.zeros ? in[kW4Codes + f.groups() * kW4Rows * 2 + g * kW4Rows + row] : 8;
+      T v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v[e] = from_f32<T>((float)((int)((word[u] >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - z) * s);
+      T* dst = W + i * ldw + j;
+      if (vec && j + 8 <= k) {
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e < k) dst[e] = v[e];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the product ---------
+// Sum over k of row i of a packed matrix times x, in 32 bits, by one warp (the result is in every lane).
+template <typename T>
+__device__ __forceinline__ float w4_row_dot(const unsigned char* __restrict__ packed, W4Format f, size_t i, size_t k,
+                                            const T* __restrict__ x) {
+  const size_t tiles = w4_k_tiles(k);
+  const int lane = threadIdx.x & 31, half = lane >> 4, t = (lane >> 2) & 3, u = lane & 3;
+  const int row = (int)(i % kW4Rows), g = 32 * u / f.group;
+  float acc = 0.f;
+  for (size_t tile = half; tile < tiles; tile += 2) {
+    const unsigned char* in = packed + (i / kW4Rows * tiles + tile) * f.tile_bytes();
+    const uint32_t w = __ldg(reinterpret_cast<const unsigned int*>(in + row * 64 + t * 16 + u * 4));
+    const float s = to_f32(reinterpret_cast<const T*>(in + kW4Codes)[g * kW4Rows + row]);
+    const int z = f.zeros ? in[kW4Codes + f.groups() * kW4Rows * 2 + g * kW4Rows + row] : 8;
+    float part = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const size_t j = tile * kW4Cols + 32 * u + 8 * t + e;
+      if (j < k) part = fmaf((float)((int)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - z), to_f32(x[j]), part);
+    }
+    acc = fmaf(s, part, acc);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  return acc;
+}
+
+template <typename T>
+__global__ void w4_gemm_simple_kernel(size_t m, size_t n, size_t k, float alpha, const unsigned char* __restrict__ packed,
+                                      W4Format f, const T* __restrict__ B, size_t ldb, float beta, T* __restrict__ C,
+                                      size_t ldc) {
+  const size_t i = (size_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (i >= m) return;
+  for (size_t j = blockIdx.y; j < n; j += gridDim.y) {
+    const float acc = w4_row_dot(packed, f, i, k, B + j * ldb);
+    if ((threadIdx.x & 31) == 0) {
+      T* c = C + j * ldc + i;
+      const float v = alpha * acc;
+      *c = from_f32<T>(beta != 0.f ? fmaf(beta, to_f32(*c), v) : v);
+    }
+  }
+}
+
+}  // namespace mmbo

@@ -13,13 +13,14 @@ import ctypes
 
 from ._lib import LIB
 
-DTYPE_F32, DTYPE_F16, DTYPE_F64 = 0, 1, 2
+DTYPE_F32, DTYPE_F16, DTYPE_F64, DTYPE_BF16 = 0, 1, 2, 3
 KERNEL_AUTO = -1
 DIST_UNIFORM, DIST_NORMAL, DIST_ZERO = 0, 1, 2
 MAT_A, MAT_B, MAT_C = 0, 1, 2
 
 _DTYPES = {"f32": DTYPE_F32, "f16": DTYPE_F16, "f64": DTYPE_F64, DTYPE_F32: DTYPE_F32, DTYPE_F16: DTYPE_F16,
            DTYPE_F64: DTYPE_F64}
+_DTYPES16 = {"f16": DTYPE_F16, "bf16": DTYPE_BF16, DTYPE_F16: DTYPE_F16, DTYPE_BF16: DTYPE_BF16}
 
 
 class MmboError(RuntimeError):
@@ -301,3 +302,73 @@ def launch_count() -> int:
 def last_kernel(dtype) -> int:
     """Table row the most recent GEMM call of `dtype` ran (-1 before the first)."""
     return int(LIB.mmbo_last_kernel(_DTYPES[dtype]))
+
+
+# ---- 4-bit weights with group scales, mixture-of-experts layer (dtype: "f16" or "bf16") ----
+
+def w4_bytes(m: int, k: int, group: int = 128, zeros: bool = False) -> int:
+    """Bytes of a packed m x k matrix of 4-bit weights."""
+    out = ctypes.c_size_t()
+    rc = LIB.mmbo_w4_bytes(m, k, group, int(bool(zeros)), ctypes.byref(out))
+    if rc != 0:
+        raise MmboError(rc, "mmbo_w4_bytes")
+    return out.value
+
+
+def w4_quantize(dtype, m: int, k: int, group: int, zeros: bool, W, ldw: int, packed, stream=None) -> None:
+    """Rounds 16-bit weights (k contiguous, rows `ldw` apart) to the packed 4-bit format."""
+    rc = LIB.mmbo_w4_quantize(_DTYPES16[dtype], m, k, group, int(bool(zeros)), _addr(W), ldw, _addr(packed),
+                              _stream(stream))
+    if rc != 0:
+        raise MmboError(rc, "mmbo_w4_quantize")
+
+
+def w4_pack(dtype, m: int, k: int, group: int, codes, ldcodes: int, scales, ldscales: int, zero_points, ldzeros: int,
+            packed, stream=None) -> None:
+    """Packs existing codes (two a byte, even column low), scales and zero points (or None)."""
+    rc = LIB.mmbo_w4_pack(_DTYPES16[dtype], m, k, group, _addr(codes), ldcodes, _addr(scales), ldscales,
+                          _addr(zero_points), ldzeros, _addr(packed), _stream(stream))
+    if rc != 0:
+        raise MmboError(rc, "mmbo_w4_pack")
+
+
+def w4_unpack(dtype, m: int, k: int, group: int, zeros: bool, packed, W, ldw: int, stream=None) -> None:
+    """Writes the weights a packed matrix stands for, rounded to `dtype`."""
+    rc = LIB.mmbo_w4_unpack(_DTYPES16[dtype], m, k, group, int(bool(zeros)), _addr(packed), _addr(W), ldw,
+                            _stream(stream))
+    if rc != 0:
+        raise MmboError(rc, "mmbo_w4_unpack")
+
+
+def gemm_w4(dtype, m: int, n: int, k: int, alpha: float, packed, group: int, zeros: bool, B, ldb: int, beta: float, C,
+            ldc: int, stream=None) -> None:
+    """C = alpha * W * B + beta * C with W an m x k matrix packed by w4_quantize or w4_pack."""
+    a, b = ctypes.c_float(alpha), ctypes.c_float(beta)
+    rc = LIB.mmbo_gemm_w4(_DTYPES16[dtype], m, n, k, a, _addr(packed), group, zeros, _addr(B), ldb, b, _addr(C), ldc,
+                          _stream(stream))
+    if rc != 0:
+        raise MmboError(rc, "mmbo_gemm_w4")
+
+
+def moe_workspace_bytes(dtype, tokens: int, d: int, f: int, experts: int, topk: int) -> int:
+    """Bytes of device workspace that `moe` needs for these sizes."""
+    out = ctypes.c_size_t()
+    rc = LIB.mmbo_moe_workspace_bytes(_DTYPES16[dtype], tokens, d, f, experts, topk, ctypes.byref(out))
+    if rc != 0:
+        raise MmboError(rc, "mmbo_moe_workspace_bytes")
+    return out.value
+
+
+def moe(dtype, tokens: int, d: int, f: int, experts: int, topk: int, X, ldx: int, router, ldr: int, gate, up, ldg: int,
+        strideG: int, down, ldd: int, strideD: int, Y, ldy: int, group: int = 0, zeros: bool = False,
+        renorm: bool = False, beta: float = 0.0, ids=None, gates=None, workspace=None, workspace_bytes: int | None = None,
+        stream=None) -> None:
+    """A whole mixture-of-experts layer for a few tokens (mmbo_moe).  `workspace`: a tensor, or an address
+    with `workspace_bytes`."""
+    if workspace_bytes is None:
+        workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    rc = LIB.mmbo_moe(_DTYPES16[dtype], tokens, d, f, experts, topk, renorm, group, zeros, _addr(X), ldx, _addr(router),
+                      ldr, _addr(gate), _addr(up), ldg, strideG, _addr(down), ldd, strideD, ctypes.c_float(beta),
+                      _addr(Y), ldy, _addr(ids), _addr(gates), _addr(workspace), workspace_bytes, _stream(stream))
+    if rc != 0:
+        raise MmboError(rc, "mmbo_moe")

@@ -34,6 +34,7 @@ extern "C" {
 #define MMBO_DTYPE_F32 0
 #define MMBO_DTYPE_F16 1
 #define MMBO_DTYPE_F64 2
+#define MMBO_DTYPE_BF16 3 /* the 4-bit and mixture-of-experts entry points only */
 
 #define MMBO_KERNEL_AUTO (-1)
 
@@ -59,6 +60,8 @@ extern "C" {
 #define MMBO_ERR_BAD_OPTION (-18)       /* mmbo_set_option / mmbo_get_option: unknown name */
 #define MMBO_ERR_NCCL (-19)             /* an NCCL call on the caller's communicator failed */
 #define MMBO_ERR_NO_NCCL (-20)          /* no libnccl.so.2 in the process or on the loader path */
+#define MMBO_ERR_BAD_GROUP (-21)        /* 4-bit weights: group not 32, 64 or 128, or zeros not 0 or 1 */
+#define MMBO_ERR_MISALIGNED (-22)       /* a pointer or stride is not aligned as the entry point asks */
 
 /* SGEMM, fp32 storage and arithmetic.  Replaces dgemm_NT / naive_dgemm
  * (src/gemm/gemm.h:47-48, :4-5) for dtype fp32; kernelId indexes the fp32 kernel table
@@ -307,6 +310,70 @@ int mmbo_set_workspace(void* ptr, size_t bytes);
 int mmbo_gemm_f32_noalloc(int transA, int transB, size_t m, size_t n, size_t k, const float* alpha,
                           const float* A, size_t lda, const float* B, size_t ldb, const float* beta,
                           float* C, size_t ldc, void* stream);
+
+/* ---- 4-bit weights with group scales, and a mixture-of-experts layer -------------------------
+ * (New capability: the reference multiplies binary64 matrices only.)  Everything above holds here
+ * too: column-major, device pointers, host alpha / beta, work queued on `stream` of the current
+ * device, status codes, nothing allocated or kept by the library, safe to capture into a graph.
+ * dtype is MMBO_DTYPE_F16 or MMBO_DTYPE_BF16 and names the type of every 16-bit operand of the call.
+ *
+ * The format.  A weight matrix W (m x k, used as the transposed operand: k is its contiguous axis)
+ * has a 4-bit code q per element and, per row and group of `group` consecutive columns (32, 64 or
+ * 128; the last group may be short), a 16-bit scale s and, with zeros = 1, a zero point z in 0..15
+ * (zeros = 0: z = 8):  W(i,j) = (q(i,j) - z(i,g)) * s(i,g).  A packed matrix is
+ * mmbo_w4_bytes(m, k, group, zeros) bytes in the library's own order (16-byte aligned). */
+int mmbo_w4_bytes(size_t m, size_t k, int group, int zeros, size_t* bytes);
+
+/* Packs 16-bit weights: W(i,j) is W[i * ldw + j], ldw >= k.  zeros = 0: s = max|w| / 7 of the group;
+ * zeros = 1: lo = min(w, 0), hi = max(w, 0), s = (hi - lo) / 15, z = rint(-lo / s); s is rounded to
+ * dtype before it is used, q = rint(w / s) + z held to 0..15, ties to even.  A group whose scale
+ * rounds to zero becomes zeros, one with an infinity or a NaN becomes NaN. */
+int mmbo_w4_quantize(int dtype, size_t m, size_t k, int group, int zeros, const void* W, size_t ldw,
+                     void* packed, void* stream);
+/* Packs codes that exist already: two a byte, the even column in the low half, rows ldcodes bytes
+ * apart (>= (k + 1) / 2); scales(i,g) = scales[i * ldscales + g] in dtype; zeroPoints(i,g) =
+ * zeroPoints[i * ldzeros + g], one a byte, 0..15, or NULL (the result then has zeros = 0). */
+int mmbo_w4_pack(int dtype, size_t m, size_t k, int group, const unsigned char* codes, size_t ldcodes,
+                 const void* scales, size_t ldscales, const unsigned char* zeroPoints, size_t ldzeros,
+                 void* packed, void* stream);
+/* The weights that a packed matrix stands for, rounded to dtype (W laid out as for quantize). */
+int mmbo_w4_unpack(int dtype, size_t m, size_t k, int group, int zeros, const void* packed, void* W,
+                   size_t ldw, void* stream);
+
+/* C = alpha * W * B + beta * C with W packed, B k x n (ldb >= k), C m x n (ldc >= m), any n: one
+ * token's vector, a decoding batch, a prompt.  Codes enter the products as exact integers and each
+ * group's sum is scaled in fp32, so the result differs from the formula by fp32 summation and the
+ * final rounding only.  C must not overlap B or packed. */
+int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, const float* alpha, const void* packed,
+                 int group, int zeros, const void* B, size_t ldb, const float* beta, void* C, size_t ldc,
+                 void* stream);
+
+/* A whole mixture-of-experts layer for a few tokens.  X is d x tokens, Y d x tokens, router d x
+ * experts (ldr >= d: expert e's vector is contiguous).  Per token t:
+ *   p = softmax(router^T x);  the topk experts of largest p, the lower number first among equals
+ *   (a NaN counts as largest);  g_e = p_e, divided by the sum over the chosen ones if renorm = 1;
+ *   y = sum g_e * down_e * (silu(gate_e x) o (up_e x)) + beta * y.
+ * gate_e and up_e are f x d, down_e is d x f, stored like W above.  group = 0: 16-bit experts, row i
+ * of gate_e at gate + e * strideG + i * ldg elements (ldg >= d; up the same), of down_e at
+ * down + e * strideD + i * ldd (ldd >= f).  group != 0: packed experts (the format above), expert e
+ * at e * strideG (strideD) BYTES, multiples of 16; ldg and ldd are not used.
+ * ids (tokens x topk, int) and gates (tokens x topk, float) receive the choice and may be NULL.
+ * tokens <= MMBO_MOE_MAX_TOKENS, topk <= MMBO_MOE_MAX_TOPK, experts <= MMBO_MOE_MAX_EXPERTS, d and f
+ * <= MMBO_MOE_MAX_WIDTH.  workspace: 256-byte aligned device memory of at least
+ * mmbo_moe_workspace_bytes; its contents need no initial value and are free to reuse once the stream
+ * has passed the call; two calls that may run at the same time, two captured graphs among them, need
+ * a workspace each.  Y may not overlap X. */
+#define MMBO_MOE_MAX_TOKENS 256
+#define MMBO_MOE_MAX_TOPK 32
+#define MMBO_MOE_MAX_EXPERTS 1024
+#define MMBO_MOE_MAX_WIDTH 65536
+int mmbo_moe_workspace_bytes(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_t topk,
+                             size_t* bytes);
+int mmbo_moe(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_t topk, int renorm,
+             int group, int zeros, const void* X, size_t ldx, const void* router, size_t ldr,
+             const void* gate, const void* up, size_t ldg, size_t strideG, const void* down, size_t ldd,
+             size_t strideD, const float* beta, void* Y, size_t ldy, int* ids, float* gates,
+             void* workspace, size_t workspaceBytes, void* stream);
 
 /* Self-test of the time-out path every barrier wait in the tensor-core kernels has:
  * launches one thread that waits, for at most limit_ns (<= 1 s), on a barrier nothing
