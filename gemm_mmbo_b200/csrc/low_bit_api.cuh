@@ -4,6 +4,7 @@
 
 #include "moe.cuh"
 #include "w4.cuh"
+#include "w4_gemv.cuh"
 
 namespace mmbo {
 
@@ -29,9 +30,147 @@ static int w4_tile_grid(size_t m, size_t k, unsigned* grid) {
   return MMBO_OK;
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per device.
+template <typename K>
+static int allow_smem(K kernel, size_t bytes, bool (&done)[kMaxDevices]) {
+  const int dev = current_device();
+  if (dev < 0 || dev >= kMaxDevices) return MMBO_ERR_TOO_LARGE;
+  if (done[dev]) return MMBO_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  done[dev] = e == cudaSuccess;
+  return (int)e;
+}
+
+// Blocks of w4_gemv_kernel (one per SM) that clusters of 1 << log2 fill at once: less than all SMs where a cluster's
+// blocks must share a group of SMs whose number is no multiple of theirs.
+static int g_gemv_clusters[kMaxDevices][3];
+
+template <typename K>
+static int gemv_clusters(K kernel, int split_log2) {
+  const int dev = current_device();
+  if (split_log2 == 0 || dev < 0 || dev >= kMaxDevices) return sm_count() >> split_log2;
+  int& known = g_gemv_clusters[dev][split_log2];
+  if (known == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(1 << split_log2));
+    cfg.blockDim = dim3(kGemvThreads);
+    cfg.dynamicSmemBytes = 128 * 1024;  // more than half an SM's: one block each
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << split_log2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int fit = 0;
+    if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess || fit <= 0) {
+      cudaGetLastError();
+      fit = (sm_count() >> split_log2) * 7 / 8;
+    }
+    known = fit < (sm_count() >> split_log2) ? fit : sm_count() >> split_log2;
+  }
+  return known;
+}
+
+constexpr size_t kGemvSmem = 227 * 1024 - 4096;  // of an SM's shared memory, less the kernel's static part
+
+// How w4_gemv_kernel cuts a problem: the cheapest of all (warps along k, blocks along k), by a sum of what was measured
+// (B200, us): 0.022 a tile of the busiest SM (0.035 with 9 columns and more, whose products take as long again), 0.3 a
+// slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join clusters of two / four.  8192 x 28672, one
+// column: 28.4 us with the chosen 16 x 2, 30.7 with 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
+template <int NT, int QG>
+static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3], size_t* smem) {
+  const size_t k_tiles = w4_k_tiles(a.k), blocks = w4_row_blocks(a.m);
+  double best = 1e30;
+  for (int wk_log2 = 0; wk_log2 <= 4; ++wk_log2)
+    for (int split_log2 = 0; split_log2 <= 2; ++split_log2) {
+      const size_t wk = (size_t)1 << wk_log2, split = (size_t)1 << split_log2, wm = kGemvWarps / wk;
+      if (split > 1 && k_tiles < split) continue;
+      const size_t groups = (blocks + wm - 1) / wm, span = (k_tiles + split - 1) / split, part = (span + wk - 1) / wk;
+      const size_t cl = groups < (size_t)clusters[split_log2] ? groups : (size_t)clusters[split_log2];
+      const size_t rounds = (groups + cl - 1) / cl;
+      const int slot_tiles = part < 4 ? (int)(part ? part : 1) : 4;
+      const size_t ring = (size_t)kGemvWarps * 2 * slot_tiles * tile_bytes;
+      const size_t one = gemv_sums_bytes((int)wk, (int)split, a.n, 1);
+      if (ring + one + gemv_x_bytes(a.n, 1, NT, 4 / QG) > kGemvSmem) continue;
+      size_t x_tiles = (kGemvSmem - ring - one - a.n * 64) / (a.n * 256 + (size_t)(4 / QG) * NT * 32);
+      if (x_tiles > span) x_tiles = span ? span : 1;
+      if (x_tiles == 0) continue;
+      const size_t x = gemv_x_bytes(a.n, x_tiles, NT, 4 / QG);
+      size_t batch = (kGemvSmem - ring - x) / one;
+      if (batch > rounds) batch = rounds;
+      if (batch == 0 || (split > 1 && batch < rounds)) continue;
+      const size_t batches = (rounds + batch - 1) / batch;
+      const double staged = (double)a.n * span * 0.25 * (x_tiles < span ? batches : 1);
+      const double cost = rounds * wm * span * (NT > 1 ? 0.035 : 0.022) + rounds * ((part + slot_tiles - 1) / slot_tiles) * 0.3 +
+                          staged * 0.05 + (split == 1 ? 0.0 : split == 2 ? 1.8 : 2.5) + (batches - 1) * 1.0;
+      if (cost < best) {
+        best = cost;
+        a.wk_log2 = wk_log2;
+        a.split_log2 = split_log2;
+        a.slots = 2;
+        a.slot_tiles = slot_tiles;
+        a.x_tiles = (int)x_tiles;
+        a.batch = (int)batch;
+        a.clusters = (int)cl;
+        *smem = ring + x + gemv_sums_bytes((int)wk, (int)split, a.n, (int)batch);
+      }
+    }
+  return best < 1e30;
+}
+
+template <typename T, int NT, int QG, bool ZEROS>
+static int launch_w4_gemv(GemvArgs a, cudaStream_t st) {
+  auto kernel = w4_gemv_kernel<T, NT, QG, ZEROS>;
+  static bool prepared[kMaxDevices];
+  int rc = allow_smem(kernel, kGemvSmem, prepared);
+  if (rc) return rc;
+  const int clusters[3] = {gemv_clusters(kernel, 0), gemv_clusters(kernel, 1), gemv_clusters(kernel, 2)};
+  size_t smem = 0;
+  if (!plan_gemv<NT, QG>(a, W4Tile<QG, ZEROS>::kBytes, clusters, &smem)) return MMBO_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.clusters << a.split_log2);
+  cfg.blockDim = dim3(kGemvThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (a.split_log2) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1u << a.split_log2;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (settings().pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  MMBO_COUNT_LAUNCH();
+  return (int)e;
+}
+
+template <typename T, int NT>
+static int dispatch_w4_gemv(const GemvArgs& a, W4Format f, cudaStream_t st) {
+  switch (f.group * 2 + f.zeros) {
+    case 64: return launch_w4_gemv<T, NT, 1, false>(a, st);
+    case 65: return launch_w4_gemv<T, NT, 1, true>(a, st);
+    case 128: return launch_w4_gemv<T, NT, 2, false>(a, st);
+    case 129: return launch_w4_gemv<T, NT, 2, true>(a, st);
+    case 256: return launch_w4_gemv<T, NT, 4, false>(a, st);
+    default: return launch_w4_gemv<T, NT, 4, true>(a, st);
+  }
+}
+
 template <typename T>
 static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* packed, W4Format f, const void* B,
                        size_t ldb, float beta, void* C, size_t ldc, cudaStream_t st) {
+  if (n <= 16) {
+    const GemvArgs a{m, n, k, ldb, ldc, alpha, beta, static_cast<const unsigned char*>(packed), B, C};
+    return n <= 8 ? dispatch_w4_gemv<T, 1>(a, f, st) : dispatch_w4_gemv<T, 2>(a, f, st);
+  }
   const dim3 grid((unsigned)((m + 7) / 8), (unsigned)(n < 65535 ? n : 65535));
   w4_gemm_simple_kernel<T><<<grid, 256, 0, st>>>(m, n, k, alpha, static_cast<const unsigned char*>(packed), f,
                                                  static_cast<const T*>(B), ldb, beta, static_cast<T*>(C), ldc);

@@ -8,12 +8,14 @@
 // another, so that whoever walks along k reads one contiguous stream.  A tile is
 //     1024 bytes of codes          row r (0..15) at 64 r; within a row, 16 bytes for each of four "lanes" t, holding one
 //                                  32-bit word for each quarter u of the tile: the columns 32 u + 8 t .. + 7
-//     (128 / group) x 16 scales    in the activations' type, group by group, row by row
-//     (128 / group) x 16 bytes     zero points, where the matrix has them
-// In a word, column j of its eight sits in nibble (j >> 1) + 4 (j & 1): `(w >> 4 p) & 0x000f000f` is the pair
-// (2p, 2p + 1) in the two halves of a register, ready to become two 16-bit floats.  With this order the four words of
-// a lane are the four k-steps a 16-row matrix instruction wants from that lane, one 16-byte load serves a whole tile
-// row, and no k-step spans two groups (groups are 32, 64 or 128 wide).
+//     (128 / group) x 16 scales    in the activations' type, group by group, rows in the order 0, 8, 1, 9, .. 7, 15
+//     (128 / group) x 16 bytes     zero points in the same order, where the matrix has them
+// In a word, columns 0 .. 7 sit in nibbles 0, 4, 2, 6, 1, 5, 3, 7: with v = w >> 8, the registers w & 0x000f000f,
+// v & 0x000f000f, w & 0x00f000f0 and v & 0x00f000f0 hold the pairs (0, 1), (2, 3), (4, 5), (6, 7), one code in each half,
+// ready to be read as two 16-bit floats.  With this order the four words of
+// a lane are the four pairs of k-steps a 16-row matrix instruction wants from that lane, one 16-byte load serves a
+// whole tile row, no k-step spans two groups (groups are 32, 64 or 128 wide), and the scales of the two rows r and
+// r + 8 whose sums a lane holds come with one load.
 // Rows past m and columns past k hold the code of weight zero.
 #pragma once
 
@@ -34,7 +36,14 @@ struct W4Format {
   int group, zeros;
   __host__ __device__ int groups() const { return kW4Cols / group; }
   __host__ __device__ uint32_t tile_bytes() const { return kW4Codes + groups() * (kW4Rows * 2 + (zeros ? kW4Rows : 0)); }
+  // places of the scale and the zero point of row r, group g within a tile
+  __host__ __device__ uint32_t scale_at(int g, int r) const { return kW4Codes + (g * kW4Rows + slot(r)) * 2; }
+  __host__ __device__ uint32_t zero_at(int g, int r) const { return kW4Codes + groups() * kW4Rows * 2 + g * kW4Rows + slot(r); }
+  __host__ __device__ static int slot(int r) { return 2 * (r & 7) + (r >> 3); }
 };
+__host__ __device__ constexpr int w4_nibble(int column) {  // of one of a word's eight columns
+  return (column >> 2) + 2 * ((column >> 1) & 1) + 4 * (column & 1);
+}
 __host__ __device__ inline size_t w4_row_blocks(size_t m) { return (m + kW4Rows - 1) / kW4Rows; }
 __host__ __device__ inline size_t w4_k_tiles(size_t k) { return (k + kW4Cols - 1) / kW4Cols; }
 
@@ -132,12 +141,12 @@ __global__ void w4_quantize_kernel(size_t m, size_t k, W4Format f, const T* __re
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float q = live ? fminf(fmaxf(rintf(to_f32(w[u][e]) / s) + z, 0.f), 15.f) : z;
-        word[u] |= (uint32_t)q << (4 * ((e >> 1) + 4 * (e & 1)));
+        word[u] |= (uint32_t)q << (4 * w4_nibble(e));
       }
       if (t == 0 && u % per == 0) {
         const int g = u / per;
-        reinterpret_cast<T*>(out + kW4Codes)[g * kW4Rows + row] = from_f32<T>(s);
-        if (f.zeros) out[kW4Codes + f.groups() * kW4Rows * 2 + g * kW4Rows + row] = (unsigned char)z;
+        *reinterpret_cast<T*>(out + f.scale_at(g, row)) = from_f32<T>(s);
+        if (f.zeros) out[f.zero_at(g, row)] = (unsigned char)z;
       }
     }
     *reinterpret_cast<uint4*>(out + row * 64 + t * 16) = make_uint4(word[0], word[1], word[2], word[3]);
@@ -178,12 +187,12 @@ __global__ void w4_pack_kernel(size_t m, size_t k, W4Format f, const unsigned ch
           const uint32_t byte = codes[i * ldcodes + j / 2];
           q = (j & 1) ? byte >> 4 : byte & 15u;
         }
-        word[u] |= q << (4 * ((e >> 1) + 4 * (e & 1)));
+        word[u] |= q << (4 * w4_nibble(e));
       }
       if (t == 0 && u % per == 0) {
         const int gt = u / per;
-        reinterpret_cast<T*>(out + kW4Codes)[gt * kW4Rows + row] = have ? scales[i * lds + g] : from_f32<T>(0.f);
-        if (f.zeros) out[kW4Codes + f.groups() * kW4Rows * 2 + gt * kW4Rows + row] = (unsigned char)z;
+        *reinterpret_cast<T*>(out + f.scale_at(gt, row)) = have ? scales[i * lds + g] : from_f32<T>(0.f);
+        if (f.zeros) out[f.zero_at(gt, row)] = (unsigned char)z;
       }
     }
     *reinterpret_cast<uint4*>(out + row * 64 + t * 16) = make_uint4(word[0], word[1], word[2], word[3]);
@@ -215,12 +224,12 @@ __global__ void w4_unpack_kernel(size_t m, size_t k, W4Format f, const unsigned 
       const size_t j = tile * kW4Cols + 32 * u + 8 * t;
       if (j >= k) continue;
       const int g = u / per;
-      const float s = to_f32(reinterpret_cast<const T*>(in + kW4Codes)[g * kW4Rows + row]);
-      const int z = f.zeros ? in[kW4Codes + f.groups() * kW4Rows * 2 + g * kW4Rows + row] : 8;
+      const float s = to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row)));
+      const int z = f.zeros ? in[f.zero_at(g, row)] : 8;
       T v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        v[e] = from_f32<T>((float)((int)((word[u] >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - z) * s);
+        v[e] = from_f32<T>((float)((int)((word[u] >> (4 * w4_nibble(e))) & 15u) - z) * s);
       T* dst = W + i * ldw + j;
       if (vec && j + 8 <= k) {
         *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
@@ -245,13 +254,13 @@ __device__ __forceinline__ float w4_row_dot(const unsigned char* __restrict__ pa
   for (size_t tile = half; tile < tiles; tile += 2) {
     const unsigned char* in = packed + (i / kW4Rows * tiles + tile) * f.tile_bytes();
     const uint32_t w = __ldg(reinterpret_cast<const unsigned int*>(in + row * 64 + t * 16 + u * 4));
-    const float s = to_f32(reinterpret_cast<const T*>(in + kW4Codes)[g * kW4Rows + row]);
-    const int z = f.zeros ? in[kW4Codes + f.groups() * kW4Rows * 2 + g * kW4Rows + row] : 8;
+    const float s = to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row)));
+    const int z = f.zeros ? in[f.zero_at(g, row)] : 8;
     float part = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const size_t j = tile * kW4Cols + 32 * u + 8 * t + e;
-      if (j < k) part = fmaf((float)((int)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - z), to_f32(x[j]), part);
+      if (j < k) part = fmaf((float)((int)((w >> (4 * w4_nibble(e))) & 15u) - z), to_f32(x[j]), part);
     }
     acc = fmaf(s, part, acc);
   }

@@ -1,0 +1,557 @@
+// Packed 4-bit weights times up to 16 columns of activations.
+//
+// What bounds it: the codes, read once (0.53 bytes a weight); for small matrices the latency of one trip to memory.
+//   - Every multiplying warp has a ring of tiles in shared memory, which a lane of the feeding warp fills with bulk
+//     copies: the copies in flight cost no registers and no instructions of the warps that multiply.  (With each warp
+//     filling its own ring the copies' issue cost 500 cycles a slot: 32 instead of 27 us at 8192 x 28672, one column.)
+//   - One block per SM, persistent over its row blocks, so the rings run on from one to the next.
+//   - The activations of the block's share of k sit in shared memory, staged once.
+//   - Each warp keeps its partial sums of every row block in shared memory; they are joined at the end, over the warps
+//     that split k within a block and over the blocks of a cluster (distributed shared memory), in a fixed order: the
+//     same bits every time, and no scratch memory.
+//   - Before it waits for the kernel in front of it the feeding warp asks L2 for its first tiles.
+// The products run on mma.sync.m16n8k16: with at most 16 columns its rate is ample (a tile takes 8 or 16 instructions of
+// 8 cycles, on four schedulers, in the 45 cycles its bytes take), and its fragments come straight from the packed order
+// without a trip through tensor memory.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+#include "ptx.cuh"
+#include "w4.cuh"
+
+namespace mmbo {
+
+constexpr uint32_t kLowCodes = 0x000f000fu, kHighCodes = 0x00f000f0u;
+
+// c (16 x 8) = a (16 x 16) * b (16 x 8) + c (or + 0), fp32 sums.
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_from_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                  uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
+// Two 16-bit floats (as stored, low half first) widened.
+template <typename T>
+__device__ __forceinline__ float2 widen2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 widen2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+template <>
+__device__ __forceinline__ float2 widen2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// Tile layout known at compile time.
+template <int QG, bool ZEROS>
+struct W4Tile {
+  static constexpr int kGroups = 4 / QG;  // QG: quarters of 32 columns in a group
+  static constexpr int kScales = kW4Codes, kZeros = kW4Codes + kGroups * kW4Rows * 2;
+  static constexpr int kBytes = kZeros + (ZEROS ? kGroups * kW4Rows : 0);
+};
+
+// acc[nt] += the products of a tile with 128 rows of 8 NT staged columns: x[nt] is this lane's place in them, `xsum` its
+// place in their group sums (shared memory addresses).  Sums are in units of 2^20.
+//
+// A code is used as the bits of a half-precision number: q in the lowest four bits is the subnormal q 2^-24, q in the
+// next four is q 2^-20, both exact, so a word becomes four operand registers with a shift and four masks.  The two kinds
+// have a sum each, and the zero point comes off once a group:  sum (q - z) x = sum q x - z sum x.  (Forming the sums of
+// x with the same instruction and a matrix of ones made the tensor pipe the bound: 16 instructions a tile, 32 cycles;
+// subtracting the zero point from each code costs as much again as unpacking it.)
+template <typename T, int NT, int QG, bool ZEROS>
+__device__ __forceinline__ void w4_tile_mma(uint32_t tile, const uint32_t (&x)[NT], uint32_t xsum, float (&acc)[NT][4]) {
+  using L = W4Tile<QG, ZEROS>;
+  const int lane = threadIdx.x & 31, r = lane >> 2;
+  const uint4 c0 = lds128(tile + lane * 16), c1 = lds128(tile + lane * 16 + 512);  // rows r and r + 8
+  const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+  for (int g = 0; g < L::kGroups; ++g) {
+    float low[NT][4], high[NT][4];
+#pragma unroll
+    for (int qq = 0; qq < QG; ++qq) {
+      const int q = g * QG + qq;
+      const uint32_t v0 = w0[q] >> 8, v1 = w1[q] >> 8;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint4 b = lds128(x[nt] + q * 64);
+        if (qq == 0) {
+          mma_f16_from_zero(low[nt], w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
+          mma_f16_from_zero(high[nt], w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
+        } else {
+          mma_f16(low[nt], w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
+          mma_f16(high[nt], w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
+        }
+      }
+    }
+    const float2 s = widen2<T>(lds32(tile + L::kScales + g * 32 + r * 4));
+    float z0 = 8.f, z1 = 8.f;
+    if (ZEROS) {
+      const uint32_t z = lds16(tile + L::kZeros + g * 16 + r * 2);
+      z0 = (float)(z & 15u);
+      z1 = (float)((z >> 8) & 15u);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float2 xs = lds_f2(xsum + (g * NT + nt) * 32);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float dot = fmaf(16.f, low[nt][i], high[nt][i]);
+        acc[nt][i] = fmaf(i < 2 ? s.x : s.y, fmaf(i < 2 ? -z0 : -z1, i & 1 ? xs.y : xs.x, dot), acc[nt][i]);
+      }
+    }
+  }
+}
+
+constexpr int kGemvWarps = 16;                       // that multiply
+constexpr int kGemvThreads = (kGemvWarps + 1) * 32;  // and one that feeds them
+constexpr int kGemvMaxSlots = 4;
+// Barrier of the multiplying warps.
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kGemvWarps * 32) : "memory"); }
+
+// What w4_tile_mma reads: `n` columns of `tiles` k-tiles in half precision and the sums of every group in the codes' units
+// of 2^-20.  Half-precision columns are used as they came.  A bfloat16 column is scaled by the power of two that brings
+// its largest magnitude into [2^14, 2^15); this is exact but for elements 2^-38 of that magnitude and less, whose
+// rounding is far below the last bit of any fp32 sum they enter, and one tile product serves both types.  The sums get
+// their true size again by two factors a column; those of a bfloat16 column with an infinity or a NaN are NaN, so that
+// they are noticed.
+//   xs: the columns as they came, x_stride bytes apart; sums: [tile][group][8 NT] floats; peak: bits of the largest
+//   magnitudes (bfloat16), zero before the call.
+template <typename T, int NT, int QG>
+__device__ __forceinline__ void w4_stage(int n, int tiles, unsigned char* xs, uint32_t x_stride, float* sums,
+                                         uint32_t* peak, float2* undo) {
+  constexpr bool kScale = !std::is_same<T, __half>::value;
+  constexpr int kLanes = 4 * QG;  // pieces of 16 bytes in a group, held by as many neighbouring lanes
+  const int pieces = tiles * 16, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int strips = (pieces + 63) / 64;  // a warp takes 64 pieces of a column at a time
+  if (kScale) {
+    for (int i = warp; i < strips * n; i += kGemvWarps) {
+      const int col = i / strips, piece = i % strips * 64 + lane;
+      uint32_t top = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (piece + 32 * h < pieces) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(xs + col * x_stride + (piece + 32 * h) * 16);
+          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = max(top, max(w[j] << 16 & 0x7fffffffu, w[j] & 0x7fff0000u));
+        }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) atomicMax(&peak[col], top);
+    }
+    workers_sync();
+  }
+  for (int i = warp; i < strips * n; i += kGemvWarps) {
+    const int col = i / strips, first = i % strips * 64 + lane;
+    float f1 = 1.f, f2 = 1.f;
+    if (kScale) {
+      // exponent of the largest magnitude (below the normal range: the smallest normal one), 2^(14 - e) as a product
+      const uint32_t top = peak[col];
+      const int up = 14 - ((int)max(top >> 23, 1u) - 127), up1 = min(max(up, -100), 100), up2 = up - up1;
+      f1 = __uint_as_float((uint32_t)(up1 + 127) << 23);
+      f2 = __uint_as_float((uint32_t)(up2 + 127) << 23);
+      if (i % strips == 0 && lane == 0)
+        undo[col] = top < 0x7f800000u ? make_float2(__uint_as_float((uint32_t)(127 - up1) << 23),
+                                                    __uint_as_float((uint32_t)(127 - up2 + 20) << 23))
+                                      : make_float2(__int_as_float(0x7fc00000), 0.f);
+    }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int piece = first + 32 * h;
+      if (piece < pieces) {
+        uint4* at = reinterpret_cast<uint4*>(xs + col * x_stride + piece * 16);
+        const uint4 raw = *at;
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t out[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float2 v = widen2<T>(w[j]);
+          if (kScale) {
+            const __half2 h2 = __floats2half2_rn(v.x * f1 * f2, v.y * f1 * f2);
+            out[j] = *reinterpret_cast<const uint32_t*>(&h2);
+            v = __half22float2(h2);
+          }
+          sum[h] += v.x + v.y;
+        }
+        if (kScale) *at = make_uint4(out[0], out[1], out[2], out[3]);
+      }
+    }
+#pragma unroll
+    for (int x = 1; x < kLanes; x <<= 1) {
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], x);
+      sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], x);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int piece = first + 32 * h;
+      if (piece < pieces && (piece & (kLanes - 1)) == 0) sums[piece / kLanes * 8 * NT + col] = sum[h] * 0x1p-20f;
+    }
+  }
+  workers_sync();
+}
+
+// Sum over k of row i times the column x, element by element.
+template <typename T>
+__device__ __noinline__ float w4_slow_dot(const unsigned char* __restrict__ packed, W4Format f, size_t i, size_t k,
+                                          const T* __restrict__ x) {
+  const size_t tiles = w4_k_tiles(k);
+  const int row = (int)(i % kW4Rows);
+  float acc = 0.f;
+  for (size_t j = 0; j < k; ++j) {
+    const unsigned char* in = packed + (i / kW4Rows * tiles + j / kW4Cols) * f.tile_bytes();
+    const int c = (int)(j % kW4Cols), g = c / f.group;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(in + row * 64 + c % 32 / 8 * 16 + c / 32 * 4);
+    const int q = (w >> (4 * w4_nibble(c % 8))) & 15u, z = f.zeros ? in[f.zero_at(g, row)] : 8;
+    acc = fmaf((float)(q - z) * to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row))), to_f32(x[j]), acc);
+  }
+  return acc;
+}
+
+// Untiled bulk copy, completion on an mbarrier of this CTA (addresses and size multiples of 16 bytes), and the request
+// to have the bytes brought into L2.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_prefetch(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
+// Bounded wait by a whole warp that sleeps in the barrier unit instead of polling: the polls of waiting warps would cost
+// the working ones issue slots.  200 tries of at most 10 ms each.
+__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                 unsigned int fault_code, unsigned int detail) {
+#pragma unroll 1
+  for (int i = 0; i < 200; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(10000000u)
+        : "memory");
+    if (done) return true;
+    if (*abort_flag) return false;
+  }
+  report_fault(fault_code, detail);
+  *abort_flag = 1u;
+  return false;
+}
+
+// Cluster barrier in its two halves, and a store to the same place in another block's shared memory.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(addr, rank)), "f"(v) : "memory");
+}
+
+// How the work is cut.  The multiplying warps are WM x WK: warp w takes the rows of row block w / WK and the (w % WK)-th
+// part of the block's k-tiles.  `split` blocks of a cluster share one set of rows and cut k; a cluster works through row
+// groups of WM row blocks: cluster_id, cluster_id + clusters, ...
+struct GemvArgs {
+  size_t m, n, k, ldb, ldc;
+  float alpha, beta;
+  const unsigned char* packed;
+  const void* B;
+  void* C;
+  int wk_log2;     // warps that cut k
+  int split_log2;  // blocks of a cluster
+  int slots;       // slots of a warp's ring
+  int slot_tiles;  // consecutive k-tiles in a slot
+  int x_tiles;     // k-tiles of activations in shared memory at a time
+  int batch;       // row groups whose partial sums are kept before they are joined and stored (split > 1: all)
+  int clusters;
+};
+
+// Staged columns with their group sums (nt: blocks of 8 columns, groups: in a tile).
+__host__ __device__ inline size_t gemv_x_bytes(size_t n, size_t tiles, int nt, int groups) {
+  return n * (tiles * 256 + 64) + tiles * groups * nt * 32;
+}
+// Partial sums of a batch of row groups, and the room for what the other blocks of a cluster hand over.
+__host__ __device__ inline size_t gemv_sums_bytes(int wk, int split, size_t n, int batch) {
+  const size_t out = (size_t)batch * (kGemvWarps / wk) * kW4Rows * n;
+  return (out * wk + (split > 1 ? out : 0)) * 4;
+}
+
+template <typename T, int NT, int QG, bool ZEROS>
+__global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs a) {
+  constexpr uint32_t TILE = W4Tile<QG, ZEROS>::kBytes;
+  constexpr bool kScale = !std::is_same<T, __half>::value;
+  constexpr int G = 4 / QG, kWorkers = kGemvWarps * 32;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) unsigned long long full_bars[kGemvWarps * kGemvMaxSlots], empty_bars[kGemvWarps * kGemvMaxSlots];
+  __shared__ __align__(8) unsigned long long x_bar;
+  __shared__ uint32_t abort_flag;
+  __shared__ uint32_t peak[8 * NT];
+  __shared__ float2 undo[8 * NT];
+  const int split = 1 << a.split_log2, rank = blockIdx.x & (split - 1), first = blockIdx.x >> a.split_log2;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int WK = 1 << a.wk_log2, WM = kGemvWarps >> a.wk_log2;
+  const int k_tiles = (int)w4_k_tiles(a.k), row_blocks = (int)w4_row_blocks(a.m), n = (int)a.n;
+  const int t0 = (int)(((long long)k_tiles * rank) >> a.split_log2);
+  const int span = (int)(((long long)k_tiles * (rank + 1)) >> a.split_log2) - t0;
+  const int groups = (row_blocks + WM - 1) / WM;
+  const int mine = first < groups ? (groups - first + a.clusters - 1) / a.clusters : 0;  // row groups of this cluster
+
+  // shared memory: rings | activations | their group sums | partial sums | sums from the cluster
+  const uint32_t slot_bytes = a.slot_tiles * TILE;
+  unsigned char* xs = smem + (size_t)kGemvWarps * a.slots * slot_bytes;
+  const uint32_t x_stride = a.x_tiles * 256 + 64;  // columns 64 bytes out of step: conflict-free 16-byte reads
+  float* xsums = reinterpret_cast<float*>(xs + (size_t)n * x_stride);
+  float* sums = xsums + a.x_tiles * G * 8 * NT;
+  float* received = sums + (size_t)a.batch * kGemvWarps * kW4Rows * n;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mbar_init(smem_u32(&x_bar), 1);
+  }
+  if (threadIdx.x < kGemvWarps * kGemvMaxSlots) {
+    mbar_init(smem_u32(&full_bars[threadIdx.x]), 1);
+    mbar_init(smem_u32(&empty_bars[threadIdx.x]), 1);
+  }
+  fence_mbar_init();
+
+  // A warp's part of the tiles of a chunk, and its weights for a row group.
+  auto part_of = [&](int chunk, int which) {
+    return chunk + (int)(((long long)min(a.x_tiles, span - chunk) * which) >> a.wk_log2);
+  };
+  auto weights_of = [&](int g, int wm, int tile) {
+    return a.packed + ((size_t)((first + g * a.clusters) * WM + wm) * k_tiles + t0 + tile) * TILE;
+  };
+  // Lane w of the last warp serves warp w.
+  const int serves = warp == kGemvWarps ? min(lane, kGemvWarps - 1) : warp, wk = serves & (WK - 1), wm = serves >> a.wk_log2;
+  if (warp == kGemvWarps && lane < kGemvWarps && mine > 0 && first * WM + wm < row_blocks) {
+    const int begin = part_of(0, wk), cnt = min(part_of(0, wk + 1) - begin, a.slots * a.slot_tiles);
+    if (cnt > 0) bulk_prefetch(weights_of(0, wm, begin), cnt * TILE);
+  }
+  __syncthreads();
+  if (split > 1) cluster_arrive();
+  griddep_launch_dependents();
+  griddep_wait();
+
+  // Activations of a chunk of k: requested before the weights, so that they do not queue behind them.
+  const bool x_bulk = a.ldb % 8 == 0 && a.k % 8 == 0 && (reinterpret_cast<uintptr_t>(a.B) & 15u) == 0;
+  uint32_t x_phase = 0;
+  auto request_x = [&](int chunk0) {
+    const size_t k0 = (size_t)(t0 + chunk0) * kW4Cols;
+    const int tiles = min(span - chunk0, a.x_tiles);
+    const int real = (int)min((size_t)tiles * kW4Cols, a.k - min(a.k, k0));  // elements of a column that exist
+    if (kScale && threadIdx.x < n) peak[threadIdx.x] = 0;
+    if (x_bulk) {
+      if (threadIdx.x == 0) {
+        mbar_expect_tx(smem_u32(&x_bar), n * real * 2);
+        if (real > 0)
+          for (int col = 0; col < n; ++col)
+            bulk_load(smem_u32(xs) + col * x_stride, static_cast<const T*>(a.B) + col * a.ldb + k0, real * 2,
+                      smem_u32(&x_bar));
+      }
+      const int fill = tiles * 16 - real / 8;  // pieces behind k
+      for (int i = threadIdx.x; i < fill * n; i += kWorkers)
+        *reinterpret_cast<uint4*>(xs + i / fill * x_stride + real * 2 + i % fill * 16) = make_uint4(0, 0, 0, 0);
+    } else {
+      const int pieces = tiles * 16;
+#pragma unroll 2
+      for (int i = threadIdx.x; i < pieces * n; i += kWorkers) {
+        const int col = i / pieces, piece = i % pieces;
+        __align__(16) T v[8];
+        load8(static_cast<const T*>(a.B) + col * a.ldb + k0 + piece * 8, (long long)real - piece * 8, false, v);
+        *reinterpret_cast<uint4*>(xs + col * x_stride + piece * 16) = *reinterpret_cast<const uint4*>(v);
+      }
+    }
+  };
+  if (warp < kGemvWarps) request_x(0);
+
+  const uint32_t full0 = smem_u32(&full_bars[serves * kGemvMaxSlots]), empty0 = smem_u32(&empty_bars[serves * kGemvMaxSlots]);
+  const uint32_t ring_at = smem_u32(smem) + serves * a.slots * slot_bytes;
+  int slot = 0;
+  uint32_t phase = 0;
+  if (warp == kGemvWarps) {
+    // For each batch of row groups, for each chunk of k, for each row group: the served warp's part of the chunk in
+    // pieces of slot_tiles.  This warp takes no part in the barriers of the others.
+    uint32_t idle = 0;
+    for (int batch0 = 0; batch0 < mine && lane < kGemvWarps; batch0 += a.batch) {
+      for (int chunk0 = 0; chunk0 < span; chunk0 += a.x_tiles) {
+        const int begin = part_of(chunk0, wk), end = part_of(chunk0, wk + 1);
+        for (int g = batch0; g < min(mine, batch0 + a.batch); ++g) {
+          const bool have = (first + g * a.clusters) * WM + wm < row_blocks;
+          const unsigned char* src = weights_of(g, wm, begin);
+          for (int tile = begin; tile < end;) {
+            if (!mbar_try_wait(empty0 + slot * 8, phase ^ 1u)) {
+              if (*(volatile uint32_t*)&abort_flag || ++idle > (1u << 24)) break;  // the others report
+              continue;
+            }
+            const int cnt = min(a.slot_tiles, end - tile);
+            mbar_expect_tx(full0 + slot * 8, have ? cnt * TILE : 0);
+            if (have) bulk_load(ring_at + slot * slot_bytes, src, cnt * TILE, full0 + slot * 8);
+            src += cnt * TILE;
+            tile += cnt;
+            if (++slot == a.slots) {
+              slot = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (split > 1) cluster_wait();
+    return;
+  }
+
+  bool ok = true;
+  uint32_t xl[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)  // columns past n repeat the last one; their sums are not stored
+    xl[nt] = smem_u32(xs) + min(nt * 8 + r, n - 1) * x_stride + t * 16;
+  for (int batch0 = 0; batch0 < mine; batch0 += a.batch) {
+    const int batch_end = min(mine, batch0 + a.batch);
+    for (int chunk0 = 0; chunk0 < span || chunk0 == 0; chunk0 += a.x_tiles) {
+      if (span > a.x_tiles || batch0 == 0) {
+        if (batch0 + chunk0 > 0) {
+          workers_sync();
+          request_x(chunk0);
+        }
+        if (x_bulk && ok) ok = mbar_wait_asleep(smem_u32(&x_bar), x_phase, &abort_flag, kFaultWaitCLoad, 0x4b10u);
+        x_phase ^= 1u;
+        workers_sync();
+        w4_stage<T, NT, QG>(n, min(span - chunk0, a.x_tiles), xs, x_stride, xsums, peak, undo);
+      }
+      const int w0 = part_of(chunk0, wk), w1 = part_of(chunk0, wk + 1);
+      for (int g = batch0; g < batch_end; ++g) {
+        float acc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
+        for (int tile = w0; tile < w1; tile += a.slot_tiles) {
+          if (ok) ok = mbar_wait_asleep(full0 + slot * 8, phase, &abort_flag, kFaultWaitFull, 0x4b00u + warp);
+          const int cnt = min(a.slot_tiles, w1 - tile);
+          uint32_t at = ring_at + slot * slot_bytes, xsum = smem_u32(xsums) + (tile - chunk0) * (G * NT * 32) + t * 8;
+          uint32_t x[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) x[nt] = xl[nt] + (tile - chunk0) * 256;
+#pragma unroll 2
+          for (int i = 0; i < cnt; ++i) {
+            w4_tile_mma<T, NT, QG, ZEROS>(at, x, xsum, acc);
+            at += TILE;
+            xsum += G * NT * 32;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) x[nt] += 256;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty0 + slot * 8);
+          if (++slot == a.slots) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+        // [row group][warp][column][row]
+        float* out = sums + (size_t)(((g - batch0) * kGemvWarps + warp) * n) * kW4Rows;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int col = nt * 8 + t * 2 + (i & 1), row = r + 8 * (i >> 1);
+            if (col < n) {
+              float* o = out + col * kW4Rows + row;
+              const float v = kScale ? acc[nt][i] * undo[col].x * undo[col].y : acc[nt][i] * 0x1p20f;
+              *o = chunk0 == 0 ? v : *o + v;
+            }
+          }
+      }
+    }
+
+    // Join the partial sums and store: over the warps that share rows, then over the cluster.  An output is named by its
+    // unit (row group, row block, column) and row; every block of a cluster finishes 16 / split of the rows, the others
+    // hand it their sums through its shared memory.
+    workers_sync();
+    const int units = (batch_end - batch0) * WM * n;
+    auto warp_sum = [&](int group_block, int col, int row) {  // group_block: row group * WM + row block
+      const float* p = sums + ((size_t)(group_block << a.wk_log2) * n + col) * kW4Rows + row;
+      float v = p[0];
+      for (int w = 1; w < WK; ++w) v += p[(size_t)w * n * kW4Rows];
+      return v;
+    };
+    auto store = [&](int group_block, int col, int row, float v) {
+      const int g = group_block >> (4 - a.wk_log2), b = group_block & (WM - 1);
+      const size_t grow = ((size_t)(first + (batch0 + g) * a.clusters) * WM + b) * kW4Rows + row;
+      if (grow >= a.m) return;
+      if (!(fabsf(v) < INFINITY))  // infinities or NaNs among the operands, which the split sums may have turned around
+        v = w4_slow_dot(a.packed, W4Format{32 * QG, ZEROS}, grow, a.k, static_cast<const T*>(a.B) + col * a.ldb);
+      T* c = static_cast<T*>(a.C) + col * a.ldc + grow;
+      v *= a.alpha;
+      *c = from_f32<T>(a.beta != 0.f ? fmaf(a.beta, to_f32(*c), v) : v);
+    };
+    // thread i: row i % 16 of the units i / 16, i / 16 + 32, ...; unit = group_block * n + column, kept without divisions
+    const int row = threadIdx.x & 15;
+    int col = threadIdx.x >> 4, gb = 0;
+    auto settle = [&]() {
+      while (col >= n) {
+        col -= n;
+        ++gb;
+      }
+    };
+    settle();
+    if (split == 1) {
+      for (int u = threadIdx.x >> 4; u < units; u += kWorkers / 16, col += kWorkers / 16, settle())
+        store(gb, col, row, warp_sum(gb, col, row));
+      if (batch_end < mine) workers_sync();
+    } else {
+      const int share = kW4Rows >> a.split_log2, owner = row >> (4 - a.split_log2);  // rows of an owner
+      cluster_wait();  // all blocks of the cluster are running
+      for (int u = threadIdx.x >> 4; u < units; u += kWorkers / 16, col += kWorkers / 16, settle())
+        cluster_store(smem_u32(received + ((size_t)u * split + rank) * share + (row & (share - 1))), owner,
+                      warp_sum(gb, col, row));
+      cluster_arrive();
+      cluster_wait();
+      const int per = kWorkers >> (4 - a.split_log2);  // units of a round
+      gb = 0;
+      col = threadIdx.x >> (4 - a.split_log2);
+      settle();
+      for (int u = threadIdx.x >> (4 - a.split_log2); u < units; u += per, col += per, settle()) {
+        const float* p = received + (size_t)u * split * share + (threadIdx.x & (share - 1));
+        float v = p[0];
+        for (int s = 1; s < split; ++s) v += p[s * share];
+        store(gb, col, rank * share + (threadIdx.x & (share - 1)), v);
+      }
+    }
+  }
+  if (!ok) {  // a wait ran out: give the copies still in flight time to land before the block's memory goes
+    const uint64_t since = global_timer_ns();
+    while (global_timer_ns() - since < MMBO_DRAIN_LIMIT_NS) __nanosleep(1000);
+  }
+}
+
+}  // namespace mmbo
