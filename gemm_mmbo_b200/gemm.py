@@ -42,15 +42,27 @@ def _addr(x) -> int | None:
     return int(x.data_ptr())  # torch tensor
 
 
+_raw_stream = None  # reads torch's current stream of the current device; set once CUDA is known to be there
+
+
+def _current_stream() -> int | None:
+    global _raw_stream
+    try:
+        import torch
+        if not torch.cuda.is_available():
+            return None
+    except ImportError:
+        return None
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    device = torch.cuda.current_device
+    # building a Stream object and asking for CUDA again cost 4 us a call, as long as a small product takes
+    _raw_stream = (lambda: raw(device())) if raw else (lambda: torch.cuda.current_stream().cuda_stream)
+    return int(_raw_stream()) or None
+
+
 def _stream(stream) -> int | None:
     if stream is None:
-        try:
-            import torch
-            if torch.cuda.is_available():
-                return int(torch.cuda.current_stream().cuda_stream) or None
-        except ImportError:
-            pass
-        return None
+        return (_raw_stream() or None) if _raw_stream else _current_stream()
     if isinstance(stream, int):
         return stream or None
     return int(stream.cuda_stream) or None
