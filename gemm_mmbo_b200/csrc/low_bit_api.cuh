@@ -5,6 +5,7 @@
 #include "moe.cuh"
 #include "w4.cuh"
 #include "w4_gemv.cuh"
+#include "w4_umma.cuh"
 
 namespace mmbo {
 
@@ -41,37 +42,67 @@ static int allow_smem(K kernel, size_t bytes, bool (&done)[kMaxDevices]) {
   return (int)e;
 }
 
-// Blocks of w4_gemv_kernel (one per SM) that clusters of 1 << log2 fill at once: less than all SMs where a cluster's
-// blocks must share a group of SMs whose number is no multiple of theirs.
-static int g_gemv_clusters[kMaxDevices][3];
+constexpr size_t kGemvSmem = 227 * 1024 - 4096;  // of an SM's shared memory, less the kernel's static part
 
-template <typename K>
-static int gemv_clusters(K kernel, int split_log2) {
+// Clusters of 1 << log2 blocks that run at once with one block per SM: fewer than SMs / blocks, since the blocks of a
+// cluster share a group of SMs whose number is no multiple of theirs.
+static int g_cluster_slots[kMaxDevices][3];
+
+static int cluster_slots(int log2) {
   const int dev = current_device();
-  if (split_log2 == 0 || dev < 0 || dev >= kMaxDevices) return sm_count() >> split_log2;
-  int& known = g_gemv_clusters[dev][split_log2];
+  if (log2 == 0 || dev < 0 || dev >= kMaxDevices) return sm_count() >> log2;
+  int& known = g_cluster_slots[dev][log2];
   if (known == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(1 << split_log2));
-    cfg.blockDim = dim3(kGemvThreads);
-    cfg.dynamicSmemBytes = 128 * 1024;  // more than half an SM's: one block each
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1u << split_log2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    static bool prepared[kMaxDevices];
+    auto kernel = w4_gemv_kernel<__half, 1, 4, false>;
     int fit = 0;
-    if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess || fit <= 0) {
-      cudaGetLastError();
-      fit = (sm_count() >> split_log2) * 7 / 8;
+    if (allow_smem(kernel, kGemvSmem, prepared) == MMBO_OK) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u << log2);
+      cfg.blockDim = dim3(kGemvThreads);
+      cfg.dynamicSmemBytes = kGemvSmem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << log2;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess) fit = 0;
     }
-    known = fit < (sm_count() >> split_log2) ? fit : sm_count() >> split_log2;
+    cudaGetLastError();
+    if (fit <= 0) fit = (sm_count() >> log2) * 7 / 8;
+    known = fit < (sm_count() >> log2) ? fit : sm_count() >> log2;
   }
   return known;
 }
 
-constexpr size_t kGemvSmem = 227 * 1024 - 4096;  // of an SM's shared memory, less the kernel's static part
+// Launch with clusters of 1 << log2 blocks and programmatic stream serialization.
+template <typename K, typename... Args>
+static int launch_clustered(K kernel, unsigned grid, unsigned threads, size_t smem, int log2, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (log2) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1u << log2;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (settings().pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  MMBO_COUNT_LAUNCH();
+  return (int)e;
+}
 
 // How w4_gemv_kernel cuts a problem: the cheapest of all (warps along k, blocks along k), by a sum of what was measured
 // (B200, us): 0.022 a tile of the busiest SM (0.035 with 9 columns and more, whose products take as long again), 0.3 a
@@ -124,32 +155,10 @@ static int launch_w4_gemv(GemvArgs a, cudaStream_t st) {
   static bool prepared[kMaxDevices];
   int rc = allow_smem(kernel, kGemvSmem, prepared);
   if (rc) return rc;
-  const int clusters[3] = {gemv_clusters(kernel, 0), gemv_clusters(kernel, 1), gemv_clusters(kernel, 2)};
+  const int clusters[3] = {cluster_slots(0), cluster_slots(1), cluster_slots(2)};
   size_t smem = 0;
   if (!plan_gemv<NT, QG>(a, W4Tile<QG, ZEROS>::kBytes, clusters, &smem)) return MMBO_ERR_TOO_LARGE;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.clusters << a.split_log2);
-  cfg.blockDim = dim3(kGemvThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (a.split_log2) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = 1u << a.split_log2;
-    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (settings().pdl) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  MMBO_COUNT_LAUNCH();
-  return (int)e;
+  return launch_clustered(kernel, (unsigned)a.clusters << a.split_log2, kGemvThreads, smem, a.split_log2, st, a);
 }
 
 template <typename T, int NT>
@@ -164,18 +173,78 @@ static int dispatch_w4_gemv(const GemvArgs& a, W4Format f, cudaStream_t st) {
   }
 }
 
+// Tile width and blocks along k of w4_umma_kernel: the smallest number of cycles of the busiest SM, counted as rounds of
+// tiles x k-tiles x the cycles of one (measured: 400, 440, 700 with 32, 64, 128 columns) and what joining a cluster costs.
+static void plan_umma(size_t m, size_t n, size_t k, int* nt, int* split_log2) {
+  const size_t row_tiles = (m + 127) / 128, k_tiles = w4_k_tiles(k);
+  double best = 1e30;
+  for (int w = 32; w <= 128; w *= 2)
+    for (int log2 = 0; log2 <= (w <= 64 ? 2 : 0); ++log2) {
+      const size_t tiles = row_tiles * ((n + w - 1) / w), slots = (size_t)cluster_slots(log2);
+      if (log2 && (tiles > slots || k_tiles < ((size_t)1 << log2))) continue;
+      const size_t rounds = (tiles + slots - 1) / slots, span = (k_tiles + ((size_t)1 << log2) - 1) >> log2;
+      const double cost = (double)rounds * span * (w == 32 ? 400.0 : w == 64 ? 440.0 : 700.0) + (double)rounds * w * 10 +
+                          (log2 == 0 ? 0.0 : log2 == 1 ? 2500.0 : 3500.0);
+      if (cost < best) {
+        best = cost;
+        *nt = w;
+        *split_log2 = log2;
+      }
+    }
+}
+
+template <typename T, int NT, int QG, bool ZEROS>
+static int launch_w4_umma(UmmaArgs a, cudaStream_t st) {
+  using S = UmmaShape<NT>;
+  auto kernel = w4_umma_kernel<T, NT, QG, ZEROS>;
+  static bool prepared[kMaxDevices];
+  int rc = allow_smem(kernel, kGemvSmem, prepared);
+  if (rc) return rc;
+  const size_t stage = S::kXBytes + 8 * W4Tile<QG, ZEROS>::kBytes, fixed = 1024 + (a.split_log2 ? NT * 512 : 0);
+  a.stages = (int)((kGemvSmem - fixed) / stage);
+  if (a.stages > kUmmaMaxStages) a.stages = kUmmaMaxStages;
+  a.col_tiles = (int)((a.n + NT - 1) / NT);
+  const size_t tiles = (a.m + 127) / 128 * (size_t)a.col_tiles;
+  if (tiles > 0x3fffffffull) return MMBO_ERR_TOO_LARGE;
+  a.tiles = (int)tiles;
+  CUtensorMap map;
+  memset(&map, 0, sizeof map);
+  a.x_tma = a.k > 0 && a.ldb % 8 == 0 && aligned16(a.B);
+  if (a.x_tma &&
+      (rc = make_map(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                     2, a.B, a.k, a.n, a.ldb, 64, NT)))
+    return rc;
+  const unsigned blocks = a.split_log2 ? (unsigned)a.tiles << a.split_log2
+                                       : (unsigned)(a.tiles < sm_count() ? a.tiles : sm_count());
+  return launch_clustered(kernel, blocks, S::kThreads, a.stages * stage + fixed, a.split_log2, st, a, map);
+}
+
+template <typename T, int NT>
+static int dispatch_w4_umma(const UmmaArgs& a, W4Format f, cudaStream_t st) {
+  switch (f.group * 2 + f.zeros) {
+    case 64: return launch_w4_umma<T, NT, 1, false>(a, st);
+    case 65: return launch_w4_umma<T, NT, 1, true>(a, st);
+    case 128: return launch_w4_umma<T, NT, 2, false>(a, st);
+    case 129: return launch_w4_umma<T, NT, 2, true>(a, st);
+    case 256: return launch_w4_umma<T, NT, 4, false>(a, st);
+    default: return launch_w4_umma<T, NT, 4, true>(a, st);
+  }
+}
+
 template <typename T>
 static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* packed, W4Format f, const void* B,
                        size_t ldb, float beta, void* C, size_t ldc, cudaStream_t st) {
+  const unsigned char* w = static_cast<const unsigned char*>(packed);
   if (n <= 16) {
-    const GemvArgs a{m, n, k, ldb, ldc, alpha, beta, static_cast<const unsigned char*>(packed), B, C};
+    const GemvArgs a{m, n, k, ldb, ldc, alpha, beta, w, B, C};
     return n <= 8 ? dispatch_w4_gemv<T, 1>(a, f, st) : dispatch_w4_gemv<T, 2>(a, f, st);
   }
-  const dim3 grid((unsigned)((m + 7) / 8), (unsigned)(n < 65535 ? n : 65535));
-  w4_gemm_simple_kernel<T><<<grid, 256, 0, st>>>(m, n, k, alpha, static_cast<const unsigned char*>(packed), f,
-                                                 static_cast<const T*>(B), ldb, beta, static_cast<T*>(C), ldc);
-  MMBO_COUNT_LAUNCH();
-  return (int)cudaGetLastError();
+  int nt = 0, split_log2 = 0;
+  plan_umma(m, n, k, &nt, &split_log2);
+  const UmmaArgs a{m, n, k, ldb, ldc, alpha, beta, w, B, C, split_log2};
+  if (nt == 32) return dispatch_w4_umma<T, 32>(a, f, st);
+  if (nt == 64) return dispatch_w4_umma<T, 64>(a, f, st);
+  return dispatch_w4_umma<T, 128>(a, f, st);
 }
 
 // Workspace of the expert layer: expert numbers and gates (where the caller takes none), hidden vectors.

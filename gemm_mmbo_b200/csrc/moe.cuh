@@ -130,7 +130,7 @@ __global__ void moe_down_simple_kernel(MoeArgs a) {
           const unsigned char* in = static_cast<const unsigned char*>(a.down) + e * a.strideD +
                                     (i / kW4Rows * tiles + j / kW4Cols) * a.fmt.tile_bytes();
           const int row = (int)(i % kW4Rows), c = (int)(j % kW4Cols), g = c / a.fmt.group;
-          const uint32_t word = *reinterpret_cast<const uint32_t*>(in + row * 64 + (c % 32) / 8 * 16 + c / 32 * 4);
+          const uint32_t word = *reinterpret_cast<const uint32_t*>(in + w4_piece(row, c % 32 / 8) + c / 32 * 4);
           const int el = c % 8, z = a.fmt.zeros ? in[a.fmt.zero_at(g, row)] : 8;
           w = (float)((int)((word >> (4 * w4_nibble(el))) & 15u) - z) *
               to_f32(*reinterpret_cast<const T*>(in + a.fmt.scale_at(g, row)));

@@ -7,7 +7,9 @@
 // Packed format.  Rows are taken in blocks of 16 and columns in tiles of 128; the tiles of one row block follow one
 // another, so that whoever walks along k reads one contiguous stream.  A tile is
 //     1024 bytes of codes          row r (0..15) at 64 r; within a row, 16 bytes for each of four "lanes" t, holding one
-//                                  32-bit word for each quarter u of the tile: the columns 32 u + 8 t .. + 7
+//                                  32-bit word for each quarter u of the tile: the columns 32 u + 8 t .. + 7.  Lane t's
+//                                  piece lies at place t ^ (r / 2 % 4), so that both ways of reading a tile from shared
+//                                  memory, four lanes a row and one lane a row, touch every bank once
 //     (128 / group) x 16 scales    in the activations' type, group by group, rows in the order 0, 8, 1, 9, .. 7, 15
 //     (128 / group) x 16 bytes     zero points in the same order, where the matrix has them
 // In a word, columns 0 .. 7 sit in nibbles 0, 4, 2, 6, 1, 5, 3, 7: with v = w >> 8, the registers w & 0x000f000f,
@@ -41,6 +43,7 @@ struct W4Format {
   __host__ __device__ uint32_t zero_at(int g, int r) const { return kW4Codes + groups() * kW4Rows * 2 + g * kW4Rows + slot(r); }
   __host__ __device__ static int slot(int r) { return 2 * (r & 7) + (r >> 3); }
 };
+__host__ __device__ constexpr int w4_piece(int r, int t) { return r * 64 + (t ^ ((r >> 1) & 3)) * 16; }  // lane t of row r
 __host__ __device__ constexpr int w4_nibble(int column) {  // of one of a word's eight columns
   return (column >> 2) + 2 * ((column >> 1) & 1) + 4 * (column & 1);
 }
@@ -149,7 +152,7 @@ __global__ void w4_quantize_kernel(size_t m, size_t k, W4Format f, const T* __re
         if (f.zeros) out[f.zero_at(g, row)] = (unsigned char)z;
       }
     }
-    *reinterpret_cast<uint4*>(out + row * 64 + t * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+    *reinterpret_cast<uint4*>(out + w4_piece(row, t)) = make_uint4(word[0], word[1], word[2], word[3]);
   }
 }
 
@@ -195,7 +198,7 @@ __global__ void w4_pack_kernel(size_t m, size_t k, W4Format f, const unsigned ch
         if (f.zeros) out[f.zero_at(gt, row)] = (unsigned char)z;
       }
     }
-    *reinterpret_cast<uint4*>(out + row * 64 + t * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+    *reinterpret_cast<uint4*>(out + w4_piece(row, t)) = make_uint4(word[0], word[1], word[2], word[3]);
   }
 }
 
@@ -217,7 +220,7 @@ __global__ void w4_unpack_kernel(size_t m, size_t k, W4Format f, const unsigned 
     const int row = r + 8 * half;
     const size_t i = block * kW4Rows + row;
     if (i >= m) continue;
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(in + row * 64 + t * 16));
+    const uint4 c = __ldg(reinterpret_cast<const uint4*>(in + w4_piece(row, t)));
     const uint32_t word[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -253,7 +256,7 @@ __device__ __forceinline__ float w4_row_dot(const unsigned char* __restrict__ pa
   float acc = 0.f;
   for (size_t tile = half; tile < tiles; tile += 2) {
     const unsigned char* in = packed + (i / kW4Rows * tiles + tile) * f.tile_bytes();
-    const uint32_t w = __ldg(reinterpret_cast<const unsigned int*>(in + row * 64 + t * 16 + u * 4));
+    const uint32_t w = __ldg(reinterpret_cast<const unsigned int*>(in + w4_piece(row, t) + u * 4));
     const float s = to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row)));
     const int z = f.zeros ? in[f.zero_at(g, row)] : 8;
     float part = 0.f;

@@ -90,7 +90,8 @@ template <typename T, int NT, int QG, bool ZEROS>
 __device__ __forceinline__ void w4_tile_mma(uint32_t tile, const uint32_t (&x)[NT], uint32_t xsum, float (&acc)[NT][4]) {
   using L = W4Tile<QG, ZEROS>;
   const int lane = threadIdx.x & 31, r = lane >> 2;
-  const uint4 c0 = lds128(tile + lane * 16), c1 = lds128(tile + lane * 16 + 512);  // rows r and r + 8
+  const uint32_t codes = tile + w4_piece(r, lane & 3);
+  const uint4 c0 = lds128(codes), c1 = lds128(codes + 512);  // rows r and r + 8
   const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
   for (int g = 0; g < L::kGroups; ++g) {
@@ -228,7 +229,7 @@ __device__ __noinline__ float w4_slow_dot(const unsigned char* __restrict__ pack
   for (size_t j = 0; j < k; ++j) {
     const unsigned char* in = packed + (i / kW4Rows * tiles + j / kW4Cols) * f.tile_bytes();
     const int c = (int)(j % kW4Cols), g = c / f.group;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(in + row * 64 + c % 32 / 8 * 16 + c / 32 * 4);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(in + w4_piece(row, c % 32 / 8) + c / 32 * 4);
     const int q = (w >> (4 * w4_nibble(c % 8))) & 15u, z = f.zeros ? in[f.zero_at(g, row)] : 8;
     acc = fmaf((float)(q - z) * to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row))), to_f32(x[j]), acc);
   }

@@ -45,6 +45,14 @@ def test_product_sizes(cuda, mm, dtype, group, zeros):
         product(mm, dtype, m, n, k, group, zeros)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("group,zeros", [(32, False), (64, True), (128, False)])
+@pytest.mark.parametrize("n,pad", [(600, 0), (777, 8), (530, 1)])
+def test_product_with_enough_columns_for_wide_tiles(cuda, mm, dtype, group, zeros, n, pad):
+    """Several rounds of 128-column tiles, ragged in both directions."""
+    product(mm, dtype, 3001, n, 520, group, zeros, alpha=0.5, beta=1.0, ldb=520 + pad, ldc=3001 + pad)
+
+
 @pytest.mark.parametrize("n", [1, 5, 12, 40, 150])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_product_strides_alpha_beta(cuda, mm, dtype, n):
