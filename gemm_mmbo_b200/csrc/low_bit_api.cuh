@@ -54,7 +54,7 @@ static int cluster_slots(int log2) {
   int& known = g_cluster_slots[dev][log2];
   if (known == 0) {
     static bool prepared[kMaxDevices];
-    auto kernel = w4_gemv_kernel<__half, 1, 4, false>;
+    auto kernel = w4_gemv_kernel<__half, 4, false>;
     int fit = 0;
     if (allow_smem(kernel, kGemvSmem, prepared) == MMBO_OK) {
       cudaLaunchConfig_t cfg = {};
@@ -105,10 +105,9 @@ static int launch_clustered(K kernel, unsigned grid, unsigned threads, size_t sm
 }
 
 // How w4_gemv_kernel cuts a problem: the cheapest of all (warps along k, blocks along k), by a sum of what was measured
-// (B200, us): 0.022 a tile of the busiest SM (0.035 with 9 columns and more, whose products take as long again), 0.3 a
-// slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join clusters of two / four.  8192 x 28672, one
+// (B200, us): 0.022 a tile of the busiest SM, 0.3 a slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join clusters of two / four.  8192 x 28672, one
 // column: 28.4 us with the chosen 16 x 2, 30.7 with 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
-template <int NT, int QG>
+template <int QG>
 static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3], size_t* smem) {
   const size_t k_tiles = w4_k_tiles(a.k), blocks = w4_row_blocks(a.m);
   double best = 1e30;
@@ -122,17 +121,17 @@ static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3]
       const int slot_tiles = part < 4 ? (int)(part ? part : 1) : 4;
       const size_t ring = (size_t)kGemvWarps * 2 * slot_tiles * tile_bytes;
       const size_t one = gemv_sums_bytes((int)wk, (int)split, a.n, 1);
-      if (ring + one + gemv_x_bytes(a.n, 1, NT, 4 / QG) > kGemvSmem) continue;
-      size_t x_tiles = (kGemvSmem - ring - one - a.n * 64) / (a.n * 256 + (size_t)(4 / QG) * NT * 32);
+      if (ring + one + gemv_x_bytes(a.n, 1, 4 / QG) > kGemvSmem) continue;
+      size_t x_tiles = (kGemvSmem - ring - one - a.n * 64) / (a.n * 256 + (size_t)(4 / QG) * 32);
       if (x_tiles > span) x_tiles = span ? span : 1;
       if (x_tiles == 0) continue;
-      const size_t x = gemv_x_bytes(a.n, x_tiles, NT, 4 / QG);
+      const size_t x = gemv_x_bytes(a.n, x_tiles, 4 / QG);
       size_t batch = (kGemvSmem - ring - x) / one;
       if (batch > rounds) batch = rounds;
       if (batch == 0 || (split > 1 && batch < rounds)) continue;
       const size_t batches = (rounds + batch - 1) / batch;
       const double staged = (double)a.n * span * 0.25 * (x_tiles < span ? batches : 1);
-      const double cost = rounds * wm * span * (NT > 1 ? 0.035 : 0.022) + rounds * ((part + slot_tiles - 1) / slot_tiles) * 0.3 +
+      const double cost = rounds * wm * span * 0.022 + rounds * ((part + slot_tiles - 1) / slot_tiles) * 0.3 +
                           staged * 0.05 + (split == 1 ? 0.0 : split == 2 ? 1.8 : 2.5) + (batches - 1) * 1.0;
       if (cost < best) {
         best = cost;
@@ -149,32 +148,32 @@ static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3]
   return best < 1e30;
 }
 
-template <typename T, int NT, int QG, bool ZEROS>
+template <typename T, int QG, bool ZEROS>
 static int launch_w4_gemv(GemvArgs a, cudaStream_t st) {
-  auto kernel = w4_gemv_kernel<T, NT, QG, ZEROS>;
+  auto kernel = w4_gemv_kernel<T, QG, ZEROS>;
   static bool prepared[kMaxDevices];
   int rc = allow_smem(kernel, kGemvSmem, prepared);
   if (rc) return rc;
   const int clusters[3] = {cluster_slots(0), cluster_slots(1), cluster_slots(2)};
   size_t smem = 0;
-  if (!plan_gemv<NT, QG>(a, W4Tile<QG, ZEROS>::kBytes, clusters, &smem)) return MMBO_ERR_TOO_LARGE;
+  if (!plan_gemv<QG>(a, W4Tile<QG, ZEROS>::kBytes, clusters, &smem)) return MMBO_ERR_TOO_LARGE;
   return launch_clustered(kernel, (unsigned)a.clusters << a.split_log2, kGemvThreads, smem, a.split_log2, st, a);
 }
 
-template <typename T, int NT>
+template <typename T>
 static int dispatch_w4_gemv(const GemvArgs& a, W4Format f, cudaStream_t st) {
   switch (f.group * 2 + f.zeros) {
-    case 64: return launch_w4_gemv<T, NT, 1, false>(a, st);
-    case 65: return launch_w4_gemv<T, NT, 1, true>(a, st);
-    case 128: return launch_w4_gemv<T, NT, 2, false>(a, st);
-    case 129: return launch_w4_gemv<T, NT, 2, true>(a, st);
-    case 256: return launch_w4_gemv<T, NT, 4, false>(a, st);
-    default: return launch_w4_gemv<T, NT, 4, true>(a, st);
+    case 64: return launch_w4_gemv<T, 1, false>(a, st);
+    case 65: return launch_w4_gemv<T, 1, true>(a, st);
+    case 128: return launch_w4_gemv<T, 2, false>(a, st);
+    case 129: return launch_w4_gemv<T, 2, true>(a, st);
+    case 256: return launch_w4_gemv<T, 4, false>(a, st);
+    default: return launch_w4_gemv<T, 4, true>(a, st);
   }
 }
 
 // Tile width and blocks along k of w4_umma_kernel: the smallest number of cycles of the busiest SM, counted as rounds of
-// tiles x k-tiles x the cycles of one (measured: 400, 440, 700 with 32, 64, 128 columns) and what joining a cluster costs.
+// tiles x k-tiles x the cycles of one (measured: 500, 620, 900 with 32, 64, 128 columns) and what joining a cluster costs.
 static void plan_umma(size_t m, size_t n, size_t k, int* nt, int* split_log2) {
   const size_t row_tiles = (m + 127) / 128, k_tiles = w4_k_tiles(k);
   double best = 1e30;
@@ -183,7 +182,7 @@ static void plan_umma(size_t m, size_t n, size_t k, int* nt, int* split_log2) {
       const size_t tiles = row_tiles * ((n + w - 1) / w), slots = (size_t)cluster_slots(log2);
       if (log2 && (tiles > slots || k_tiles < ((size_t)1 << log2))) continue;
       const size_t rounds = (tiles + slots - 1) / slots, span = (k_tiles + ((size_t)1 << log2) - 1) >> log2;
-      const double cost = (double)rounds * span * (w == 32 ? 400.0 : w == 64 ? 440.0 : 700.0) + (double)rounds * w * 10 +
+      const double cost = (double)rounds * span * (w == 32 ? 500.0 : w == 64 ? 620.0 : 900.0) + (double)rounds * w * 10 +
                           (log2 == 0 ? 0.0 : log2 == 1 ? 2500.0 : 3500.0);
       if (cost < best) {
         best = cost;
@@ -200,15 +199,22 @@ static int launch_w4_umma(UmmaArgs a, cudaStream_t st) {
   static bool prepared[kMaxDevices];
   int rc = allow_smem(kernel, kGemvSmem, prepared);
   if (rc) return rc;
-  const size_t stage = S::kXBytes + 8 * W4Tile<QG, ZEROS>::kBytes, fixed = 1024 + (a.split_log2 ? NT * 512 : 0);
+  constexpr uint32_t kTile = W4Tile<QG, ZEROS>::kBytes;
+  const size_t stage = S::kXBytes + umma_code_bytes(kTile), fixed = 1024 + (a.split_log2 ? NT * 512 : 0);
   a.stages = (int)((kGemvSmem - fixed) / stage);
   if (a.stages > kUmmaMaxStages) a.stages = kUmmaMaxStages;
   a.col_tiles = (int)((a.n + NT - 1) / NT);
   const size_t tiles = (a.m + 127) / 128 * (size_t)a.col_tiles;
   if (tiles > 0x3fffffffull) return MMBO_ERR_TOO_LARGE;
   a.tiles = (int)tiles;
-  CUtensorMap map;
+  // packed tiles as 64-bit words: a row block is a row of the map, one load takes a k-tile of eight
+  CUtensorMap w_map, map;
+  memset(&w_map, 0, sizeof w_map);
   memset(&map, 0, sizeof map);
+  const size_t row_words = w4_k_tiles(a.k) * kTile / 8;
+  if (a.k > 0 && (rc = make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_INT64, 8, a.packed, row_words, w4_row_blocks(a.m), row_words,
+                                kTile / 8, 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
   a.x_tma = a.k > 0 && a.ldb % 8 == 0 && aligned16(a.B);
   if (a.x_tma &&
       (rc = make_map(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
@@ -216,7 +222,7 @@ static int launch_w4_umma(UmmaArgs a, cudaStream_t st) {
     return rc;
   const unsigned blocks = a.split_log2 ? (unsigned)a.tiles << a.split_log2
                                        : (unsigned)(a.tiles < sm_count() ? a.tiles : sm_count());
-  return launch_clustered(kernel, blocks, S::kThreads, a.stages * stage + fixed, a.split_log2, st, a, map);
+  return launch_clustered(kernel, blocks, S::kThreads, a.stages * stage + fixed, a.split_log2, st, a, w_map, map);
 }
 
 template <typename T, int NT>
@@ -235,10 +241,7 @@ template <typename T>
 static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* packed, W4Format f, const void* B,
                        size_t ldb, float beta, void* C, size_t ldc, cudaStream_t st) {
   const unsigned char* w = static_cast<const unsigned char*>(packed);
-  if (n <= 16) {
-    const GemvArgs a{m, n, k, ldb, ldc, alpha, beta, w, B, C};
-    return n <= 8 ? dispatch_w4_gemv<T, 1>(a, f, st) : dispatch_w4_gemv<T, 2>(a, f, st);
-  }
+  if (n <= 8) return dispatch_w4_gemv<T>(GemvArgs{m, n, k, ldb, ldc, alpha, beta, w, B, C}, f, st);
   int nt = 0, split_log2 = 0;
   plan_umma(m, n, k, &nt, &split_log2);
   const UmmaArgs a{m, n, k, ldb, ldc, alpha, beta, w, B, C, split_log2};

@@ -56,16 +56,31 @@ __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive elements as they lie in memory.  `vec`: the address is 16-byte aligned and all eight exist;
-// otherwise the `left` (possibly none) that exist are read one by one and the others are zero.
+// Elements at .. at + 7 of an array of `len`, zero behind its end, as they lie in memory; the array starts on any 2-byte
+// boundary.  Off the 16-byte boundaries two aligned loads are shifted together (eight loads of two bytes took four times
+// as long); nothing outside the array is read.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, long long left, bool vec, T (&out)[8]) {
-  if (vec && left >= 8) {
-    *reinterpret_cast<uint4*>(out) = __ldg(reinterpret_cast<const uint4*>(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = i < left ? p[i] : from_f32<T>(0.f);
+__device__ __forceinline__ uint4 load8(const T* array, long long len, long long at) {
+  if (at + 8 <= len) {
+    const T* p = array + at;
+    const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15u);
+    if (off == 0) return *reinterpret_cast<const uint4*>(p);
+    if (2 * at >= off && at + 16 - off / 2 <= len) {
+      const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+      const uint4 u = q[0], v = q[1];
+      const bool two = off & 8, one = off & 4;
+      const uint32_t w0 = two ? u.z : u.x, w1 = two ? u.w : u.y, w2 = two ? v.x : u.z, w3 = two ? v.y : u.w,
+                     w4 = two ? v.z : v.x, w5 = two ? v.w : v.y;
+      const uint32_t a0 = one ? w1 : w0, a1 = one ? w2 : w1, a2 = one ? w3 : w2, a3 = one ? w4 : w3, a4 = one ? w5 : w4;
+      const int bits = (off & 2) * 8;
+      return make_uint4(__funnelshift_r(a0, a1, bits), __funnelshift_r(a1, a2, bits), __funnelshift_r(a2, a3, bits),
+                        __funnelshift_r(a3, a4, bits));
+    }
   }
+  __align__(16) T v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = at + i < len ? array[at + i] : from_f32<T>(0.f);
+  return *reinterpret_cast<const uint4*>(v);
 }
 
 // ---------------------------------------------------------------- writing the format --
@@ -85,19 +100,16 @@ __global__ void w4_quantize_kernel(size_t m, size_t k, W4Format f, const T* __re
   const size_t block = unit / tiles, tile = unit % tiles;
   const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   unsigned char* out = packed + unit * f.tile_bytes();
-  const bool vec = ldw % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15u) == 0;
   const int per = f.group / 32;  // quarters in a group
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int row = r + 8 * half;
     const size_t i = block * kW4Rows + row;
-    T w[4][8];
+    __align__(16) T w[4][8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const size_t j = tile * kW4Cols + 32 * u + 8 * t;
-      const long long left = i < m ? (long long)k - (long long)j : 0;
-      load8(W + i * ldw + j, left, vec, w[u]);
-    }
+    for (int u = 0; u < 4; ++u)
+      *reinterpret_cast<uint4*>(w[u]) =
+          load8(W + i * ldw, i < m ? (long long)k : 0, (long long)(tile * kW4Cols + 32 * u + 8 * t));
     float lo[4], hi[4];
     bool bad[4];
 #pragma unroll
@@ -270,22 +282,6 @@ __device__ __forceinline__ float w4_row_dot(const unsigned char* __restrict__ pa
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
   return acc;
-}
-
-template <typename T>
-__global__ void w4_gemm_simple_kernel(size_t m, size_t n, size_t k, float alpha, const unsigned char* __restrict__ packed,
-                                      W4Format f, const T* __restrict__ B, size_t ldb, float beta, T* __restrict__ C,
-                                      size_t ldc) {
-  const size_t i = (size_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (i >= m) return;
-  for (size_t j = blockIdx.y; j < n; j += gridDim.y) {
-    const float acc = w4_row_dot(packed, f, i, k, B + j * ldb);
-    if ((threadIdx.x & 31) == 0) {
-      T* c = C + j * ldc + i;
-      const float v = alpha * acc;
-      *c = from_f32<T>(beta != 0.f ? fmaf(beta, to_f32(*c), v) : v);
-    }
-  }
 }
 
 }  // namespace mmbo

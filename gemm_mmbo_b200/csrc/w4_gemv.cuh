@@ -1,4 +1,4 @@
-// Packed 4-bit weights times up to 16 columns of activations.
+// Packed 4-bit weights times up to 8 columns of activations.
 //
 // What bounds it: the codes, read once (0.53 bytes a weight); for small matrices the latency of one trip to memory.
 //   - Every multiplying warp has a ring of tiles in shared memory, which a lane of the feeding warp fills with bulk
@@ -10,9 +10,10 @@
 //     that split k within a block and over the blocks of a cluster (distributed shared memory), in a fixed order: the
 //     same bits every time, and no scratch memory.
 //   - Before it waits for the kernel in front of it the feeding warp asks L2 for its first tiles.
-// The products run on mma.sync.m16n8k16: with at most 16 columns its rate is ample (a tile takes 8 or 16 instructions of
-// 8 cycles, on four schedulers, in the 45 cycles its bytes take), and its fragments come straight from the packed order
-// without a trip through tensor memory.
+// The products run on mma.sync.m16n8k16: with at most 8 columns its rate is ample (a tile takes 8 instructions of 8
+// cycles, on four schedulers, in the 45 cycles its bytes take), and its fragments come straight from the packed order
+// without a trip through tensor memory.  (With 16 columns the kernel of w4_umma.cuh is ahead: 17 against 23 us at
+// 8192 x 8192.)
 #pragma once
 
 #include <cooperative_groups.h>
@@ -78,16 +79,16 @@ struct W4Tile {
   static constexpr int kBytes = kZeros + (ZEROS ? kGroups * kW4Rows : 0);
 };
 
-// acc[nt] += the products of a tile with 128 rows of 8 NT staged columns: x[nt] is this lane's place in them, `xsum` its
-// place in their group sums (shared memory addresses).  Sums are in units of 2^20.
+// acc += the products of a tile with 128 rows of 8 staged columns: x is this lane's place in them, `xsum` its place in
+// their group sums (shared memory addresses).  Sums are in units of 2^20.
 //
 // A code is used as the bits of a half-precision number: q in the lowest four bits is the subnormal q 2^-24, q in the
 // next four is q 2^-20, both exact, so a word becomes four operand registers with a shift and four masks.  The two kinds
 // have a sum each, and the zero point comes off once a group:  sum (q - z) x = sum q x - z sum x.  (Forming the sums of
 // x with the same instruction and a matrix of ones made the tensor pipe the bound: 16 instructions a tile, 32 cycles;
 // subtracting the zero point from each code costs as much again as unpacking it.)
-template <typename T, int NT, int QG, bool ZEROS>
-__device__ __forceinline__ void w4_tile_mma(uint32_t tile, const uint32_t (&x)[NT], uint32_t xsum, float (&acc)[NT][4]) {
+template <typename T, int QG, bool ZEROS>
+__device__ __forceinline__ void w4_tile_mma(uint32_t tile, uint32_t x, uint32_t xsum, float (&acc)[4]) {
   using L = W4Tile<QG, ZEROS>;
   const int lane = threadIdx.x & 31, r = lane >> 2;
   const uint32_t codes = tile + w4_piece(r, lane & 3);
@@ -95,21 +96,18 @@ __device__ __forceinline__ void w4_tile_mma(uint32_t tile, const uint32_t (&x)[N
   const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
   for (int g = 0; g < L::kGroups; ++g) {
-    float low[NT][4], high[NT][4];
+    float low[4], high[4];
 #pragma unroll
     for (int qq = 0; qq < QG; ++qq) {
       const int q = g * QG + qq;
       const uint32_t v0 = w0[q] >> 8, v1 = w1[q] >> 8;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const uint4 b = lds128(x[nt] + q * 64);
-        if (qq == 0) {
-          mma_f16_from_zero(low[nt], w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
-          mma_f16_from_zero(high[nt], w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
-        } else {
-          mma_f16(low[nt], w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
-          mma_f16(high[nt], w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
-        }
+      const uint4 b = lds128(x + q * 64);
+      if (qq == 0) {
+        mma_f16_from_zero(low, w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
+        mma_f16_from_zero(high, w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
+      } else {
+        mma_f16(low, w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
+        mma_f16(high, w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
       }
     }
     const float2 s = widen2<T>(lds32(tile + L::kScales + g * 32 + r * 4));
@@ -119,14 +117,11 @@ __device__ __forceinline__ void w4_tile_mma(uint32_t tile, const uint32_t (&x)[N
       z0 = (float)(z & 15u);
       z1 = (float)((z >> 8) & 15u);
     }
+    const float2 xs = lds_f2(xsum + g * 32);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float2 xs = lds_f2(xsum + (g * NT + nt) * 32);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float dot = fmaf(16.f, low[nt][i], high[nt][i]);
-        acc[nt][i] = fmaf(i < 2 ? s.x : s.y, fmaf(i < 2 ? -z0 : -z1, i & 1 ? xs.y : xs.x, dot), acc[nt][i]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const float dot = fmaf(16.f, low[i], high[i]);
+      acc[i] = fmaf(i < 2 ? s.x : s.y, fmaf(i < 2 ? -z0 : -z1, i & 1 ? xs.y : xs.x, dot), acc[i]);
     }
   }
 }
@@ -143,9 +138,9 @@ __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" 
 // rounding is far below the last bit of any fp32 sum they enter, and one tile product serves both types.  The sums get
 // their true size again by two factors a column; those of a bfloat16 column with an infinity or a NaN are NaN, so that
 // they are noticed.
-//   xs: the columns as they came, x_stride bytes apart; sums: [tile][group][8 NT] floats; peak: bits of the largest
+//   xs: the columns as they came, x_stride bytes apart; sums: [tile][group][8] floats; peak: bits of the largest
 //   magnitudes (bfloat16), zero before the call.
-template <typename T, int NT, int QG>
+template <typename T, int QG>
 __device__ __forceinline__ void w4_stage(int n, int tiles, unsigned char* xs, uint32_t x_stride, float* sums,
                                          uint32_t* peak, float2* undo) {
   constexpr bool kScale = !std::is_same<T, __half>::value;
@@ -213,7 +208,7 @@ __device__ __forceinline__ void w4_stage(int n, int tiles, unsigned char* xs, ui
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int piece = first + 32 * h;
-      if (piece < pieces && (piece & (kLanes - 1)) == 0) sums[piece / kLanes * 8 * NT + col] = sum[h] * 0x1p-20f;
+      if (piece < pieces && (piece & (kLanes - 1)) == 0) sums[piece / kLanes * 8 + col] = sum[h] * 0x1p-20f;
     }
   }
   workers_sync();
@@ -247,10 +242,12 @@ __device__ __forceinline__ void bulk_prefetch(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 
-// Bounded wait by a whole warp that sleeps in the barrier unit instead of polling: the polls of waiting warps would cost
-// the working ones issue slots.  200 tries of at most 10 ms each.
+// Bounded wait that sleeps in the barrier unit instead of polling: the polls of waiting warps would cost the working ones
+// issue slots.  A first try without a time to sleep: where the phase has passed already, the sleeping form takes 300
+// cycles to say so.  Then 200 tries of at most 10 ms each.
 __device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
                                                  unsigned int fault_code, unsigned int detail) {
+  if (mbar_try_wait(bar, parity)) return true;
 #pragma unroll 1
   for (int i = 0; i < 200; ++i) {
     uint32_t done;
@@ -296,9 +293,9 @@ struct GemvArgs {
   int clusters;
 };
 
-// Staged columns with their group sums (nt: blocks of 8 columns, groups: in a tile).
-__host__ __device__ inline size_t gemv_x_bytes(size_t n, size_t tiles, int nt, int groups) {
-  return n * (tiles * 256 + 64) + tiles * groups * nt * 32;
+// Staged columns with their group sums (groups: in a tile).
+__host__ __device__ inline size_t gemv_x_bytes(size_t n, size_t tiles, int groups) {
+  return n * (tiles * 256 + 64) + tiles * groups * 32;
 }
 // Partial sums of a batch of row groups, and the room for what the other blocks of a cluster hand over.
 __host__ __device__ inline size_t gemv_sums_bytes(int wk, int split, size_t n, int batch) {
@@ -306,7 +303,7 @@ __host__ __device__ inline size_t gemv_sums_bytes(int wk, int split, size_t n, i
   return (out * wk + (split > 1 ? out : 0)) * 4;
 }
 
-template <typename T, int NT, int QG, bool ZEROS>
+template <typename T, int QG, bool ZEROS>
 __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs a) {
   constexpr uint32_t TILE = W4Tile<QG, ZEROS>::kBytes;
   constexpr bool kScale = !std::is_same<T, __half>::value;
@@ -315,8 +312,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
   __shared__ __align__(8) unsigned long long full_bars[kGemvWarps * kGemvMaxSlots], empty_bars[kGemvWarps * kGemvMaxSlots];
   __shared__ __align__(8) unsigned long long x_bar;
   __shared__ uint32_t abort_flag;
-  __shared__ uint32_t peak[8 * NT];
-  __shared__ float2 undo[8 * NT];
+  __shared__ uint32_t peak[8];
+  __shared__ float2 undo[8];
   const int split = 1 << a.split_log2, rank = blockIdx.x & (split - 1), first = blockIdx.x >> a.split_log2;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int WK = 1 << a.wk_log2, WM = kGemvWarps >> a.wk_log2;
@@ -331,7 +328,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
   unsigned char* xs = smem + (size_t)kGemvWarps * a.slots * slot_bytes;
   const uint32_t x_stride = a.x_tiles * 256 + 64;  // columns 64 bytes out of step: conflict-free 16-byte reads
   float* xsums = reinterpret_cast<float*>(xs + (size_t)n * x_stride);
-  float* sums = xsums + a.x_tiles * G * 8 * NT;
+  float* sums = xsums + a.x_tiles * G * 8;
   float* received = sums + (size_t)a.batch * kGemvWarps * kW4Rows * n;
 
   if (threadIdx.x == 0) {
@@ -363,34 +360,23 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
   griddep_wait();
 
   // Activations of a chunk of k: requested before the weights, so that they do not queue behind them.
-  const bool x_bulk = a.ldb % 8 == 0 && a.k % 8 == 0 && (reinterpret_cast<uintptr_t>(a.B) & 15u) == 0;
+  const bool x_bulk = a.ldb % 8 == 0 && (reinterpret_cast<uintptr_t>(a.B) & 15u) == 0;
   uint32_t x_phase = 0;
   auto request_x = [&](int chunk0) {
     const size_t k0 = (size_t)(t0 + chunk0) * kW4Cols;
-    const int tiles = min(span - chunk0, a.x_tiles);
-    const int real = (int)min((size_t)tiles * kW4Cols, a.k - min(a.k, k0));  // elements of a column that exist
+    const int pieces = min(span - chunk0, a.x_tiles) * 16;  // of 16 bytes in a column
+    const int whole = x_bulk ? (int)min((size_t)pieces, (a.k - min(a.k, k0)) / 8) : 0;
     if (kScale && threadIdx.x < n) peak[threadIdx.x] = 0;
-    if (x_bulk) {
-      if (threadIdx.x == 0) {
-        mbar_expect_tx(smem_u32(&x_bar), n * real * 2);
-        if (real > 0)
-          for (int col = 0; col < n; ++col)
-            bulk_load(smem_u32(xs) + col * x_stride, static_cast<const T*>(a.B) + col * a.ldb + k0, real * 2,
-                      smem_u32(&x_bar));
-      }
-      const int fill = tiles * 16 - real / 8;  // pieces behind k
-      for (int i = threadIdx.x; i < fill * n; i += kWorkers)
-        *reinterpret_cast<uint4*>(xs + i / fill * x_stride + real * 2 + i % fill * 16) = make_uint4(0, 0, 0, 0);
-    } else {
-      const int pieces = tiles * 16;
-#pragma unroll 2
-      for (int i = threadIdx.x; i < pieces * n; i += kWorkers) {
-        const int col = i / pieces, piece = i % pieces;
-        __align__(16) T v[8];
-        load8(static_cast<const T*>(a.B) + col * a.ldb + k0 + piece * 8, (long long)real - piece * 8, false, v);
-        *reinterpret_cast<uint4*>(xs + col * x_stride + piece * 16) = *reinterpret_cast<const uint4*>(v);
-      }
+    if (x_bulk && threadIdx.x == 0) {
+      mbar_expect_tx(smem_u32(&x_bar), n * whole * 16);
+      for (int col = 0; col < n && whole > 0; ++col)
+        bulk_load(smem_u32(xs) + col * x_stride, static_cast<const T*>(a.B) + col * a.ldb + k0, whole * 16, smem_u32(&x_bar));
     }
+    for (int col = 0; col < n; ++col)
+#pragma unroll 2
+      for (int piece = whole + threadIdx.x; piece < pieces; piece += kWorkers)
+        *reinterpret_cast<uint4*>(xs + col * x_stride + piece * 16) =
+            load8(static_cast<const T*>(a.B) + col * a.ldb, (long long)a.k, (long long)k0 + piece * 8);
   };
   if (warp < kGemvWarps) request_x(0);
 
@@ -432,10 +418,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
   }
 
   bool ok = true;
-  uint32_t xl[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)  // columns past n repeat the last one; their sums are not stored
-    xl[nt] = smem_u32(xs) + min(nt * 8 + r, n - 1) * x_stride + t * 16;
+  // columns past n repeat the last one; their sums are not stored
+  const uint32_t x_lane = smem_u32(xs) + min(r, n - 1) * x_stride + t * 16, xsum_lane = smem_u32(xsums) + t * 8;
   for (int batch0 = 0; batch0 < mine; batch0 += a.batch) {
     const int batch_end = min(mine, batch0 + a.batch);
     for (int chunk0 = 0; chunk0 < span || chunk0 == 0; chunk0 += a.x_tiles) {
@@ -447,29 +431,22 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
         if (x_bulk && ok) ok = mbar_wait_asleep(smem_u32(&x_bar), x_phase, &abort_flag, kFaultWaitCLoad, 0x4b10u);
         x_phase ^= 1u;
         workers_sync();
-        w4_stage<T, NT, QG>(n, min(span - chunk0, a.x_tiles), xs, x_stride, xsums, peak, undo);
+        w4_stage<T, QG>(n, min(span - chunk0, a.x_tiles), xs, x_stride, xsums, peak, undo);
       }
       const int w0 = part_of(chunk0, wk), w1 = part_of(chunk0, wk + 1);
       for (int g = batch0; g < batch_end; ++g) {
-        float acc[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
         for (int tile = w0; tile < w1; tile += a.slot_tiles) {
           if (ok) ok = mbar_wait_asleep(full0 + slot * 8, phase, &abort_flag, kFaultWaitFull, 0x4b00u + warp);
           const int cnt = min(a.slot_tiles, w1 - tile);
-          uint32_t at = ring_at + slot * slot_bytes, xsum = smem_u32(xsums) + (tile - chunk0) * (G * NT * 32) + t * 8;
-          uint32_t x[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) x[nt] = xl[nt] + (tile - chunk0) * 256;
+          uint32_t at = ring_at + slot * slot_bytes, x = x_lane + (tile - chunk0) * 256;
+          uint32_t xsum = xsum_lane + (tile - chunk0) * (G * 32);
 #pragma unroll 2
           for (int i = 0; i < cnt; ++i) {
-            w4_tile_mma<T, NT, QG, ZEROS>(at, x, xsum, acc);
+            w4_tile_mma<T, QG, ZEROS>(at, x, xsum, acc);
             at += TILE;
-            xsum += G * NT * 32;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) x[nt] += 256;
+            x += 256;
+            xsum += G * 32;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(empty0 + slot * 8);
@@ -481,16 +458,14 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
         // [row group][warp][column][row]
         float* out = sums + (size_t)(((g - batch0) * kGemvWarps + warp) * n) * kW4Rows;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int col = nt * 8 + t * 2 + (i & 1), row = r + 8 * (i >> 1);
-            if (col < n) {
-              float* o = out + col * kW4Rows + row;
-              const float v = kScale ? acc[nt][i] * undo[col].x * undo[col].y : acc[nt][i] * 0x1p20f;
-              *o = chunk0 == 0 ? v : *o + v;
-            }
+        for (int i = 0; i < 4; ++i) {
+          const int col = t * 2 + (i & 1), row = r + 8 * (i >> 1);
+          if (col < n) {
+            float* o = out + col * kW4Rows + row;
+            const float v = kScale ? acc[i] * undo[col].x * undo[col].y : acc[i] * 0x1p20f;
+            *o = chunk0 == 0 ? v : *o + v;
           }
+        }
       }
     }
 

@@ -1,7 +1,7 @@
 // Packed 4-bit weights times many columns of activations, on the fifth-generation tensor cores.
 //
 // A block computes 128 rows x NT columns.  The weights never exist in 16 bits outside tensor memory:
-//   warp 0      feeds: bulk copies of the packed tiles (8 row blocks), TMA loads of the activations (128 x NT), into a ring
+//   warp 0      feeds: TMA loads of the packed tiles (8 row blocks in one) and of the activations (128 x NT) into a ring
 //   warp 1      issues the products: A (the unpacked weights) from tensor memory, B (the activations) from shared memory
 //   warps 2, 3  stand in for TMA where the activations are not aligned for it
 //   unpackers   (4 or 8 warps) turn codes into exact integers q - z in the activations' type and write them to tensor
@@ -127,19 +127,22 @@ struct UmmaShape {
   static constexpr int kXBytes = NT * 256;               // activations of a k-tile
 };
 constexpr int kUmmaMaxStages = 10;
+constexpr int kUmmaASlots = 4;  // unpacked tiles in tensor memory, 64 columns each
+// Packed tiles of a stage, in the order of the row blocks; TMA wants its destination on a 128-byte boundary.
+__host__ __device__ constexpr uint32_t umma_code_bytes(uint32_t tile_bytes) { return (8 * tile_bytes + 127) / 128 * 128; }
 
 template <typename T, int NT, int QG, bool ZEROS>
 __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
-    w4_umma_kernel(const UmmaArgs a, const __grid_constant__ CUtensorMap x_map) {
+    w4_umma_kernel(const UmmaArgs a, const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map) {
   using S = UmmaShape<NT>;
   using L = W4Tile<QG, ZEROS>;
-  constexpr uint32_t TILE = L::kBytes;
+  constexpr uint32_t TILE = L::kBytes, CODES = umma_code_bytes(TILE);
   constexpr int G = 4 / QG;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) unsigned long long full_bars[kUmmaMaxStages], empty_bars[kUmmaMaxStages];
-  __shared__ __align__(8) unsigned long long a_full[2], a_empty[2], d_full[S::kSums], d_empty[S::kSums];
+  __shared__ __align__(8) unsigned long long a_full[kUmmaASlots], a_empty[kUmmaASlots], d_full[S::kSums], d_empty[S::kSums];
   __shared__ uint32_t abort_flag, tmem_slot;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const int split = 1 << a.split_log2, rank = blockIdx.x & (split - 1);
   const int k_tiles = (int)w4_k_tiles(a.k), row_blocks = (int)w4_row_blocks(a.m);
   const int t0 = (int)(((long long)k_tiles * rank) >> a.split_log2);
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
   const int first = blockIdx.x >> a.split_log2, step = gridDim.x >> a.split_log2;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t codes_at = smem + a.stages * S::kXBytes;
-  float* received = reinterpret_cast<float*>(smem_raw + (codes_at + a.stages * 8 * TILE - smem_u32(smem_raw)));
+  float* received = reinterpret_cast<float*>(smem_raw + (codes_at + a.stages * CODES - smem_u32(smem_raw)));
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -155,7 +158,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
       mbar_init(smem_u32(&full_bars[s]), a.x_tma ? 1 : 3);  // the feeder, and the two warps that stand in for TMA
       mbar_init(smem_u32(&empty_bars[s]), 5);               // four unpackers and the products
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kUmmaASlots; ++i) {
       mbar_init(smem_u32(&a_full[i]), 4);
       mbar_init(smem_u32(&a_empty[i]), 1);
     }
@@ -173,36 +176,38 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
     const int block = first / a.col_tiles * 8 + (lane & 7), cnt = min(span, a.stages);
     if (lane < 8 && block < row_blocks && cnt > 0)
       bulk_prefetch(a.packed + ((size_t)block * k_tiles + t0) * TILE, cnt * TILE);
-    if (lane == 8 && a.x_tma) prefetch_tensormap(&x_map);
+    if (lane == 8) prefetch_tensormap(&w_map);
+    if (lane == 9 && a.x_tma) prefetch_tensormap(&x_map);
   }
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = tmem_slot;
-  const uint32_t a_cols = tmem + 256;  // group sums in columns 0 .. 255, two tiles of weights in 256 .. 383
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  const uint32_t a_cols = tmem + 256;  // group sums in columns 0 .. 255, four tiles of weights in 256 .. 511
   if (split > 1) cluster_arrive();
   griddep_launch_dependents();
   griddep_wait();
 
   bool ok = true;
   if (warp == 0) {
-    // ---- feeder
+    // ---- feeder (one elected lane, for the same reason as below)
     int stage = 0;
     uint32_t phase = 0;
     for (int tile = first; ok && tile < a.tiles; tile += step) {
       const int row_tile = tile / a.col_tiles, col0 = (tile - row_tile * a.col_tiles) * NT;
-      const int have = min(8, row_blocks - row_tile * 8);
-      const unsigned char* src = a.packed + ((size_t)row_tile * 8 * k_tiles + t0) * TILE;
       for (int i = 0; ok && i < span; ++i) {
         ok = mbar_wait_together(smem_u32(&empty_bars[stage]), phase ^ 1u, &abort_flag, kFaultWaitEmpty, 0x4c00u + stage);
-        const uint32_t bar = smem_u32(&full_bars[stage]);
-        if (ok && lane == 0) mbar_expect_tx(bar, have * TILE + (a.x_tma ? S::kXBytes : 0));
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t bar = smem_u32(&full_bars[stage]), x = smem + stage * S::kXBytes;
+          mbar_expect_tx(bar, 8 * TILE + (a.x_tma ? S::kXBytes : 0));
+          tma_load_2d(codes_at + stage * CODES, &w_map, bar, (t0 + i) * (int)(TILE / 8), row_tile * 8);
+          if (a.x_tma) {
+            tma_load_2d(x, &x_map, bar, (t0 + i) * kW4Cols, col0);
+            tma_load_2d(x + NT * 128, &x_map, bar, (t0 + i) * kW4Cols + 64, col0);
+          }
+        }
         __syncwarp();
-        if (ok && lane < have)
-          bulk_load(codes_at + (stage * 8 + lane) * TILE, src + ((size_t)lane * k_tiles + i) * TILE, TILE, bar);
-        if (ok && a.x_tma && (lane == 8 || lane == 9))
-          tma_load_2d(smem + stage * S::kXBytes + (lane - 8) * (NT * 128), &x_map, bar, (t0 + i) * kW4Cols + (lane - 8) * 64,
-                      col0);
         if (++stage == a.stages) {
           stage = 0;
           phase ^= 1u;
@@ -210,25 +215,33 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ---- products
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc(std::is_same<T, __half>::value ? 0u : 1u, 0u, 0u, 128u, (uint32_t)NT);
-      int stage = 0;
-      uint32_t phase = 0, sums = 0, done = 0;
-      for (int tile = first; ok && tile < a.tiles; tile += step)
-        for (int i = 0; ok && i < span; ++i, ++done) {
-          const uint32_t slot = done & 1u;
-          ok = mbar_wait_asleep(smem_u32(&a_full[slot]), (done >> 1) & 1u, &abort_flag, kFaultWaitFull, 0x4c10u) &&
-               mbar_wait_asleep(smem_u32(&full_bars[stage]), phase, &abort_flag, kFaultWaitFull, 0x4c11u);
-          if (!ok) break;
-          const uint64_t desc = make_smem_desc_sw128(smem + stage * S::kXBytes, 16u, 1024u);
+    // ---- products.  The whole warp walks the loop and one elected lane issues: what the instructions take (uniform
+    // registers) then comes from uniform arithmetic; under `if (lane == 0)` each cost 100 cycles to get ready.
+    constexpr uint32_t idesc = make_idesc(std::is_same<T, __half>::value ? 0u : 1u, 0u, 0u, 128u, (uint32_t)NT);
+    int stage = 0;
+    uint32_t phase = 0, sums = 0, done = 0;
+    for (int tile = first; ok && tile < a.tiles; tile += step)
+      for (int i = 0; ok && i < span; ++i, ++done) {
+        const uint32_t slot = done % kUmmaASlots, slot_phase = done / kUmmaASlots & 1u;
+        // one answer of the barrier unit takes 60 cycles: ask all three before looking at any
+        const uint32_t d0 = sums % S::kSums;
+        const bool ready = mbar_try_wait(smem_u32(&a_full[slot]), slot_phase) & mbar_try_wait(smem_u32(&full_bars[stage]), phase) &
+                           mbar_try_wait(smem_u32(&d_empty[d0]), ((sums / S::kSums) & 1u) ^ 1u);
+        bool asked = __all_sync(0xffffffffu, ready);
+        if (!asked)
+          ok = mbar_wait_together(smem_u32(&a_full[slot]), slot_phase, &abort_flag, kFaultWaitFull, 0x4c10u) &&
+               mbar_wait_together(smem_u32(&full_bars[stage]), phase, &abort_flag, kFaultWaitFull, 0x4c11u);
+        if (!ok) break;
+        const uint64_t desc = make_smem_desc_sw128(smem + stage * S::kXBytes, 16u, 1024u);
 #pragma unroll
-          for (int g = 0; g < G; ++g, ++sums) {
-            const uint32_t d = sums % S::kSums;
-            ok = mbar_wait_asleep(smem_u32(&d_empty[d]), ((sums / S::kSums) & 1u) ^ 1u, &abort_flag, kFaultWaitTmemEmpty,
-                                  0x4c12u);
-            if (!ok) break;
-            tcgen05_fence_after();
+        for (int g = 0; g < G; ++g, ++sums) {
+          const uint32_t d = sums % S::kSums;
+          if (!(g == 0 && asked))
+            ok = mbar_wait_together(smem_u32(&d_empty[d]), ((sums / S::kSums) & 1u) ^ 1u, &abort_flag, kFaultWaitTmemEmpty,
+                                    0x4c12u);
+          if (!ok) break;
+          tcgen05_fence_after();
+          if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < 2 * QG; ++j) {
               const int step16 = g * 2 * QG + j;  // of the tile's eight steps of 16; four to a 64-column half
@@ -236,17 +249,19 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
                           desc + (((step16 >> 2) * (NT * 128) + (step16 & 3) * 32) >> 4), idesc, j > 0);
             }
             umma_commit(smem_u32(&d_full[d]));
+            if (g == G - 1) {
+              umma_commit(smem_u32(&a_empty[slot]));
+              umma_commit(smem_u32(&empty_bars[stage]));
+            }
           }
-          if (!ok) break;
-          umma_commit(smem_u32(&a_empty[slot]));
-          umma_commit(smem_u32(&empty_bars[stage]));
-          if (++stage == a.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          __syncwarp();
         }
-    }
-    __syncwarp();
+        if (!ok) break;
+        if (++stage == a.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
   } else if (warp < 4) {
     // ---- activations that TMA cannot address
     if (!a.x_tma) {
@@ -258,13 +273,13 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
           ok = mbar_wait_together(smem_u32(&empty_bars[stage]), phase ^ 1u, &abort_flag, kFaultWaitEmpty, 0x4c20u);
           if (!ok) break;
           unsigned char* xs = smem_raw + (smem + stage * S::kXBytes - smem_u32(smem_raw));
+#pragma unroll 4
           for (int p = (warp - 2) * 32 + lane; p < NT * 16; p += 64) {
             const int row = p >> 4, chunk = p & 15;  // 16-byte chunks of a column's 128 elements
-            const size_t k0 = (size_t)(t0 + i) * kW4Cols + chunk * 8, col = (size_t)col0 + row;
-            __align__(16) T v[8];
-            load8(static_cast<const T*>(a.B) + col * a.ldb + k0, col < a.n ? (long long)a.k - (long long)k0 : 0, false, v);
+            const size_t col = (size_t)col0 + row;
             *reinterpret_cast<uint4*>(xs + (chunk >> 3) * (NT * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
-                *reinterpret_cast<const uint4*>(v);
+                load8(static_cast<const T*>(a.B) + col * a.ldb, col < a.n ? (long long)a.k : 0,
+                      (long long)(t0 + i) * kW4Cols + chunk * 8);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -284,12 +299,12 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
     uint32_t phase = (uint32_t)(set / a.stages) & 1u;
     const int total = first < a.tiles ? ((a.tiles - first + step - 1) / step) * span : 0;
     for (int i = set; ok && i < total; i += S::kUnpackSets) {
-      const uint32_t slot = (uint32_t)i & 1u;
+      const uint32_t slot = (uint32_t)i % kUmmaASlots;
       ok = mbar_wait_together(smem_u32(&full_bars[stage]), phase, &abort_flag, kFaultWaitFull, 0x4c30u) &&
-           mbar_wait_together(smem_u32(&a_empty[slot]), (((uint32_t)i >> 1) & 1u) ^ 1u, &abort_flag, kFaultWaitEmpty, 0x4c31u);
+           mbar_wait_together(smem_u32(&a_empty[slot]), ((uint32_t)i / kUmmaASlots & 1u) ^ 1u, &abort_flag, kFaultWaitEmpty, 0x4c31u);
       if (!ok) break;
       tcgen05_fence_after();
-      const uint32_t block = codes_at + (stage * 8 + (row >> 4)) * TILE;
+      const uint32_t block = codes_at + stage * CODES + (row >> 4) * TILE;
       uint4 c[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) c[t] = lds128(block + w4_piece(r, t));
