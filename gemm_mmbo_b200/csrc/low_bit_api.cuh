@@ -173,16 +173,17 @@ static int dispatch_w4_gemv(const GemvArgs& a, W4Format f, cudaStream_t st) {
 }
 
 // Tile width and blocks along k of w4_umma_kernel: the smallest number of cycles of the busiest SM, counted as rounds of
-// tiles x k-tiles x the cycles of one (measured: 500, 620, 900 with 32, 64, 128 columns) and what joining a cluster costs.
-static void plan_umma(size_t m, size_t n, size_t k, int* nt, int* split_log2) {
+// tiles x k-tiles x the cycles of one (measured: 500, 620, 900 with 32, 64, 128 columns; 700, 1100 where the unpacking
+// warps have to bring the activations, not worth it with 128) and what joining a cluster costs.
+static void plan_umma(size_t m, size_t n, size_t k, bool x_tma, int* nt, int* split_log2) {
   const size_t row_tiles = (m + 127) / 128, k_tiles = w4_k_tiles(k);
   double best = 1e30;
-  for (int w = 32; w <= 128; w *= 2)
+  for (int w = 32; w <= (x_tma ? 128 : 64); w *= 2)
     for (int log2 = 0; log2 <= (w <= 64 ? 2 : 0); ++log2) {
       const size_t tiles = row_tiles * ((n + w - 1) / w), slots = (size_t)cluster_slots(log2);
       if (log2 && (tiles > slots || k_tiles < ((size_t)1 << log2))) continue;
       const size_t rounds = (tiles + slots - 1) / slots, span = (k_tiles + ((size_t)1 << log2) - 1) >> log2;
-      const double cost = (double)rounds * span * (w == 32 ? 500.0 : w == 64 ? 620.0 : 900.0) + (double)rounds * w * 10 +
+      const double cost = (double)rounds * span * (w == 32 ? (x_tma ? 500.0 : 700.0) : w == 64 ? (x_tma ? 620.0 : 1100.0) : 900.0) + (double)rounds * w * 10 +
                           (log2 == 0 ? 0.0 : log2 == 1 ? 2500.0 : 3500.0);
       if (cost < best) {
         best = cost;
@@ -215,7 +216,6 @@ static int launch_w4_umma(UmmaArgs a, cudaStream_t st) {
   if (a.k > 0 && (rc = make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_INT64, 8, a.packed, row_words, w4_row_blocks(a.m), row_words,
                                 kTile / 8, 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return rc;
-  a.x_tma = a.k > 0 && a.ldb % 8 == 0 && aligned16(a.B);
   if (a.x_tma &&
       (rc = make_map(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                      2, a.B, a.k, a.n, a.ldb, 64, NT)))
@@ -243,8 +243,9 @@ static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* pa
   const unsigned char* w = static_cast<const unsigned char*>(packed);
   if (n <= 8) return dispatch_w4_gemv<T>(GemvArgs{m, n, k, ldb, ldc, alpha, beta, w, B, C}, f, st);
   int nt = 0, split_log2 = 0;
-  plan_umma(m, n, k, &nt, &split_log2);
-  const UmmaArgs a{m, n, k, ldb, ldc, alpha, beta, w, B, C, split_log2};
+  const bool x_tma = k > 0 && ldb % 8 == 0 && aligned16(B);
+  plan_umma(m, n, k, x_tma, &nt, &split_log2);
+  const UmmaArgs a{m, n, k, ldb, ldc, alpha, beta, w, B, C, split_log2, x_tma};
   if (nt == 32) return dispatch_w4_umma<T, 32>(a, f, st);
   if (nt == 64) return dispatch_w4_umma<T, 64>(a, f, st);
   return dispatch_w4_umma<T, 128>(a, f, st);

@@ -58,16 +58,26 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 
 // Elements at .. at + 7 of an array of `len`, zero behind its end, as they lie in memory; the array starts on any 2-byte
 // boundary.  Off the 16-byte boundaries two aligned loads are shifted together (eight loads of two bytes took four times
-// as long); nothing outside the array is read.
-template <typename T>
-__device__ __forceinline__ uint4 load8(const T* array, long long len, long long at) {
-  if (at + 8 <= len) {
-    const T* p = array + at;
-    const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15u);
-    if (off == 0) return *reinterpret_cast<const uint4*>(p);
-    if (2 * at >= off && at + 16 - off / 2 <= len) {
-      const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
-      const uint4 u = q[0], v = q[1];
+// as long); nothing outside the array is read.  In two steps, so that several can be under way at a time.
+struct Load8 {
+  uint4 u, v;
+  int off;    // bytes past the boundary
+  bool fast;
+  template <typename T>
+  __device__ __forceinline__ void issue(const T* array, long long len, long long at) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(array + at);
+    off = (int)(p & 15u);
+    fast = 2 * at >= off && at + (off ? 16 - off / 2 : 8) <= len;
+    if (fast) {
+      const uint4* q = reinterpret_cast<const uint4*>(p & ~(uintptr_t)15);
+      u = q[0];
+      if (off) v = q[1];
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ uint4 finish(const T* array, long long len, long long at) const {
+    if (fast) {
+      if (off == 0) return u;
       const bool two = off & 8, one = off & 4;
       const uint32_t w0 = two ? u.z : u.x, w1 = two ? u.w : u.y, w2 = two ? v.x : u.z, w3 = two ? v.y : u.w,
                      w4 = two ? v.z : v.x, w5 = two ? v.w : v.y;
@@ -76,11 +86,17 @@ __device__ __forceinline__ uint4 load8(const T* array, long long len, long long 
       return make_uint4(__funnelshift_r(a0, a1, bits), __funnelshift_r(a1, a2, bits), __funnelshift_r(a2, a3, bits),
                         __funnelshift_r(a3, a4, bits));
     }
-  }
-  __align__(16) T v[8];
+    __align__(16) T e[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = at + i < len ? array[at + i] : from_f32<T>(0.f);
-  return *reinterpret_cast<const uint4*>(v);
+    for (int i = 0; i < 8; ++i) e[i] = at + i < len ? array[at + i] : from_f32<T>(0.f);
+    return *reinterpret_cast<const uint4*>(e);
+  }
+};
+template <typename T>
+__device__ __forceinline__ uint4 load8(const T* array, long long len, long long at) {
+  Load8 l;
+  l.issue(array, len, at);
+  return l.finish(array, len, at);
 }
 
 // ---------------------------------------------------------------- writing the format --

@@ -3,9 +3,8 @@
 // A block computes 128 rows x NT columns.  The weights never exist in 16 bits outside tensor memory:
 //   warp 0      feeds: TMA loads of the packed tiles (8 row blocks in one) and of the activations (128 x NT) into a ring
 //   warp 1      issues the products: A (the unpacked weights) from tensor memory, B (the activations) from shared memory
-//   warps 2, 3  stand in for TMA where the activations are not aligned for it
 //   unpackers   (4 or 8 warps) turn codes into exact integers q - z in the activations' type and write them to tensor
-//               memory, thread = row
+//               memory, thread = row; where the activations are not aligned for TMA they bring those, too
 //   drainers    (4 or 8 warps) take each group's sums out of tensor memory, multiply by the group's scale and add them to
 //               the tile's sums in fp32 registers: the scales never meet a 16-bit rounding
 // Bounds: with few columns the codes' bytes (a 128 x 128 tile is 8.4 KB, 365 cycles of an SM's share of the memory); with
@@ -155,8 +154,8 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(smem_u32(&full_bars[s]), a.x_tma ? 1 : 3);  // the feeder, and the two warps that stand in for TMA
-      mbar_init(smem_u32(&empty_bars[s]), 5);               // four unpackers and the products
+      mbar_init(smem_u32(&full_bars[s]), 1);
+      mbar_init(smem_u32(&empty_bars[s]), 5);  // four unpackers and the products
     }
     for (int i = 0; i < kUmmaASlots; ++i) {
       mbar_init(smem_u32(&a_full[i]), 4);
@@ -262,36 +261,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
           phase ^= 1u;
         }
       }
-  } else if (warp < 4) {
-    // ---- activations that TMA cannot address
-    if (!a.x_tma) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int tile = first; ok && tile < a.tiles; tile += step) {
-        const int row_tile = tile / a.col_tiles, col0 = (tile - row_tile * a.col_tiles) * NT;
-        for (int i = 0; ok && i < span; ++i) {
-          ok = mbar_wait_together(smem_u32(&empty_bars[stage]), phase ^ 1u, &abort_flag, kFaultWaitEmpty, 0x4c20u);
-          if (!ok) break;
-          unsigned char* xs = smem_raw + (smem + stage * S::kXBytes - smem_u32(smem_raw));
-#pragma unroll 4
-          for (int p = (warp - 2) * 32 + lane; p < NT * 16; p += 64) {
-            const int row = p >> 4, chunk = p & 15;  // 16-byte chunks of a column's 128 elements
-            const size_t col = (size_t)col0 + row;
-            *reinterpret_cast<uint4*>(xs + (chunk >> 3) * (NT * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
-                load8(static_cast<const T*>(a.B) + col * a.ldb, col < a.n ? (long long)a.k : 0,
-                      (long long)(t0 + i) * kW4Cols + chunk * 8);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&full_bars[stage]));
-          if (++stage == a.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-    }
-  } else if (warp < 4 + 4 * S::kUnpackSets) {
+  } else if (warp >= 4 && warp < 4 + 4 * S::kUnpackSets) {
     // ---- unpackers: thread = row of the tile
     const int set = (warp - 4) / 4, row = (warp & 3) * 32 + lane, r = row & 15;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -328,6 +298,31 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
         }
         tmem_st_32x32(a_cols + slot * 64 + half * 32 + lane_base, w);
       }
+      if (!a.x_tma) {
+        // 16-byte chunks of 128 elements of a column, four under way at a time
+        const int tile = first + i / span * step, col0 = tile % a.col_tiles * NT;
+        unsigned char* xs = smem_raw + (smem + stage * S::kXBytes - smem_u32(smem_raw));
+#pragma unroll 1
+        for (int p0 = (warp & 3) * 32 + lane; p0 < NT * 16; p0 += 512) {
+          Load8 l[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int p = p0 + b * 128;
+            const size_t col = (size_t)col0 + (p >> 4);
+            l[b].issue(static_cast<const T*>(a.B) + col * a.ldb, col < a.n ? (long long)a.k : 0,
+                       (long long)(t0 + i % span) * kW4Cols + (p & 15) * 8);
+          }
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int p = p0 + b * 128, row_x = p >> 4, chunk = p & 15;
+            const size_t col = (size_t)col0 + row_x;
+            *reinterpret_cast<uint4*>(xs + (chunk >> 3) * (NT * 128) + row_x * 128 + (((chunk & 7) ^ (row_x & 7)) << 4)) =
+                l[b].finish(static_cast<const T*>(a.B) + col * a.ldb, col < a.n ? (long long)a.k : 0,
+                            (long long)(t0 + i % span) * kW4Cols + chunk * 8);
+          }
+        }
+        fence_proxy_async_smem();
+      }
       tmem_st_wait();
       tcgen05_fence_before();
       __syncwarp();
@@ -341,7 +336,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
         phase ^= 1u;
       }
     }
-  } else {
+  } else if (warp >= 4) {
     // ---- drainers: thread = row of the tile
     const int part = (warp - 4 - 4 * S::kUnpackSets) / 4, row = (warp & 3) * 32 + lane, r = row & 15;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
