@@ -251,16 +251,20 @@ static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* pa
   return dispatch_w4_umma<T, 128>(a, f, st);
 }
 
-// Workspace of the expert layer: expert numbers and gates (where the caller takes none), hidden vectors.
+// Workspace of the expert layer, for a pass of at most kMoeTokens tokens.
 struct MoeWorkspace {
-  size_t ids, gates, hidden, total;
+  size_t scores, x, hidden, peak, plan, total;
 };
-static MoeWorkspace moe_workspace(size_t tokens, size_t f, size_t topk) {
+static MoeWorkspace moe_workspace(size_t tokens, size_t d, size_t f, size_t experts, size_t topk) {
+  if (tokens > (size_t)kMoeTokens) tokens = kMoeTokens;
+  const size_t pairs = tokens * topk;
   MoeWorkspace w;
-  w.ids = 0;
-  w.gates = align_up(tokens * topk * 4, 256);
-  w.hidden = w.gates + align_up(tokens * topk * 4, 256);
-  w.total = w.hidden + align_up(tokens * topk * f * 4, 256);
+  w.scores = 0;
+  w.x = w.scores + align_up(tokens * experts * 4, 256);
+  w.hidden = w.x + align_up(tokens * align_up(d, 128) * 2, 256);
+  w.peak = w.hidden + align_up(pairs * align_up(f, 128) * 4, 256);
+  w.plan = w.peak + align_up(pairs * 4, 256);
+  w.total = w.plan + align_up((size_t)MoePlan::words((int)experts, (int)pairs) * 4, 256);
   return w;
 }
 
@@ -272,16 +276,31 @@ static int check_moe_sizes(int dtype, size_t tokens, size_t d, size_t f, size_t 
   return MMBO_OK;
 }
 
-template <typename T>
-static int run_moe(const MoeArgs& a, cudaStream_t st) {
-  moe_route_kernel<T><<<(unsigned)a.tokens, 256, a.experts * 4, st>>>(a);
+template <typename T, bool W4>
+static int launch_moe(const MoeArgs& a, cudaStream_t st) {
+  const size_t pairs = (size_t)a.tokens * a.topk, words = MoePlan::words(a.experts, (int)pairs);
+  const size_t up_smem = align_up((words + pairs + a.experts) * 4, 16) + 2 * kMoeWarps * 256 * 4;
+  const size_t down_smem = align_up(words * 4, 16) + (size_t)kMoeWarps * a.tokens * 16 * 4;
+  auto up = moe_up_kernel<T, W4>;
+  auto down = moe_down_kernel<T, W4>;
+  static bool up_ready[kMaxDevices], down_ready[kMaxDevices];
+  int rc;
+  if ((rc = allow_smem(up, kGemvSmem, up_ready)) || (rc = allow_smem(down, kGemvSmem, down_ready))) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.experts + 7) / 8), (unsigned)a.tokens);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = settings().pdl ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
   MMBO_COUNT_LAUNCH();
-  const unsigned pairs = (unsigned)(a.tokens * a.topk);
-  moe_up_simple_kernel<T><<<dim3((unsigned)((a.f + 7) / 8), pairs), 256, 0, st>>>(a);
-  MMBO_COUNT_LAUNCH();
-  moe_down_simple_kernel<T><<<dim3((unsigned)((a.d + 7) / 8), (unsigned)a.tokens), 256, 0, st>>>(a);
-  MMBO_COUNT_LAUNCH();
-  return (int)cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  if ((rc = launch_clustered(up, (unsigned)sm_count(), kMoeThreads, up_smem, 0, st, a))) return rc;
+  const int blocks = (a.d + 15) / 16;
+  return launch_clustered(down, (unsigned)(blocks < sm_count() ? blocks : sm_count()), kMoeThreads, down_smem, 0, st, a);
 }
 
 }  // namespace mmbo
@@ -392,7 +411,7 @@ int mmbo_moe_workspace_bytes(int dtype, size_t tokens, size_t d, size_t f, size_
   int rc = check_moe_sizes(dtype, tokens, d, f, experts, topk);
   if (rc) return rc;
   if (!bytes) return MMBO_ERR_NULL_POINTER;
-  *bytes = moe_workspace(tokens, f, topk).total;
+  *bytes = moe_workspace(tokens, d, f, experts, topk).total;
   return MMBO_OK;
 }
 
@@ -426,14 +445,49 @@ int mmbo_moe(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_
   if (!aligned_to(X, 2) || !aligned_to(router, 2) || !aligned_to(Y, 2) || !aligned_to(ids, 4) ||
       !aligned_to(gates, 4) || !aligned_to(workspace, 256))
     return MMBO_ERR_MISALIGNED;
-  const MoeWorkspace ws = moe_workspace(tokens, f, topk);
+  const MoeWorkspace ws = moe_workspace(tokens, d, f, experts, topk);
   if (workspaceBytes < ws.total) return MMBO_ERR_WORKSPACE;
   char* base = static_cast<char*>(workspace);
-  MoeArgs a{tokens, d, f, experts, topk, renorm, fmt, X, router, gate, up, down, ldx, ldr, ldg, strideG, ldd, strideD,
-            *beta, Y, ldy, ids ? ids : reinterpret_cast<int*>(base + ws.ids),
-            gates ? gates : reinterpret_cast<float*>(base + ws.gates), reinterpret_cast<float*>(base + ws.hidden)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == MMBO_DTYPE_F16 ? run_moe<__half>(a, st) : run_moe<__nv_bfloat16>(a, st);
+  for (size_t t0 = 0; t0 < tokens; t0 += kMoeTokens) {
+    const size_t n = tokens - t0 < (size_t)kMoeTokens ? tokens - t0 : (size_t)kMoeTokens;
+    MoeArgs a{};
+    a.tokens = (int)n;
+    a.d = (int)d;
+    a.f = (int)f;
+    a.experts = (int)experts;
+    a.topk = (int)topk;
+    a.renorm = renorm;
+    a.fmt = fmt;
+    a.X = static_cast<const char*>(X) + t0 * ldx * 2;
+    a.router = router;
+    a.gate = gate;
+    a.up = up;
+    a.down = down;
+    a.ldx = ldx;
+    a.ldr = ldr;
+    a.ldg = ldg;
+    a.strideG = strideG;
+    a.ldd = ldd;
+    a.strideD = strideD;
+    a.beta = *beta;
+    a.Y = static_cast<char*>(Y) + t0 * ldy * 2;
+    a.ldy = ldy;
+    a.ids = ids ? ids + t0 * topk : nullptr;
+    a.gates = gates ? gates + t0 * topk : nullptr;
+    a.scores = reinterpret_cast<float*>(base + ws.scores);
+    a.x = base + ws.x;
+    a.hidden = base + ws.hidden;
+    a.peak = reinterpret_cast<uint32_t*>(base + ws.peak);
+    a.plan = reinterpret_cast<int*>(base + ws.plan);
+    a.d_pad = (int)align_up(d, 128);
+    a.f_pad = (int)align_up(f, 128);
+    a.hidden_f32 = group == 0 && dtype == MMBO_DTYPE_F16;
+    if (dtype == MMBO_DTYPE_F16) rc = group ? launch_moe<__half, true>(a, st) : launch_moe<__half, false>(a, st);
+    else rc = group ? launch_moe<__nv_bfloat16, true>(a, st) : launch_moe<__nv_bfloat16, false>(a, st);
+    if (rc) return rc;
+  }
+  return MMBO_OK;
 }
 
 }  // extern "C"

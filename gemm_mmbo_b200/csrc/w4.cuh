@@ -273,31 +273,4 @@ __global__ void w4_unpack_kernel(size_t m, size_t k, W4Format f, const unsigned 
   }
 }
 
-// ---------------------------------------------------------------- the product ---------
-// Sum over k of row i of a packed matrix times x, in 32 bits, by one warp (the result is in every lane).
-template <typename T>
-__device__ __forceinline__ float w4_row_dot(const unsigned char* __restrict__ packed, W4Format f, size_t i, size_t k,
-                                            const T* __restrict__ x) {
-  const size_t tiles = w4_k_tiles(k);
-  const int lane = threadIdx.x & 31, half = lane >> 4, t = (lane >> 2) & 3, u = lane & 3;
-  const int row = (int)(i % kW4Rows), g = 32 * u / f.group;
-  float acc = 0.f;
-  for (size_t tile = half; tile < tiles; tile += 2) {
-    const unsigned char* in = packed + (i / kW4Rows * tiles + tile) * f.tile_bytes();
-    const uint32_t w = __ldg(reinterpret_cast<const unsigned int*>(in + w4_piece(row, t) + u * 4));
-    const float s = to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row)));
-    const int z = f.zeros ? in[f.zero_at(g, row)] : 8;
-    float part = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const size_t j = tile * kW4Cols + 32 * u + 8 * t + e;
-      if (j < k) part = fmaf((float)((int)((w >> (4 * w4_nibble(e))) & 15u) - z), to_f32(x[j]), part);
-    }
-    acc = fmaf(s, part, acc);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  return acc;
-}
-
 }  // namespace mmbo
