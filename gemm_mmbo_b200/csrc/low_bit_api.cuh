@@ -251,17 +251,19 @@ static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* pa
   return dispatch_w4_umma<T, 128>(a, f, st);
 }
 
-// Workspace of the expert layer, for a pass of at most kMoeTokens tokens.
+// Workspace of the expert layer, for one pass.
 struct MoeWorkspace {
-  size_t scores, x, hidden, peak, plan, total;
+  size_t scores, x, x_sums, x_undo, hidden, peak, plan, total;
 };
 static MoeWorkspace moe_workspace(size_t tokens, size_t d, size_t f, size_t experts, size_t topk) {
-  if (tokens > (size_t)kMoeTokens) tokens = kMoeTokens;
+  if (tokens > (size_t)moe_pass_tokens((int)topk)) tokens = moe_pass_tokens((int)topk);
   const size_t pairs = tokens * topk;
   MoeWorkspace w;
   w.scores = 0;
   w.x = w.scores + align_up(tokens * experts * 4, 256);
-  w.hidden = w.x + align_up(tokens * align_up(d, 128) * 2, 256);
+  w.x_sums = w.x + align_up(tokens * align_up(d, 128) * 2, 256);
+  w.x_undo = w.x_sums + align_up(tokens * (align_up(d, 128) / 32) * 4, 256);
+  w.hidden = w.x_undo + align_up(tokens * 8, 256);
   w.peak = w.hidden + align_up(pairs * align_up(f, 128) * 4, 256);
   w.plan = w.peak + align_up(pairs * 4, 256);
   w.total = w.plan + align_up((size_t)MoePlan::words((int)experts, (int)pairs) * 4, 256);
@@ -276,18 +278,21 @@ static int check_moe_sizes(int dtype, size_t tokens, size_t d, size_t f, size_t 
   return MMBO_OK;
 }
 
-template <typename T, bool W4>
+template <typename T, int QG>
 static int launch_moe(const MoeArgs& a, cudaStream_t st) {
+  using Up = MoeUpShape<QG>;
+  using Down = MoeDownShape<QG>;
   const size_t pairs = (size_t)a.tokens * a.topk, words = MoePlan::words(a.experts, (int)pairs);
-  const size_t up_smem = align_up((words + pairs + a.experts) * 4, 16) + 2 * kMoeWarps * 256 * 4;
-  const size_t down_smem = align_up(words * 4, 16) + (size_t)kMoeWarps * a.tokens * 16 * 4;
-  auto up = moe_up_kernel<T, W4>;
-  auto down = moe_down_kernel<T, W4>;
+  const size_t up_smem = (size_t)kMoeWarps * Up::kSlots * Up::kSlot + kMoeUpSums + (words + pairs + a.experts) * 4;
+  const size_t down_smem = (size_t)kMoeWarps * (Down::kSlots * Down::kSlot + a.tokens * 16 * 4) + words * 4;
+  if (up_smem > kGemvSmem || down_smem > kGemvSmem) return MMBO_ERR_TOO_LARGE;
+  auto up = moe_up_kernel<T, QG>;
+  auto down = moe_down_kernel<T, QG>;
   static bool up_ready[kMaxDevices], down_ready[kMaxDevices];
   int rc;
   if ((rc = allow_smem(up, kGemvSmem, up_ready)) || (rc = allow_smem(down, kGemvSmem, down_ready))) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.experts + 7) / 8), (unsigned)a.tokens);
+  cfg.gridDim = dim3((unsigned)((a.experts + 7) / 8 + 1), (unsigned)a.tokens);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -295,12 +300,22 @@ static int launch_moe(const MoeArgs& a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = settings().pdl ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
   MMBO_COUNT_LAUNCH();
   if (e != cudaSuccess) return (int)e;
   if ((rc = launch_clustered(up, (unsigned)sm_count(), kMoeThreads, up_smem, 0, st, a))) return rc;
   const int blocks = (a.d + 15) / 16;
   return launch_clustered(down, (unsigned)(blocks < sm_count() ? blocks : sm_count()), kMoeThreads, down_smem, 0, st, a);
+}
+
+template <typename T>
+static int run_moe(const MoeArgs& a, cudaStream_t st) {
+  switch (a.fmt.group) {
+    case 0: return launch_moe<T, 0>(a, st);
+    case 32: return launch_moe<T, 1>(a, st);
+    case 64: return launch_moe<T, 2>(a, st);
+    default: return launch_moe<T, 4>(a, st);
+  }
 }
 
 }  // namespace mmbo
@@ -449,8 +464,9 @@ int mmbo_moe(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_
   if (workspaceBytes < ws.total) return MMBO_ERR_WORKSPACE;
   char* base = static_cast<char*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  for (size_t t0 = 0; t0 < tokens; t0 += kMoeTokens) {
-    const size_t n = tokens - t0 < (size_t)kMoeTokens ? tokens - t0 : (size_t)kMoeTokens;
+  const size_t pass = moe_pass_tokens((int)topk);
+  for (size_t t0 = 0; t0 < tokens; t0 += pass) {
+    const size_t n = tokens - t0 < pass ? tokens - t0 : pass;
     MoeArgs a{};
     a.tokens = (int)n;
     a.d = (int)d;
@@ -477,14 +493,15 @@ int mmbo_moe(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_
     a.gates = gates ? gates + t0 * topk : nullptr;
     a.scores = reinterpret_cast<float*>(base + ws.scores);
     a.x = base + ws.x;
+    a.x_sums = reinterpret_cast<float*>(base + ws.x_sums);
+    a.x_undo = reinterpret_cast<float2*>(base + ws.x_undo);
     a.hidden = base + ws.hidden;
     a.peak = reinterpret_cast<uint32_t*>(base + ws.peak);
     a.plan = reinterpret_cast<int*>(base + ws.plan);
     a.d_pad = (int)align_up(d, 128);
     a.f_pad = (int)align_up(f, 128);
     a.hidden_f32 = group == 0 && dtype == MMBO_DTYPE_F16;
-    if (dtype == MMBO_DTYPE_F16) rc = group ? launch_moe<__half, true>(a, st) : launch_moe<__half, false>(a, st);
-    else rc = group ? launch_moe<__nv_bfloat16, true>(a, st) : launch_moe<__nv_bfloat16, false>(a, st);
+    rc = dtype == MMBO_DTYPE_F16 ? run_moe<__half>(a, st) : run_moe<__nv_bfloat16>(a, st);
     if (rc) return rc;
   }
   return MMBO_OK;

@@ -8,15 +8,18 @@
 //
 // What bounds it: the bytes of the experts that the tokens choose.  Three kernels in one stream, each started while the
 // one in front drains (programmatic dependent launch):
-//   scores   one warp per (token, expert); also an aligned, zero-padded copy of the activations
+//   scores   one warp per (token, expert); also an aligned, zero-padded copy of the activations (for 4-bit experts in half
+//            precision with the groups' sums, as w4_tile_mma wants them)
 //   up       every block repeats the selection for itself (a microsecond, cheaper than another kernel and its launch), then
 //            works through its share of the units (expert, 16 rows of gate and up): sixteen warps split d
 //   down     a block owns 16 rows of the output for all tokens, its warps split the list of (expert, part of f); the sums
 //            of the experts meet in shared memory in a fixed order
-// Weights go straight from memory to registers, in the order of the fragments of mma.sync.m16n8k16: a lane reads 16 bytes
-// of a row and the same 16 bytes' worth of k of its token, so that nothing is staged, and a warp has its next 64 columns
-// (4 or 8 KB) under way while it multiplies.  Tokens are the eight columns of the instruction; an expert with more
-// tokens is taken in groups of eight, the later ones finding its weights in L2.
+// Each warp has a ring in shared memory that its lanes fill with 16-byte asynchronous copies of weights, every lane with
+// the pieces that it will itself read as fragments of mma.sync.m16n8k16, so the ring needs no barrier and the copies in
+// flight no registers; the columns come straight from L2, the same 16 bytes' worth of k of a lane's token, asked for
+// before the wait for the weights.  (Weights loaded straight to registers one step ahead left 64 KB in flight an SM at
+// best: 255 us for the batch of 48 tokens in `up`, 2.9 TB/s.)  Tokens are the eight columns of the instruction; an expert with more tokens is taken in groups of
+// eight, the later ones finding its weights in L2.
 #pragma once
 
 #include "w4_umma.cuh"
@@ -24,7 +27,8 @@
 namespace mmbo {
 
 constexpr int kMoeWarps = 16, kMoeThreads = kMoeWarps * 32;
-constexpr int kMoeTokens = 64;  // of one pass; more are taken in several
+// Tokens of one pass (more are taken in several): what the plan and the sums of `down` leave room for in shared memory.
+__host__ __device__ constexpr int moe_pass_tokens(int topk) { return 512 / topk < 64 ? 512 / topk : 64; }
 
 struct MoeArgs {
   int tokens, d, f, experts, topk, renorm;
@@ -38,7 +42,9 @@ struct MoeArgs {
   float* gates;  // tokens x topk, the caller's or null
   // workspace
   float* scores;    // tokens x experts
-  void* x;          // tokens x d_pad: the activations, zero behind d
+  void* x;          // tokens x d_pad: the activations, zero behind d (4-bit experts: in half precision, scaled)
+  float* x_sums;    // 4-bit experts: tokens x (d_pad / group) sums of these, in units of 2^20
+  float2* x_undo;   // 4-bit experts: two factors a token that undo its scale and the unit of 2^20
   void* hidden;     // pairs x f_pad: floats, or bfloat16 twice (the value and what its rounding left)
   uint32_t* peak;   // pairs: bits of the largest hidden magnitude
   int* plan;        // what `up` found out for `down`, see MoePlan
@@ -78,28 +84,77 @@ __device__ __forceinline__ uint32_t moe_score_key(float v) {
 
 template <typename T>
 __global__ void __launch_bounds__(256) moe_scores_kernel(const MoeArgs a) {
+  __shared__ uint32_t peak;
   griddep_launch_dependents();
+  if (threadIdx.x == 0) peak = 0;
+  __syncthreads();
   griddep_wait();
-  const int t = blockIdx.y, e = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int t = blockIdx.y, lane = threadIdx.x & 31;
   const T* x = static_cast<const T*>(a.X) + (size_t)t * a.ldx;
-  if (blockIdx.x == 0) {
-    T* copy = static_cast<T*>(a.x) + (size_t)t * a.d_pad;
-    for (int j = threadIdx.x * 8; j < a.d_pad; j += 256 * 8) *reinterpret_cast<uint4*>(copy + j) = load8(x, a.d, j);
+  if (blockIdx.x == gridDim.x - 1) {  // the last block of a token prepares the workspace instead
     for (int s = threadIdx.x; s < a.topk; s += 256) a.peak[t * a.topk + s] = 0;
     // hidden vectors behind f: floats, or two rows of bfloat16 (zero bytes either way)
     uint16_t* h = static_cast<uint16_t*>(a.hidden) + (size_t)t * a.topk * a.f_pad * 2;
-    const int pad = a.f_pad - a.f, per = a.hidden_f32 ? 1 : 2, width = a.hidden_f32 ? 2 : 1;
-    for (int i = threadIdx.x; i < a.topk * per * pad * width; i += 256) {
-      const int row = i / (pad * width), at = i % (pad * width);
-      h[(size_t)row * a.f_pad * width + a.f * width + at] = 0;
+    const int per = a.hidden_f32 ? 1 : 2, width = a.hidden_f32 ? 2 : 1, pad = (a.f_pad - a.f) * width;
+    for (int i = threadIdx.x; i < a.topk * per * pad; i += 256)
+      h[(size_t)(i / pad) * a.f_pad * width + a.f * width + i % pad] = 0;
+    if (!a.fmt.group) {
+      T* copy = static_cast<T*>(a.x) + (size_t)t * a.d_pad;
+      for (int j = threadIdx.x * 8; j < a.d_pad; j += 256 * 8) *reinterpret_cast<uint4*>(copy + j) = load8(x, a.d, j);
+      return;
     }
+    float f1 = 1.f, f2 = 1.f;
+    if (!std::is_same<T, __half>::value) {
+      // exponent of the largest magnitude (below the normal range: the smallest normal one), 2^(14 - e) as a product
+      uint32_t top = 0;
+      for (int j = threadIdx.x * 8; j < a.d; j += 256 * 8) {
+        const uint4 v = load8(x, a.d, j);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, max(w[i] << 16 & 0x7fffffffu, w[i] & 0x7fff0000u));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) atomicMax(&peak, top);
+      __syncthreads();
+      const int up = 14 - ((int)max(peak >> 23, 1u) - 127), up1 = min(max(up, -100), 100), up2 = up - up1;
+      f1 = __uint_as_float((uint32_t)(up1 + 127) << 23);
+      f2 = __uint_as_float((uint32_t)(up2 + 127) << 23);
+      if (threadIdx.x == 0)
+        a.x_undo[t] = peak < 0x7f800000u ? make_float2(__uint_as_float((uint32_t)(127 - up1) << 23),
+                                                       __uint_as_float((uint32_t)(127 - up2 + 20) << 23))
+                                         : make_float2(__int_as_float(0x7fc00000), 0.f);
+    } else if (threadIdx.x == 0) {
+      a.x_undo[t] = make_float2(1.f, 0x1p20f);
+    }
+    __half* copy = static_cast<__half*>(a.x) + (size_t)t * a.d_pad;
+    const int lanes = a.fmt.group / 8;  // neighbouring threads that hold a group
+    for (int j0 = 0; j0 < a.d_pad; j0 += 256 * 8) {
+      const int j = j0 + threadIdx.x * 8;
+      const uint4 v = load8(x, a.d, j);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      uint32_t out[4];
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 e = widen2<T>(w[i]);
+        const __half2 c = __floats2half2_rn(e.x * f1 * f2, e.y * f1 * f2);
+        out[i] = *reinterpret_cast<const uint32_t*>(&c);
+        const float2 back = __half22float2(c);
+        sum += back.x + back.y;
+      }
+      for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (j < a.d_pad) {
+        *reinterpret_cast<uint4*>(copy + j) = make_uint4(out[0], out[1], out[2], out[3]);
+        if (threadIdx.x % lanes == 0) a.x_sums[(size_t)t * (a.d_pad / a.fmt.group) + j / a.fmt.group] = sum * 0x1p-20f;
+      }
+    }
+    return;
   }
+  const int e = blockIdx.x * 8 + threadIdx.x / 32;
   if (e >= a.experts) return;
   const T* w = static_cast<const T*>(a.router) + (size_t)e * a.ldr;
   float sum = 0.f;
-#pragma unroll 4
-  for (int j = lane * 8; j < a.d; j += 256) {
-    const uint4 u = load8(w, a.d, j), v = load8(x, a.d, j);
+  auto dot = [&](const uint4& u, const uint4& v) {
     const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -107,15 +162,33 @@ __global__ void __launch_bounds__(256) moe_scores_kernel(const MoeArgs a) {
       sum = fmaf(p.x, q.x, sum);
       sum = fmaf(p.y, q.y, sum);
     }
+  };
+  if (a.d % 8 == 0 && ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(x)) & 15u) == 0) {
+    for (int j = lane * 8; j < a.d; j += 8 * 256) {  // eight pieces of each under way at a time
+      uint4 u[8], v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool have = j + i * 256 < a.d;
+        u[i] = have ? *reinterpret_cast<const uint4*>(w + j + i * 256) : make_uint4(0, 0, 0, 0);
+        v[i] = have ? *reinterpret_cast<const uint4*>(x + j + i * 256) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot(u[i], v[i]);
+    }
+  } else {
+    for (int j = lane * 8; j < a.d; j += 256) dot(load8(w, a.d, j), load8(x, a.d, j));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) a.scores[(size_t)t * a.experts + e] = sum;
 }
 
-// The topk experts of one token by one warp: ids and gates (shared memory).
-__device__ __forceinline__ void moe_select(const MoeArgs& a, const float* scores, int* ids, float* gates) {
+// The topk experts of one token by one warp: ids and gates (shared memory); `scores`: room for the experts' scores in
+// shared memory (read once from memory: each of the topk rounds would wait for it again).
+__device__ __forceinline__ void moe_select(const MoeArgs& a, const float* from, float* scores, int* ids, float* gates) {
   const int lane = threadIdx.x & 31;
+  for (int e = lane; e < a.experts; e += 32) scores[e] = from[e];
+  __syncwarp();
   float top = -INFINITY, sum = 0.f;
   for (int e = lane; e < a.experts; e += 32) top = fmaxf(top, scores[e]);
 #pragma unroll
@@ -167,89 +240,95 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Sixteen rows of 16-bit weights, 64 columns at a time: lane 4 r + t holds columns 32 u + 8 t .. + 7 of rows r and r + 8.
-// `rows` that exist; the others and what lies behind `k` are zero.
-template <typename T>
-struct Rows16 {
-  static constexpr int kStep = 64;
-  uint4 w[2][2];
-  __device__ __forceinline__ void load(const T* base, size_t ld, int rows, int k, int step, bool vec) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const T* row = base + (size_t)(r + 8 * h) * ld;
-      const bool have = r + 8 * h < rows;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int j = step * 64 + u * 32 + t * 8;
-        if (vec) {
-          w[h][u] = have && j < k ? __ldcs(reinterpret_cast<const uint4*>(row + j)) : make_uint4(0, 0, 0, 0);
-        } else {
-          w[h][u] = load8(row, have ? k : 0, j);
-        }
-      }
-    }
-  }
-  // acc += weights * columns; b: this lane's 16 bytes of each 32 columns
-  __device__ __forceinline__ void multiply(float (&acc)[4], const uint4 (&b)[2]) const {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      mma_16816<T>(acc, w[0][u].x, w[1][u].x, w[0][u].y, w[1][u].y, b[u].x, b[u].y);
-      mma_16816<T>(acc, w[0][u].z, w[1][u].z, w[0][u].w, w[1][u].w, b[u].z, b[u].w);
-    }
-  }
-};
+// ---------------------------------------------------------------- rings ---------------
+// 16 bytes to shared memory, in the background; zeros where `have` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool have) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most N of the groups committed are under way.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 
-// Sixteen rows of packed weights, a tile of 128 columns at a time; U: the 16-bit type the products are formed in, S: the
-// scales'.
-template <typename S, typename U>
-struct Rows4 {
-  static constexpr int kStep = 128;
-  uint4 c[2];
-  uint32_t scale[4], zero[4];  // rows r and r + 8, by group
-  __device__ __forceinline__ void load(const unsigned char* tile, const W4Format& f) {
-    const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3, groups = f.groups();
-    c[0] = __ldcs(reinterpret_cast<const uint4*>(tile + w4_piece(r, t)));
-    c[1] = __ldcs(reinterpret_cast<const uint4*>(tile + w4_piece(r, t) + 512));
+// Sixteen rows of 16-bit weights, 32 C columns: piece (h, u) of a lane, columns 32 u + 8 t .. + 7 of row r + 8 h, lies at
+// (h C + u) * 512 + lane * 16.  `rows` exist; the others, and columns behind k, are zero.
+template <typename T, int C>
+__device__ __forceinline__ void rows16_fetch(uint32_t to, const T* base, size_t ld, int rows, int k, int step, bool vec) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      if (g < groups) {
-        scale[g] = *reinterpret_cast<const uint32_t*>(tile + f.scale_at(g, r));
-        zero[g] = f.zeros ? *reinterpret_cast<const uint16_t*>(tile + f.zero_at(g, r)) : 0x0808u;
-      }
-  }
-  // acc += weights * (columns of every b[i])
-  template <int N>
-  __device__ __forceinline__ void multiply(float (&acc)[4], const uint4 (&b)[N][4], const W4Format& f) const {
-    const uint32_t w0[4] = {c[0].x, c[0].y, c[0].z, c[0].w}, w1[4] = {c[1].x, c[1].y, c[1].z, c[1].w};
-    const int per = f.group / 32;
-    W4Unpacker<U> lo, hi;
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int h = 0; h < 2; ++h) {
+    const bool have = r + 8 * h < rows;
+    const T* row = base + (size_t)(have ? r + 8 * h : 0) * ld;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int g = per == 4 ? 0 : per == 2 ? u >> 1 : u;
-      const uint32_t z = g == 0 ? zero[0] : g == 1 ? zero[1] : g == 2 ? zero[2] : zero[3];
-      lo.set_zero(z & 15u);
-      hi.set_zero(z >> 8 & 15u);
-      uint32_t p[4], q[4];
-      lo.unpack(w0[u], p);
-      hi.unpack(w1[u], q);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        mma_16816<U>(part, p[0], q[0], p[1], q[1], b[i][u].x, b[i][u].y);
-        mma_16816<U>(part, p[2], q[2], p[3], q[3], b[i][u].z, b[i][u].w);
-      }
-      if (u == 3 || per == 1 || (per == 2 && u == 1)) {  // the group is complete
-        const float2 s = widen2<S>(g == 0 ? scale[0] : g == 1 ? scale[1] : g == 2 ? scale[2] : scale[3]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[i] = fmaf(i < 2 ? s.x : s.y, part[i], acc[i]);
-          part[i] = 0.f;
-        }
-      }
+    for (int u = 0; u < C; ++u) {
+      const int j = (step * C + u) * 32 + t * 8;
+      const uint32_t dst = to + (h * C + u) * 512 + lane * 16;
+      if (vec) copy16(dst, row + (j < k ? j : 0), have && j < k);
+      else sts128(dst, load8(row, have ? k : 0, j));
     }
   }
-};
+}
+// acc += those weights * columns; b: this lane's 16 bytes of each 32 columns
+template <typename T, int C>
+__device__ __forceinline__ void rows16_multiply(uint32_t from, float (&acc)[4], const uint4 (&b)[C]) {
+  const uint32_t at = from + (threadIdx.x & 31) * 16;
+#pragma unroll
+  for (int u = 0; u < C; ++u) {
+    const uint4 lo = lds128(at + u * 512), hi = lds128(at + (C + u) * 512);
+    mma_16816<T>(acc, lo.x, hi.x, lo.y, hi.y, b[u].x, b[u].y);
+    mma_16816<T>(acc, lo.z, hi.z, lo.w, hi.w, b[u].z, b[u].w);
+  }
+}
+
+// A packed tile in its own layout: two pieces of codes a lane, scales and zero points by the first lanes from `lane0` on.
+// (Others read what a lane copied: __syncwarp() behind the wait.)
+__device__ __forceinline__ void tile_fetch(uint32_t to, const unsigned char* tile) {
+  const int lane = threadIdx.x & 31, at = w4_piece(lane >> 2, lane & 3);
+  copy16(to + at, tile + at, true);
+  copy16(to + at + 512, tile + at + 512, true);
+}
+__device__ __forceinline__ void tile_fetch_scales(uint32_t to, const unsigned char* tile, const W4Format& f, int i) {
+  if (i >= 0 && i * 16 < (int)f.tile_bytes() - kW4Codes) copy16(to + kW4Codes + i * 16, tile + kW4Codes + i * 16, true);
+}
+// acc += a packed tile * two bfloat16 columns' worth (a value and its remainder, by quarters).  Codes become exact integers:
+// for w4_tile_mma a hidden vector would first have to be brought to half precision.
+template <typename T, int QG>
+__device__ __forceinline__ void tile_multiply_bf16(uint32_t tile, const uint4 (&b)[2][4], bool zeros, float (&acc)[4]) {
+  using L = W4Tile<QG, true>;
+  const int lane = threadIdx.x & 31, r = lane >> 2;
+  const uint32_t codes = tile + w4_piece(r, lane & 3);
+  const uint4 c0 = lds128(codes), c1 = lds128(codes + 512);
+  const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+  W4Unpacker<__nv_bfloat16> lo, hi;
+#pragma unroll
+  for (int g = 0; g < L::kGroups; ++g) {
+    const uint32_t z = zeros ? lds16(tile + L::kZeros + g * 16 + r * 2) : 0x0808u;
+    lo.set_zero(z & 15u);
+    hi.set_zero(z >> 8 & 15u);
+    float part[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int qq = 0; qq < QG; ++qq) {
+      const int q = g * QG + qq;
+      uint32_t p[4], s[4];
+      lo.unpack(w0[q], p);
+      hi.unpack(w1[q], s);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mma_16816<__nv_bfloat16>(part[i], p[0], s[0], p[1], s[1], b[i][q].x, b[i][q].y);
+        mma_16816<__nv_bfloat16>(part[i], p[2], s[2], p[3], s[3], b[i][q].z, b[i][q].w);
+      }
+    }
+    const float2 s = widen2<T>(lds32(tile + L::kScales + g * 32 + r * 4));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(i < 2 ? s.x : s.y, part[0][i] + part[1][i], acc[i]);
+  }
+}
+constexpr uint32_t kTileRoom = kW4Codes + 4 * 48;  // of a tile in a ring, whatever its groups
 
 // The power of two that brings a vector whose largest magnitude has these bits below 2^15.
 __device__ __forceinline__ float moe_scale(uint32_t peak) {
@@ -258,23 +337,37 @@ __device__ __forceinline__ float moe_scale(uint32_t peak) {
 }
 
 // ---------------------------------------------------------------- up ------------------
-// Shared memory of both kernels: the plan, then partial sums.
-template <typename T, bool W4>
+// QG: quarters of a group of packed weights, 0: 16-bit weights.
+template <int QG>
+struct MoeUpShape {
+  static constexpr int kStep = QG ? 128 : 32;  // columns
+  static constexpr uint32_t kHalf = QG ? kTileRoom : 1024, kSlot = 2 * kHalf;  // gate, up
+  static constexpr int kSlots = QG ? 4 : 5;
+};
+constexpr size_t kMoeUpSums = (size_t)2 * kMoeWarps * 256 * 4;
+
+template <typename T, int QG>
 __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
+  using S = MoeUpShape<QG>;
+  constexpr bool W4 = QG > 0;
+  extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int pairs = a.tokens * a.topk;
-  MoePlan plan(reinterpret_cast<int*>(smem), a.experts, pairs);
-  int* ids = reinterpret_cast<int*>(smem) + MoePlan::words(a.experts, pairs);
+  // shared memory: rings | partial sums (before that: scores) | plan | ids | count
+  const uint32_t ring = smem_u32(smem) + warp * S::kSlots * S::kSlot;
+  float* sums = reinterpret_cast<float*>(smem + kMoeWarps * S::kSlots * S::kSlot);
+  int* at_plan = reinterpret_cast<int*>(sums) + kMoeUpSums / 4;
+  MoePlan plan(at_plan, a.experts, pairs);
+  int* ids = at_plan + MoePlan::words(a.experts, pairs);
   int* count = ids + pairs;  // experts
-  float* sums = reinterpret_cast<float*>(smem + ((size_t)(MoePlan::words(a.experts, pairs) + pairs + a.experts) * 4 + 15) / 16 * 16);
   griddep_launch_dependents();
+  for (int e = threadIdx.x; e < a.experts; e += kMoeThreads) count[e] = 0;
   griddep_wait();
 
   // the selection, by every block for itself
-  for (int e = threadIdx.x; e < a.experts; e += kMoeThreads) count[e] = 0;
-  for (int tok = warp; tok < a.tokens; tok += kMoeWarps)
-    moe_select(a, a.scores + (size_t)tok * a.experts, ids + tok * a.topk, plan.gate + tok * a.topk);
+  const int selecting = min(kMoeWarps, (int)(kMoeUpSums / 4) / a.experts);  // warps that have room for a token's scores
+  for (int tok = warp; warp < selecting && tok < a.tokens; tok += selecting)
+    moe_select(a, a.scores + (size_t)tok * a.experts, sums + warp * a.experts, ids + tok * a.topk, plan.gate + tok * a.topk);
   __syncthreads();
   for (int p = threadIdx.x; p < pairs; p += kMoeThreads) atomicAdd(&count[ids[p]], 1);
   __syncthreads();
@@ -311,7 +404,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < MoePlan::words(a.experts, pairs); i += kMoeThreads) a.plan[i] = reinterpret_cast<int*>(smem)[i];
+    for (int i = threadIdx.x; i < MoePlan::words(a.experts, pairs); i += kMoeThreads) a.plan[i] = at_plan[i];
     for (int p = threadIdx.x; p < pairs; p += kMoeThreads) {
       if (a.ids) a.ids[p] = ids[p];
       if (a.gates) a.gates[p] = plan.gate[p];
@@ -324,9 +417,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
   for (int i = 0; i < active; ++i) total += blocks * ((plan.start[i + 1] - plan.start[i] + 7) / 8);
   const int begin = (int)((long long)total * blockIdx.x / gridDim.x), end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
   struct Unit {
-    int index, rows, group, groups, left;  // expert (of the active ones), row block, group of tokens; units left of the expert
+    int index, rows, group, groups;  // expert (of the active ones), row block, group of tokens
   };
-  Unit unit{0, 0, 0, 0, 0};
+  Unit unit{0, 0, 0, 0};
   {
     int at = 0;
     for (; unit.index < active; ++unit.index) {
@@ -348,56 +441,74 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
     if (++u.index < active) u.groups = (plan.start[u.index + 1] - plan.start[u.index] + 7) / 8;
   };
 
-  using Stream = typename std::conditional<W4, Rows4<T, T>, Rows16<T>>::type;
-  constexpr int kStep = Stream::kStep;
-  const int steps = (a.d + kStep - 1) / kStep, s0 = steps * warp / kMoeWarps, s1 = steps * (warp + 1) / kMoeWarps;
+  const int steps = (a.d + S::kStep - 1) / S::kStep, s0 = steps * warp / kMoeWarps, s1 = steps * (warp + 1) / kMoeWarps;
   const bool vec = !W4 && a.ldg % 8 == 0 && a.strideG % 8 == 0 && a.d % 8 == 0 &&
                    ((reinterpret_cast<uintptr_t>(a.gate) | reinterpret_cast<uintptr_t>(a.up)) & 15u) == 0;
-  const int k_tiles = (a.d + 127) / 128;
-  auto load = [&](Stream& g, Stream& u, const Unit& at, int step) {
-    const size_t e = plan.expert[at.index];
-    if constexpr (W4) {
-      const size_t off = e * a.strideG + ((size_t)at.rows * k_tiles + step) * a.fmt.tile_bytes();
-      g.load(static_cast<const unsigned char*>(a.gate) + off, a.fmt);
-      u.load(static_cast<const unsigned char*>(a.up) + off, a.fmt);
-    } else {
-      const size_t off = e * a.strideG + (size_t)at.rows * 16 * a.ldg;
-      g.load(static_cast<const T*>(a.gate) + off, a.ldg, a.f - at.rows * 16, a.d, step, vec);
-      u.load(static_cast<const T*>(a.up) + off, a.ldg, a.f - at.rows * 16, a.d, step, vec);
+  const uint32_t tile_bytes = W4 ? a.fmt.tile_bytes() : 0;
+  // the copies run ahead of the products, through the same order
+  Unit ahead = unit;
+  int ahead_n = s0 < s1 ? begin : end, ahead_s = s0, ahead_slot = 0;
+  auto fetch = [&]() {
+    if (ahead_n < end) {
+      const size_t e = plan.expert[ahead.index];
+      const uint32_t to = ring + ahead_slot * S::kSlot;
+      if constexpr (W4) {
+        const size_t off = e * a.strideG + ((size_t)ahead.rows * steps + ahead_s) * tile_bytes;
+        const unsigned char *g = static_cast<const unsigned char*>(a.gate) + off, *u = static_cast<const unsigned char*>(a.up) + off;
+        tile_fetch(to, g);
+        tile_fetch(to + S::kHalf, u);
+        tile_fetch_scales(lane < 16 ? to : to + S::kHalf, lane < 16 ? g : u, a.fmt, lane & 15);
+      } else {
+        const size_t off = e * a.strideG + (size_t)ahead.rows * 16 * a.ldg;
+        rows16_fetch<T, 1>(to, static_cast<const T*>(a.gate) + off, a.ldg, a.f - ahead.rows * 16, a.d, ahead_s, vec);
+        rows16_fetch<T, 1>(to + S::kHalf, static_cast<const T*>(a.up) + off, a.ldg, a.f - ahead.rows * 16, a.d, ahead_s, vec);
+      }
+      if (++ahead_slot == S::kSlots) ahead_slot = 0;
+      if (++ahead_s == s1) {
+        ahead_s = s0;
+        ++ahead_n;
+        if (ahead_n < end) advance(ahead);
+      }
     }
+    copies_commit();
   };
-  // one step ahead, across units
-  Stream gate[2], up[2];
-  if (begin < end && s0 < s1) load(gate[0], up[0], unit, s0);
-  int cur = 0;
+  for (int i = 0; i + 1 < S::kSlots; ++i) fetch();
+
+  int slot = 0;
   for (int n = begin; n < end; ++n) {
-    Unit next = unit;
-    advance(next);
     const int p0 = plan.start[unit.index] + unit.group * 8, cols = min(8, plan.start[unit.index + 1] - p0);
-    const T* x = static_cast<const T*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] / a.topk) * a.d_pad + t * 8;
+    // columns past the last token repeat it; their sums are not used
+    const uint16_t* x = static_cast<const uint16_t*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] / a.topk) * a.d_pad + t * 8;
+    const float *sums0 = nullptr, *sums1 = nullptr;
+    if constexpr (W4) {
+      const int per = a.d_pad / (32 * QG);
+      sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] / a.topk) * per;
+      sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] / a.topk) * per;
+    }
     float accg[4] = {0.f, 0.f, 0.f, 0.f}, accu[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s = s0; s < s1; ++s) {
-      const bool more = s + 1 < s1;
-      auto body = [&](Stream& g0, Stream& u0, Stream& g1, Stream& u1) {
-        if (more) load(g1, u1, unit, s + 1);
-        else if (n + 1 < end) load(g1, u1, next, s0);
-        if constexpr (W4) {
-          uint4 b[1][4];
+      constexpr int kQuarters = S::kStep / 32;
+      uint4 b[kQuarters];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) b[0][q] = *reinterpret_cast<const uint4*>(x + s * 128 + q * 32);
-          g0.multiply(accg, b, a.fmt);
-          u0.multiply(accu, b, a.fmt);
-        } else {
-          uint4 b[2];
+      for (int q = 0; q < kQuarters; ++q) b[q] = *reinterpret_cast<const uint4*>(x + s * S::kStep + q * 32);
+      float2 xs[W4 ? 4 / (QG ? QG : 1) : 1];
+      if constexpr (W4) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) b[q] = *reinterpret_cast<const uint4*>(x + s * 64 + q * 32);
-          g0.multiply(accg, b);
-          u0.multiply(accu, b);
-        }
-      };
-      if (cur == 0) body(gate[0], up[0], gate[1], up[1]);
-      else body(gate[1], up[1], gate[0], up[0]);
-      cur ^= 1;
+        for (int g = 0; g < 4 / QG; ++g) xs[g] = make_float2(sums0[s * (4 / QG) + g], sums1[s * (4 / QG) + g]);
+      }
+      __syncwarp();
+      fetch();
+      copies_wait<S::kSlots - 1>();
+      const uint32_t from = ring + slot * S::kSlot;
+      if constexpr (W4) {
+        __syncwarp();
+        w4_tile_mma<T, QG>(from, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, accg);
+        w4_tile_mma<T, QG>(from + S::kHalf, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, accu);
+      } else {
+        rows16_multiply<T, 1>(from, accg, b);
+        rows16_multiply<T, 1>(from + S::kHalf, accu, b);
+      }
+      if (++slot == S::kSlots) slot = 0;
     }
     // [warp][gate, up][column][row]
     float* mine = sums + ((n & 1) * kMoeWarps + warp) * 256;
@@ -419,6 +530,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
         u += p[w * 256 + 128];
       }
       const int row = unit.rows * 16 + (i & 15), pair = plan.order[p0 + i / 16];
+      if (W4) {
+        const float2 undo = a.x_undo[pair / a.topk];
+        g *= undo.x * undo.y;
+        u *= undo.x * undo.y;
+      }
       const float h = row < a.f ? g / (1.f + expf(-g)) * u : 0.f;
       if (W4 || !std::is_same<T, __half>::value) {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.hidden) + (size_t)pair * 2 * a.f_pad + row;
@@ -434,35 +550,47 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
         if ((lane & 15) == 0) atomicMax(&a.peak[pair], top);
       }
     }
-    unit = next;
+    if (n + 1 < end) advance(unit);
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- down ----------------
-template <typename T, bool W4>
+template <int QG>
+struct MoeDownShape {
+  static constexpr int kStep = QG ? 128 : 64;
+  static constexpr uint32_t kSlot = QG ? kTileRoom : 2048;
+  static constexpr int kSlots = QG ? 6 : 4;
+};
+
+template <typename T, int QG>
 __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
+  using S = MoeDownShape<QG>;
+  constexpr bool W4 = QG > 0;
+  constexpr bool kScaled = !W4 && std::is_same<T, __half>::value;  // hidden vectors as floats, scaled here into half precision
+  extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int pairs = a.tokens * a.topk, words = MoePlan::words(a.experts, pairs);
-  MoePlan plan(reinterpret_cast<int*>(smem), a.experts, pairs);
-  float* sums = reinterpret_cast<float*>(smem + ((size_t)words * 4 + 15) / 16 * 16);  // [warp][token][row]
+  const uint32_t ring = smem_u32(smem) + warp * S::kSlots * S::kSlot;
+  float* sums = reinterpret_cast<float*>(smem + kMoeWarps * S::kSlots * S::kSlot);  // [warp][token][row]
+  int* at_plan = reinterpret_cast<int*>(sums + kMoeWarps * a.tokens * 16);
+  MoePlan plan(at_plan, a.experts, pairs);
   griddep_launch_dependents();
   griddep_wait();
-  for (int i = threadIdx.x; i < words; i += kMoeThreads) reinterpret_cast<int*>(smem)[i] = a.plan[i];
+  for (int i = threadIdx.x; i < words; i += kMoeThreads) at_plan[i] = a.plan[i];
+  for (int i = threadIdx.x; i < kMoeWarps * a.tokens * 16; i += kMoeThreads) sums[i] = 0.f;
   __syncthreads();
   const int active = *plan.active;
 
-  using U = typename std::conditional<W4, __nv_bfloat16, T>::type;  // type of the products
-  using Stream = typename std::conditional<W4, Rows4<T, U>, Rows16<T>>::type;
-  constexpr int kStep = Stream::kStep;
-  constexpr bool kScaled = !W4 && std::is_same<T, __half>::value;  // hidden vectors as floats, scaled here into half precision
-  const int steps = (a.f + kStep - 1) / kStep, k_tiles = (a.f + 127) / 128;
+  const int steps = (a.f + S::kStep - 1) / S::kStep;
   int total = 0;
   for (int i = 0; i < active; ++i) total += (plan.start[i + 1] - plan.start[i] + 7) / 8;
   const long long all = (long long)total * steps;
+  const int row_blocks = (a.d + 15) / 16;
   const long long w0 = all * warp / kMoeWarps, w1 = all * (warp + 1) / kMoeWarps;
   const bool vec = !W4 && a.ldd % 8 == 0 && a.strideD % 8 == 0 && a.f % 8 == 0 &&
                    (reinterpret_cast<uintptr_t>(a.down) & 15u) == 0;
+  const uint32_t tile_bytes = W4 ? a.fmt.tile_bytes() : 0;
   struct Place {
     int index, group, groups, step;
   };
@@ -486,75 +614,94 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs 
     p.group = 0;
     if (++p.index < active) p.groups = (plan.start[p.index + 1] - plan.start[p.index] + 7) / 8;
   };
-  auto load = [&](Stream& s, int rows, const Place& p) {
-    const size_t e = plan.expert[p.index];
-    if constexpr (W4)
-      s.load(static_cast<const unsigned char*>(a.down) + e * a.strideD + ((size_t)rows * k_tiles + p.step) * a.fmt.tile_bytes(),
-             a.fmt);
-    else
-      s.load(static_cast<const T*>(a.down) + e * a.strideD + (size_t)rows * 16 * a.ldd, a.ldd, a.d - rows * 16, a.f, p.step, vec);
+  // the copies run ahead of the products, through the same order, on into the next row block
+  Place ahead = first;
+  int ahead_rows = w0 < w1 ? blockIdx.x : row_blocks, ahead_slot = 0;
+  long long ahead_n = w0;
+  auto fetch = [&]() {
+    if (ahead_rows < row_blocks) {
+      const size_t e = plan.expert[ahead.index];
+      const uint32_t to = ring + ahead_slot * S::kSlot;
+      if constexpr (W4) {
+        const unsigned char* w = static_cast<const unsigned char*>(a.down) + e * a.strideD +
+                                 ((size_t)ahead_rows * steps + ahead.step) * tile_bytes;
+        tile_fetch(to, w);
+        tile_fetch_scales(to, w, a.fmt, lane);
+      } else {
+        rows16_fetch<T, 2>(to, static_cast<const T*>(a.down) + e * a.strideD + (size_t)ahead_rows * 16 * a.ldd, a.ldd,
+                           a.d - ahead_rows * 16, a.f, ahead.step, vec);
+      }
+      if (++ahead_slot == S::kSlots) ahead_slot = 0;
+      if (++ahead_n == w1) {
+        ahead_n = w0;
+        ahead = first;
+        ahead_rows += gridDim.x;
+      } else {
+        advance(ahead);
+      }
+    }
+    copies_commit();
   };
+  for (int i = 0; i + 1 < S::kSlots; ++i) fetch();
 
-  const int row_blocks = (a.d + 15) / 16;
+  int slot = 0;
   for (int rows = blockIdx.x; rows < row_blocks; rows += gridDim.x) {
-    for (int i = threadIdx.x; i < kMoeWarps * a.tokens * 16; i += kMoeThreads) sums[i] = 0.f;
-    __syncthreads();
     Place place = first;
-    Stream w[2];
-    if (w0 < w1) load(w[0], rows, place);
-    int cur = 0;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (long long n = w0; n < w1; ++n) {
-      Place next = place;
-      advance(next);
       const int p0 = plan.start[place.index] + place.group * 8, cols = min(8, plan.start[place.index + 1] - p0);
       const int pair = plan.order[p0 + min(r, cols - 1)];
-      auto body = [&](Stream& now, Stream& then) {
-        if (n + 1 < w1) load(then, rows, next);
-        if constexpr (W4) {
-          const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(a.hidden) + (size_t)pair * 2 * a.f_pad + place.step * 128 + t * 8;
-          uint4 b[2][4];
+      // the hidden vectors: a value and its remainder, or floats (twice as wide)
+      constexpr int kQuarters = S::kStep / 32;
+      uint4 h[2][kQuarters];
+      float up = 1.f;
+      if constexpr (kScaled) {
+        const float* from = static_cast<const float*>(a.hidden) + (size_t)pair * a.f_pad + place.step * S::kStep + t * 8;
+        up = moe_scale(a.peak[pair]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+        for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) b[i][q] = *reinterpret_cast<const uint4*>(h + (size_t)i * a.f_pad + q * 32);
-          now.multiply(acc, b, a.fmt);
-        } else if constexpr (!kScaled) {
-          const T* h = static_cast<const T*>(a.hidden) + (size_t)pair * 2 * a.f_pad + place.step * 64 + t * 8;
+          for (int i = 0; i < 2; ++i) h[i][q] = *reinterpret_cast<const uint4*>(from + q * 32 + i * 4);
+      } else {
+        const __nv_bfloat16* from =
+            static_cast<const __nv_bfloat16*>(a.hidden) + (size_t)pair * 2 * a.f_pad + place.step * S::kStep + t * 8;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint4 b[2];
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) b[q] = *reinterpret_cast<const uint4*>(h + (size_t)i * a.f_pad + q * 32);
-            now.multiply(acc, b);
-          }
-        } else {
-          const float* h = static_cast<const float*>(a.hidden) + (size_t)pair * a.f_pad + place.step * 64 + t * 8;
-          const float up = moe_scale(a.peak[pair]);
-          uint4 hi[2], lo[2];
+          for (int q = 0; q < kQuarters; ++q) h[i][q] = *reinterpret_cast<const uint4*>(from + (size_t)i * a.f_pad + q * 32);
+      }
+      __syncwarp();
+      fetch();
+      copies_wait<S::kSlots - 1>();
+      if (W4) __syncwarp();
+      const uint32_t from = ring + slot * S::kSlot;
+      if (++slot == S::kSlots) slot = 0;
+      if constexpr (W4) {
+        tile_multiply_bf16<T, QG>(from, h, a.fmt.zeros, acc);
+      } else {
+        if constexpr (kScaled) {  // floats into half precision and its remainder
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const float4 u = *reinterpret_cast<const float4*>(h + q * 32), v = *reinterpret_cast<const float4*>(h + q * 32 + 4);
-            const float e[8] = {u.x * up, u.y * up, u.z * up, u.w * up, v.x * up, v.y * up, v.z * up, v.w * up};
-            uint32_t* ph = &hi[q].x;
-            uint32_t* pl = &lo[q].x;
+          for (int q = 0; q < kQuarters; ++q) {
+            const uint32_t raw[8] = {h[0][q].x, h[0][q].y, h[0][q].z, h[0][q].w, h[1][q].x, h[1][q].y, h[1][q].z, h[1][q].w};
+            uint32_t hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const __half2 c = __floats2half2_rn(e[2 * i], e[2 * i + 1]);
+              const float e0 = __uint_as_float(raw[2 * i]) * up, e1 = __uint_as_float(raw[2 * i + 1]) * up;
+              const __half2 c = __floats2half2_rn(e0, e1);
               const float2 back = __half22float2(c);
-              const __half2 d = __floats2half2_rn(e[2 * i] - back.x, e[2 * i + 1] - back.y);
-              ph[i] = *reinterpret_cast<const uint32_t*>(&c);
-              pl[i] = *reinterpret_cast<const uint32_t*>(&d);
+              const __half2 d = __floats2half2_rn(e0 - back.x, e1 - back.y);
+              hi[i] = *reinterpret_cast<const uint32_t*>(&c);
+              lo[i] = *reinterpret_cast<const uint32_t*>(&d);
             }
+            h[0][q] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            h[1][q] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
-          now.multiply(acc, hi);
-          now.multiply(acc, lo);
         }
-      };
-      if (cur == 0) body(w[0], w[1]);
-      else body(w[1], w[0]);
-      cur ^= 1;
-      if (next.step == 0 || n + 1 == w1) {  // the expert's tokens are finished (as far as this warp goes)
+        rows16_multiply<T, 2>(from, acc, h[0]);
+        rows16_multiply<T, 2>(from, acc, h[1]);
+      }
+      advance(place);
+      if (place.step == 0 || n + 1 == w1) {  // the expert's tokens are finished (as far as this warp goes)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int col = t * 2 + (i & 1);
@@ -568,13 +715,16 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs 
         }
         __syncwarp();
       }
-      place = next;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.tokens * 16; i += kMoeThreads) {
       float v = 0.f;
 #pragma unroll
-      for (int w2 = 0; w2 < kMoeWarps; ++w2) v += sums[w2 * a.tokens * 16 + i];
+      for (int w = 0; w < kMoeWarps; ++w) {
+        float* p = sums + w * a.tokens * 16 + i;
+        v += *p;
+        *p = 0.f;
+      }
       const int row = rows * 16 + (i & 15);
       if (row < a.d) {
         T* y = static_cast<T*>(a.Y) + (size_t)(i / 16) * a.ldy + row;
@@ -583,6 +733,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs 
     }
     __syncthreads();
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 }  // namespace mmbo

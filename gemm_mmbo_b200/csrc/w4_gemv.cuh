@@ -79,17 +79,17 @@ struct W4Tile {
   static constexpr int kBytes = kZeros + (ZEROS ? kGroups * kW4Rows : 0);
 };
 
-// acc += the products of a tile with 128 rows of 8 staged columns: x is this lane's place in them, `xsum` its place in
-// their group sums (shared memory addresses).  Sums are in units of 2^20.
+// acc += the products of a tile with 128 rows of 8 columns: b(q) is this lane's 16 bytes of quarter q of its column, xs(g)
+// the sums of group g of the columns 2 t and 2 t + 1.  Sums are in units of 2^20.
 //
 // A code is used as the bits of a half-precision number: q in the lowest four bits is the subnormal q 2^-24, q in the
 // next four is q 2^-20, both exact, so a word becomes four operand registers with a shift and four masks.  The two kinds
 // have a sum each, and the zero point comes off once a group:  sum (q - z) x = sum q x - z sum x.  (Forming the sums of
 // x with the same instruction and a matrix of ones made the tensor pipe the bound: 16 instructions a tile, 32 cycles;
 // subtracting the zero point from each code costs as much again as unpacking it.)
-template <typename T, int QG, bool ZEROS>
-__device__ __forceinline__ void w4_tile_mma(uint32_t tile, uint32_t x, uint32_t xsum, float (&acc)[4]) {
-  using L = W4Tile<QG, ZEROS>;
+template <typename T, int QG, typename Columns, typename Sums>
+__device__ __forceinline__ void w4_tile_mma(uint32_t tile, Columns column, Sums sums, bool zeros, float (&acc)[4]) {
+  using L = W4Tile<QG, true>;  // (where there are zero points does not depend on whether there are)
   const int lane = threadIdx.x & 31, r = lane >> 2;
   const uint32_t codes = tile + w4_piece(r, lane & 3);
   const uint4 c0 = lds128(codes), c1 = lds128(codes + 512);  // rows r and r + 8
@@ -101,7 +101,7 @@ __device__ __forceinline__ void w4_tile_mma(uint32_t tile, uint32_t x, uint32_t 
     for (int qq = 0; qq < QG; ++qq) {
       const int q = g * QG + qq;
       const uint32_t v0 = w0[q] >> 8, v1 = w1[q] >> 8;
-      const uint4 b = lds128(x + q * 64);
+      const uint4 b = column(q);
       if (qq == 0) {
         mma_f16_from_zero(low, w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
         mma_f16_from_zero(high, w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
@@ -112,12 +112,12 @@ __device__ __forceinline__ void w4_tile_mma(uint32_t tile, uint32_t x, uint32_t 
     }
     const float2 s = widen2<T>(lds32(tile + L::kScales + g * 32 + r * 4));
     float z0 = 8.f, z1 = 8.f;
-    if (ZEROS) {
+    if (zeros) {
       const uint32_t z = lds16(tile + L::kZeros + g * 16 + r * 2);
       z0 = (float)(z & 15u);
       z1 = (float)((z >> 8) & 15u);
     }
-    const float2 xs = lds_f2(xsum + g * 32);
+    const float2 xs = sums(g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float dot = fmaf(16.f, low[i], high[i]);
@@ -443,7 +443,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
           uint32_t xsum = xsum_lane + (tile - chunk0) * (G * 32);
 #pragma unroll 2
           for (int i = 0; i < cnt; ++i) {
-            w4_tile_mma<T, QG, ZEROS>(at, x, xsum, acc);
+            w4_tile_mma<T, QG>(at, [&](int q) { return lds128(x + q * 64); }, [&](int g) { return lds_f2(xsum + g * 32); },
+                               ZEROS, acc);
             at += TILE;
             x += 256;
             xsum += G * 32;

@@ -106,6 +106,13 @@ def test_every_token_at_one_expert_and_none_at_others(cuda, mm):
     Layer(mm, "bf16", 33, 160, 96, 64, 2, renorm=True, x=x, group=32, zeros=True).check()
 
 
+@pytest.mark.parametrize("group", [0, 128])
+def test_the_largest_selections(cuda, mm, group):
+    """As many experts and choices as a call may have, with more tokens than one pass takes."""
+    Layer(mm, "bf16", 20, 64, 16, 1024, 32, renorm=True, group=group).check()
+    Layer(mm, "f16", 130, 32, 24, 9, 7, group=group).check()
+
+
 def test_equal_scores_go_to_the_lowest_index(cuda, mm):
     for experts, topk in ((8, 3), (70, 32), (256, 9)):
         layer = Layer(mm, "f16", 4, 64, 32, experts, topk)
