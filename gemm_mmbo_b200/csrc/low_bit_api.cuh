@@ -253,7 +253,7 @@ static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* pa
 
 // Workspace of the expert layer, for one pass.
 struct MoeWorkspace {
-  size_t scores, x, x_sums, x_undo, hidden, peak, plan, total;
+  size_t scores, x, x_sums, x_undo, hidden, plan, total;
 };
 static MoeWorkspace moe_workspace(size_t tokens, size_t d, size_t f, size_t experts, size_t topk) {
   if (tokens > (size_t)moe_pass_tokens((int)topk)) tokens = moe_pass_tokens((int)topk);
@@ -264,8 +264,7 @@ static MoeWorkspace moe_workspace(size_t tokens, size_t d, size_t f, size_t expe
   w.x_sums = w.x + align_up(tokens * align_up(d, 128) * 2, 256);
   w.x_undo = w.x_sums + align_up(tokens * (align_up(d, 128) / 32) * 4, 256);
   w.hidden = w.x_undo + align_up(tokens * 8, 256);
-  w.peak = w.hidden + align_up(pairs * align_up(f, 128) * 4, 256);
-  w.plan = w.peak + align_up(pairs * 4, 256);
+  w.plan = w.hidden + align_up(pairs * align_up(f, 128) * 4, 256);
   w.total = w.plan + align_up((size_t)MoePlan::words((int)experts, (int)pairs) * 4, 256);
   return w;
 }
@@ -496,11 +495,9 @@ int mmbo_moe(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_
     a.x_sums = reinterpret_cast<float*>(base + ws.x_sums);
     a.x_undo = reinterpret_cast<float2*>(base + ws.x_undo);
     a.hidden = base + ws.hidden;
-    a.peak = reinterpret_cast<uint32_t*>(base + ws.peak);
     a.plan = reinterpret_cast<int*>(base + ws.plan);
     a.d_pad = (int)align_up(d, 128);
     a.f_pad = (int)align_up(f, 128);
-    a.hidden_f32 = group == 0 && dtype == MMBO_DTYPE_F16;
     rc = dtype == MMBO_DTYPE_F16 ? run_moe<__half>(a, st) : run_moe<__nv_bfloat16>(a, st);
     if (rc) return rc;
   }

@@ -45,11 +45,9 @@ struct MoeArgs {
   void* x;          // tokens x d_pad: the activations, zero behind d (4-bit experts: in half precision, scaled)
   float* x_sums;    // 4-bit experts: tokens x (d_pad / group) sums of these, in units of 2^20
   float2* x_undo;   // 4-bit experts: two factors a token that undo its scale and the unit of 2^20
-  void* hidden;     // pairs x f_pad: floats, or bfloat16 twice (the value and what its rounding left)
-  uint32_t* peak;   // pairs: bits of the largest hidden magnitude
+  void* hidden;     // pairs x 2 x f_pad, zero behind f: hidden vectors as a 16-bit value and what its rounding left, see MoeHidden
   int* plan;        // what `up` found out for `down`, see MoePlan
   int d_pad, f_pad; // multiples of 128
-  int hidden_f32;
 };
 
 // The selection, sorted by expert: `order` holds the pairs (token * topk + slot) of expert 0's tokens, then expert 1's ..;
@@ -92,12 +90,9 @@ __global__ void __launch_bounds__(256) moe_scores_kernel(const MoeArgs a) {
   const int t = blockIdx.y, lane = threadIdx.x & 31;
   const T* x = static_cast<const T*>(a.X) + (size_t)t * a.ldx;
   if (blockIdx.x == gridDim.x - 1) {  // the last block of a token prepares the workspace instead
-    for (int s = threadIdx.x; s < a.topk; s += 256) a.peak[t * a.topk + s] = 0;
-    // hidden vectors behind f: floats, or two rows of bfloat16 (zero bytes either way)
     uint16_t* h = static_cast<uint16_t*>(a.hidden) + (size_t)t * a.topk * a.f_pad * 2;
-    const int per = a.hidden_f32 ? 1 : 2, width = a.hidden_f32 ? 2 : 1, pad = (a.f_pad - a.f) * width;
-    for (int i = threadIdx.x; i < a.topk * per * pad; i += 256)
-      h[(size_t)(i / pad) * a.f_pad * width + a.f * width + i % pad] = 0;
+    const int pad = a.f_pad - a.f;
+    for (int i = threadIdx.x; i < a.topk * 2 * pad; i += 256) h[(size_t)(i / pad) * a.f_pad + a.f + i % pad] = 0;
     if (!a.fmt.group) {
       T* copy = static_cast<T*>(a.x) + (size_t)t * a.d_pad;
       for (int j = threadIdx.x * 8; j < a.d_pad; j += 256 * 8) *reinterpret_cast<uint4*>(copy + j) = load8(x, a.d, j);
@@ -255,24 +250,41 @@ __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// Sixteen rows of 16-bit weights, 32 C columns: piece (h, u) of a lane, columns 32 u + 8 t .. + 7 of row r + 8 h, lies at
-// (h C + u) * 512 + lane * 16.  `rows` exist; the others, and columns behind k, are zero.
+// Feeds a ring with sixteen rows of 16-bit weights, 32 C columns at a time: piece (h, u) of a lane, columns 32 u + 8 t ..
+// + 7 of row r + 8 h, goes to (h C + u) * 512 + lane * 16.  Rows that do not exist and columns behind k come as zeros.
 template <typename T, int C>
-__device__ __forceinline__ void rows16_fetch(uint32_t to, const T* base, size_t ld, int rows, int k, int step, bool vec) {
-  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const bool have = r + 8 * h < rows;
-    const T* row = base + (size_t)(have ? r + 8 * h : 0) * ld;
+struct RowsFeed {
+  const T *lo, *hi;  // this lane's place in rows r and r + 8
+  int j, k;          // its column; a row's length
+  bool have_lo, have_hi, vec;
+  __device__ __forceinline__ void start(const T* base, size_t ld, int rows, int k_, int step, bool vec_) {
+    const int lane = threadIdx.x & 31, r = lane >> 2;
+    have_lo = r < rows;
+    have_hi = r + 8 < rows;
+    j = step * 32 * C + (lane & 3) * 8;
+    k = k_;
+    vec = vec_;
+    lo = base + (have_lo ? r * ld : 0) + j;
+    hi = base + (have_hi ? (r + 8) * ld : 0) + j;
+  }
+  __device__ __forceinline__ void fetch(uint32_t to) {
+    to += (threadIdx.x & 31) * 16;
 #pragma unroll
     for (int u = 0; u < C; ++u) {
-      const int j = (step * C + u) * 32 + t * 8;
-      const uint32_t dst = to + (h * C + u) * 512 + lane * 16;
-      if (vec) copy16(dst, row + (j < k ? j : 0), have && j < k);
-      else sts128(dst, load8(row, have ? k : 0, j));
+      const bool in = j + 32 * u < k;
+      if (vec) {
+        copy16(to + u * 512, in ? lo + 32 * u : lo - j, in && have_lo);
+        copy16(to + (C + u) * 512, in ? hi + 32 * u : hi - j, in && have_hi);
+      } else {
+        sts128(to + u * 512, load8(lo - j, have_lo ? k : 0, j + 32 * u));
+        sts128(to + (C + u) * 512, load8(hi - j, have_hi ? k : 0, j + 32 * u));
+      }
     }
+    lo += 32 * C;
+    hi += 32 * C;
+    j += 32 * C;
   }
-}
+};
 // acc += those weights * columns; b: this lane's 16 bytes of each 32 columns
 template <typename T, int C>
 __device__ __forceinline__ void rows16_multiply(uint32_t from, float (&acc)[4], const uint4 (&b)[C]) {
@@ -285,16 +297,29 @@ __device__ __forceinline__ void rows16_multiply(uint32_t from, float (&acc)[4], 
   }
 }
 
-// A packed tile in its own layout: two pieces of codes a lane, scales and zero points by the first lanes from `lane0` on.
-// (Others read what a lane copied: __syncwarp() behind the wait.)
-__device__ __forceinline__ void tile_fetch(uint32_t to, const unsigned char* tile) {
-  const int lane = threadIdx.x & 31, at = w4_piece(lane >> 2, lane & 3);
-  copy16(to + at, tile + at, true);
-  copy16(to + at + 512, tile + at + 512, true);
-}
-__device__ __forceinline__ void tile_fetch_scales(uint32_t to, const unsigned char* tile, const W4Format& f, int i) {
-  if (i >= 0 && i * 16 < (int)f.tile_bytes() - kW4Codes) copy16(to + kW4Codes + i * 16, tile + kW4Codes + i * 16, true);
-}
+// The same with packed tiles, in their own layout: two pieces of codes a lane, scales and zero points by the lanes from
+// `first` on.  (Others read what a lane copied: __syncwarp() behind the wait.)
+struct TileFeed {
+  const unsigned char *codes, *scales;
+  uint32_t piece, scale_piece, bytes;
+  bool has_scale;
+  __device__ __forceinline__ void start(const unsigned char* tile, uint32_t tile_bytes, int first) {
+    const int lane = threadIdx.x & 31, i = lane - first;
+    bytes = tile_bytes;
+    piece = w4_piece(lane >> 2, lane & 3);
+    has_scale = i >= 0 && i * 16 < (int)tile_bytes - kW4Codes;
+    scale_piece = kW4Codes + (has_scale ? i * 16 : 0);
+    codes = tile + piece;
+    scales = tile + scale_piece;
+  }
+  __device__ __forceinline__ void fetch(uint32_t to) {
+    copy16(to + piece, codes, true);
+    copy16(to + piece + 512, codes + 512, true);
+    if (has_scale) copy16(to + scale_piece, scales, true);
+    codes += bytes;
+    scales += bytes;
+  }
+};
 // acc += a packed tile * two bfloat16 columns' worth (a value and its remainder, by quarters).  Codes become exact integers:
 // for w4_tile_mma a hidden vector would first have to be brought to half precision.
 template <typename T, int QG>
@@ -330,11 +355,19 @@ __device__ __forceinline__ void tile_multiply_bf16(uint32_t tile, const uint4 (&
 }
 constexpr uint32_t kTileRoom = kW4Codes + 4 * 48;  // of a tile in a ring, whatever its groups
 
-// The power of two that brings a vector whose largest magnitude has these bits below 2^15.
-__device__ __forceinline__ float moe_scale(uint32_t peak) {
-  const int up = 14 - ((int)max(peak >> 23, 1u) - 127);
-  return __uint_as_float((uint32_t)(min(max(up, -100), 100) + 127) << 23);
-}
+// Hidden vectors as products take them: a 16-bit value and what its rounding left, so that 16 bits and more survive.
+// bfloat16 has the range of a float.  Half precision holds h / 64 and 2^11 times the remainder: magnitudes up to 4.19e6,
+// steps of 2^-30 near zero (results in half precision have steps of 2^-24).
+template <typename U>
+struct MoeHidden;
+template <>
+struct MoeHidden<__nv_bfloat16> {
+  static constexpr float kScale = 1.f, kRest = 1.f;
+};
+template <>
+struct MoeHidden<__half> {
+  static constexpr float kScale = 0x1p-6f, kRest = 0x1p11f;
+};
 
 // ---------------------------------------------------------------- up ------------------
 // QG: quarters of a group of packed weights, 0: 16-bit weights.
@@ -446,60 +479,68 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
                    ((reinterpret_cast<uintptr_t>(a.gate) | reinterpret_cast<uintptr_t>(a.up)) & 15u) == 0;
   const uint32_t tile_bytes = W4 ? a.fmt.tile_bytes() : 0;
   // the copies run ahead of the products, through the same order
+  using Feed = typename std::conditional<W4, TileFeed, RowsFeed<T, 1>>::type;
+  Feed gate, up;
   Unit ahead = unit;
-  int ahead_n = s0 < s1 ? begin : end, ahead_s = s0, ahead_slot = 0;
+  int ahead_n = s0 < s1 ? begin : end, ahead_left = s1 - s0;
+  uint32_t ahead_at = ring;
+  auto start = [&]() {
+    if (ahead_n >= end) return;
+    const size_t e = plan.expert[ahead.index];
+    if constexpr (W4) {
+      const size_t off = e * a.strideG + ((size_t)ahead.rows * steps + s0) * tile_bytes;
+      gate.start(static_cast<const unsigned char*>(a.gate) + off, tile_bytes, 0);
+      up.start(static_cast<const unsigned char*>(a.up) + off, tile_bytes, 16);
+    } else {
+      const size_t off = e * a.strideG + (size_t)ahead.rows * 16 * a.ldg;
+      gate.start(static_cast<const T*>(a.gate) + off, a.ldg, a.f - ahead.rows * 16, a.d, s0, vec);
+      up.start(static_cast<const T*>(a.up) + off, a.ldg, a.f - ahead.rows * 16, a.d, s0, vec);
+    }
+  };
   auto fetch = [&]() {
     if (ahead_n < end) {
-      const size_t e = plan.expert[ahead.index];
-      const uint32_t to = ring + ahead_slot * S::kSlot;
-      if constexpr (W4) {
-        const size_t off = e * a.strideG + ((size_t)ahead.rows * steps + ahead_s) * tile_bytes;
-        const unsigned char *g = static_cast<const unsigned char*>(a.gate) + off, *u = static_cast<const unsigned char*>(a.up) + off;
-        tile_fetch(to, g);
-        tile_fetch(to + S::kHalf, u);
-        tile_fetch_scales(lane < 16 ? to : to + S::kHalf, lane < 16 ? g : u, a.fmt, lane & 15);
-      } else {
-        const size_t off = e * a.strideG + (size_t)ahead.rows * 16 * a.ldg;
-        rows16_fetch<T, 1>(to, static_cast<const T*>(a.gate) + off, a.ldg, a.f - ahead.rows * 16, a.d, ahead_s, vec);
-        rows16_fetch<T, 1>(to + S::kHalf, static_cast<const T*>(a.up) + off, a.ldg, a.f - ahead.rows * 16, a.d, ahead_s, vec);
-      }
-      if (++ahead_slot == S::kSlots) ahead_slot = 0;
-      if (++ahead_s == s1) {
-        ahead_s = s0;
-        ++ahead_n;
-        if (ahead_n < end) advance(ahead);
+      gate.fetch(ahead_at);
+      up.fetch(ahead_at + S::kHalf);
+      ahead_at += S::kSlot;
+      if (ahead_at == ring + S::kSlots * S::kSlot) ahead_at = ring;
+      if (--ahead_left == 0) {
+        ahead_left = s1 - s0;
+        if (++ahead_n < end) advance(ahead);
+        start();
       }
     }
     copies_commit();
   };
+  start();
   for (int i = 0; i + 1 < S::kSlots; ++i) fetch();
 
-  int slot = 0;
+  uint32_t from = ring;
   for (int n = begin; n < end; ++n) {
     const int p0 = plan.start[unit.index] + unit.group * 8, cols = min(8, plan.start[unit.index + 1] - p0);
     // columns past the last token repeat it; their sums are not used
-    const uint16_t* x = static_cast<const uint16_t*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] / a.topk) * a.d_pad + t * 8;
+    const uint16_t* x = static_cast<const uint16_t*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] / a.topk) * a.d_pad +
+                        s0 * S::kStep + t * 8;
     const float *sums0 = nullptr, *sums1 = nullptr;
     if constexpr (W4) {
-      const int per = a.d_pad / (32 * QG);
-      sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] / a.topk) * per;
-      sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] / a.topk) * per;
+      const int per = a.d_pad / (32 * QG), at = s0 * (4 / QG);
+      sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] / a.topk) * per + at;
+      sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] / a.topk) * per + at;
     }
     float accg[4] = {0.f, 0.f, 0.f, 0.f}, accu[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s = s0; s < s1; ++s) {
       constexpr int kQuarters = S::kStep / 32;
       uint4 b[kQuarters];
 #pragma unroll
-      for (int q = 0; q < kQuarters; ++q) b[q] = *reinterpret_cast<const uint4*>(x + s * S::kStep + q * 32);
+      for (int q = 0; q < kQuarters; ++q) b[q] = *reinterpret_cast<const uint4*>(x + q * 32);
+      x += S::kStep;
       float2 xs[W4 ? 4 / (QG ? QG : 1) : 1];
       if constexpr (W4) {
 #pragma unroll
-        for (int g = 0; g < 4 / QG; ++g) xs[g] = make_float2(sums0[s * (4 / QG) + g], sums1[s * (4 / QG) + g]);
+        for (int g = 0; g < 4 / QG; ++g) xs[g] = make_float2(*sums0++, *sums1++);
       }
       __syncwarp();
       fetch();
       copies_wait<S::kSlots - 1>();
-      const uint32_t from = ring + slot * S::kSlot;
       if constexpr (W4) {
         __syncwarp();
         w4_tile_mma<T, QG>(from, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, accg);
@@ -508,7 +549,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
         rows16_multiply<T, 1>(from, accg, b);
         rows16_multiply<T, 1>(from + S::kHalf, accu, b);
       }
-      if (++slot == S::kSlots) slot = 0;
+      from += S::kSlot;
+      if (from == ring + S::kSlots * S::kSlot) from = ring;
     }
     // [warp][gate, up][column][row]
     float* mine = sums + ((n & 1) * kMoeWarps + warp) * 256;
@@ -536,19 +578,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
         u *= undo.x * undo.y;
       }
       const float h = row < a.f ? g / (1.f + expf(-g)) * u : 0.f;
-      if (W4 || !std::is_same<T, __half>::value) {
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.hidden) + (size_t)pair * 2 * a.f_pad + row;
-        const __nv_bfloat16 v = __float2bfloat16_rn(h);
-        out[0] = v;
-        out[a.f_pad] = __float2bfloat16_rn(isfinite(h) ? h - __bfloat162float(v) : 0.f);
-      } else {
-        static_cast<float*>(a.hidden)[(size_t)pair * a.f_pad + row] = h;
-        uint32_t top = __float_as_uint(fabsf(h));  // sixteen lanes hold the rows of a pair
-        const unsigned lanes = 0xffffu << (lane & 16);
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(lanes, top, o));
-        if ((lane & 15) == 0) atomicMax(&a.peak[pair], top);
-      }
+      using U = typename std::conditional<W4, __nv_bfloat16, T>::type;  // type of the products with down
+      U* out = static_cast<U*>(a.hidden) + (size_t)pair * 2 * a.f_pad + row;
+      const float scaled = h * MoeHidden<U>::kScale;
+      const U v = from_f32<U>(scaled);
+      const float rest = (scaled - to_f32(v)) * MoeHidden<U>::kRest;
+      out[0] = v;
+      out[a.f_pad] = from_f32<U>(isfinite(rest) ? rest : 0.f);
     }
     if (n + 1 < end) advance(unit);
   }
@@ -567,7 +603,7 @@ template <typename T, int QG>
 __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs a) {
   using S = MoeDownShape<QG>;
   constexpr bool W4 = QG > 0;
-  constexpr bool kScaled = !W4 && std::is_same<T, __half>::value;  // hidden vectors as floats, scaled here into half precision
+  using U = typename std::conditional<W4, __nv_bfloat16, T>::type;  // type of the products
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int pairs = a.tokens * a.topk, words = MoePlan::words(a.experts, pairs);
@@ -591,10 +627,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs 
   const bool vec = !W4 && a.ldd % 8 == 0 && a.strideD % 8 == 0 && a.f % 8 == 0 &&
                    (reinterpret_cast<uintptr_t>(a.down) & 15u) == 0;
   const uint32_t tile_bytes = W4 ? a.fmt.tile_bytes() : 0;
-  struct Place {
+  // a run: what of this warp's part belongs to one expert and group of tokens
+  struct Run {
     int index, group, groups, step;
   };
-  Place first{0, 0, 0, 0};
+  Run first{0, 0, 0, 0};
   {
     long long at = 0;
     for (; first.index < active; ++first.index) {
@@ -607,114 +644,94 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs 
       at += (long long)first.groups * steps;
     }
   }
-  auto advance = [&](Place& p) {
-    if (++p.step < steps) return;
+  auto advance = [&](Run& p) {
     p.step = 0;
     if (++p.group < p.groups) return;
     p.group = 0;
     if (++p.index < active) p.groups = (plan.start[p.index + 1] - plan.start[p.index] + 7) / 8;
   };
   // the copies run ahead of the products, through the same order, on into the next row block
-  Place ahead = first;
-  int ahead_rows = w0 < w1 ? blockIdx.x : row_blocks, ahead_slot = 0;
+  using Feed = typename std::conditional<W4, TileFeed, RowsFeed<T, 2>>::type;
+  Feed feed;
+  Run ahead = first;
+  int ahead_rows = w0 < w1 ? blockIdx.x : row_blocks, ahead_left = 0;
   long long ahead_n = w0;
+  uint32_t ahead_at = ring;
+  auto start = [&]() {
+    if (ahead_rows >= row_blocks) return;
+    const size_t e = plan.expert[ahead.index];
+    ahead_left = (int)min((long long)(steps - ahead.step), w1 - ahead_n);
+    if constexpr (W4)
+      feed.start(static_cast<const unsigned char*>(a.down) + e * a.strideD + ((size_t)ahead_rows * steps + ahead.step) * tile_bytes,
+                 tile_bytes, 0);
+    else
+      feed.start(static_cast<const T*>(a.down) + e * a.strideD + (size_t)ahead_rows * 16 * a.ldd, a.ldd, a.d - ahead_rows * 16,
+                 a.f, ahead.step, vec);
+    ahead_n += ahead_left;
+  };
   auto fetch = [&]() {
     if (ahead_rows < row_blocks) {
-      const size_t e = plan.expert[ahead.index];
-      const uint32_t to = ring + ahead_slot * S::kSlot;
-      if constexpr (W4) {
-        const unsigned char* w = static_cast<const unsigned char*>(a.down) + e * a.strideD +
-                                 ((size_t)ahead_rows * steps + ahead.step) * tile_bytes;
-        tile_fetch(to, w);
-        tile_fetch_scales(to, w, a.fmt, lane);
-      } else {
-        rows16_fetch<T, 2>(to, static_cast<const T*>(a.down) + e * a.strideD + (size_t)ahead_rows * 16 * a.ldd, a.ldd,
-                           a.d - ahead_rows * 16, a.f, ahead.step, vec);
-      }
-      if (++ahead_slot == S::kSlots) ahead_slot = 0;
-      if (++ahead_n == w1) {
-        ahead_n = w0;
-        ahead = first;
-        ahead_rows += gridDim.x;
-      } else {
-        advance(ahead);
+      feed.fetch(ahead_at);
+      ahead_at += S::kSlot;
+      if (ahead_at == ring + S::kSlots * S::kSlot) ahead_at = ring;
+      if (--ahead_left == 0) {
+        if (ahead_n == w1) {
+          ahead_n = w0;
+          ahead = first;
+          ahead_rows += gridDim.x;
+        } else {
+          advance(ahead);
+        }
+        start();
       }
     }
     copies_commit();
   };
+  start();
   for (int i = 0; i + 1 < S::kSlots; ++i) fetch();
 
-  int slot = 0;
+  uint32_t from = ring;
   for (int rows = blockIdx.x; rows < row_blocks; rows += gridDim.x) {
-    Place place = first;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (long long n = w0; n < w1; ++n) {
-      const int p0 = plan.start[place.index] + place.group * 8, cols = min(8, plan.start[place.index + 1] - p0);
-      const int pair = plan.order[p0 + min(r, cols - 1)];
-      // the hidden vectors: a value and its remainder, or floats (twice as wide)
-      constexpr int kQuarters = S::kStep / 32;
-      uint4 h[2][kQuarters];
-      float up = 1.f;
-      if constexpr (kScaled) {
-        const float* from = static_cast<const float*>(a.hidden) + (size_t)pair * a.f_pad + place.step * S::kStep + t * 8;
-        up = moe_scale(a.peak[pair]);
+    Run run = first;
+    for (long long n = w0; n < w1; advance(run)) {
+      const int p0 = plan.start[run.index] + run.group * 8, cols = min(8, plan.start[run.index + 1] - p0);
+      const int length = (int)min((long long)(steps - run.step), w1 - n);
+      n += length;
+      const uint16_t* h = static_cast<const uint16_t*>(a.hidden) + (size_t)plan.order[p0 + min(r, cols - 1)] * 2 * a.f_pad +
+                          run.step * S::kStep + t * 8;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f}, rest[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < length; ++i) {
+        constexpr int kQuarters = S::kStep / 32;
+        uint4 b[2][kQuarters];
 #pragma unroll
-        for (int q = 0; q < kQuarters; ++q)
+        for (int q = 0; q < kQuarters; ++q) {
+          b[0][q] = *reinterpret_cast<const uint4*>(h + q * 32);
+          b[1][q] = *reinterpret_cast<const uint4*>(h + a.f_pad + q * 32);
+        }
+        h += S::kStep;
+        __syncwarp();
+        fetch();
+        copies_wait<S::kSlots - 1>();
+        if constexpr (W4) {
+          __syncwarp();
+          tile_multiply_bf16<T, QG>(from, b, a.fmt.zeros, acc);
+        } else {
+          rows16_multiply<T, 2>(from, acc, b[0]);
+          rows16_multiply<T, 2>(from, rest, b[1]);
+        }
+        from += S::kSlot;
+        if (from == ring + S::kSlots * S::kSlot) from = ring;
+      }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) h[i][q] = *reinterpret_cast<const uint4*>(from + q * 32 + i * 4);
-      } else {
-        const __nv_bfloat16* from =
-            static_cast<const __nv_bfloat16*>(a.hidden) + (size_t)pair * 2 * a.f_pad + place.step * S::kStep + t * 8;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int q = 0; q < kQuarters; ++q) h[i][q] = *reinterpret_cast<const uint4*>(from + (size_t)i * a.f_pad + q * 32);
+      for (int i = 0; i < 4; ++i) {
+        const int col = t * 2 + (i & 1);
+        if (col < cols) {
+          const int p = plan.order[p0 + col];
+          const float v = (acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest)) * (1.f / MoeHidden<U>::kScale);
+          sums[(warp * a.tokens + p / a.topk) * 16 + r + 8 * (i >> 1)] += plan.gate[p] * v;
+        }
       }
       __syncwarp();
-      fetch();
-      copies_wait<S::kSlots - 1>();
-      if (W4) __syncwarp();
-      const uint32_t from = ring + slot * S::kSlot;
-      if (++slot == S::kSlots) slot = 0;
-      if constexpr (W4) {
-        tile_multiply_bf16<T, QG>(from, h, a.fmt.zeros, acc);
-      } else {
-        if constexpr (kScaled) {  // floats into half precision and its remainder
-#pragma unroll
-          for (int q = 0; q < kQuarters; ++q) {
-            const uint32_t raw[8] = {h[0][q].x, h[0][q].y, h[0][q].z, h[0][q].w, h[1][q].x, h[1][q].y, h[1][q].z, h[1][q].w};
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float e0 = __uint_as_float(raw[2 * i]) * up, e1 = __uint_as_float(raw[2 * i + 1]) * up;
-              const __half2 c = __floats2half2_rn(e0, e1);
-              const float2 back = __half22float2(c);
-              const __half2 d = __floats2half2_rn(e0 - back.x, e1 - back.y);
-              hi[i] = *reinterpret_cast<const uint32_t*>(&c);
-              lo[i] = *reinterpret_cast<const uint32_t*>(&d);
-            }
-            h[0][q] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            h[1][q] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          }
-        }
-        rows16_multiply<T, 2>(from, acc, h[0]);
-        rows16_multiply<T, 2>(from, acc, h[1]);
-      }
-      advance(place);
-      if (place.step == 0 || n + 1 == w1) {  // the expert's tokens are finished (as far as this warp goes)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = t * 2 + (i & 1);
-          if (col < cols) {
-            const int p = plan.order[p0 + col];
-            float v = acc[i];
-            if (kScaled) v /= moe_scale(a.peak[p]);
-            sums[(warp * a.tokens + p / a.topk) * 16 + r + 8 * (i >> 1)] += plan.gate[p] * v;
-          }
-          acc[i] = 0.f;
-        }
-        __syncwarp();
-      }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.tokens * 16; i += kMoeThreads) {
