@@ -302,7 +302,12 @@ static int launch_moe(const MoeArgs& a, cudaStream_t st) {
   const cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
   MMBO_COUNT_LAUNCH();
   if (e != cudaSuccess) return (int)e;
-  if ((rc = launch_clustered(up, (unsigned)sm_count(), kMoeThreads, up_smem, 0, st, a))) return rc;
+  // teams of `up`: small ones (fewer sums to join, fewer barriers) as long as every team has a unit
+  MoeArgs b = a;
+  const size_t experts = pairs < (size_t)a.experts ? pairs : (size_t)a.experts, units = experts * ((a.f + 15) / 16);
+  b.team_log2 = 4;
+  while (b.team_log2 > 2 && units >= (size_t)sm_count() * (kMoeWarps >> (b.team_log2 - 1)) * 3 / 4) --b.team_log2;
+  if ((rc = launch_clustered(up, (unsigned)sm_count(), kMoeThreads, up_smem, 0, st, b))) return rc;
   const int blocks = (a.d + 15) / 16;
   return launch_clustered(down, (unsigned)(blocks < sm_count() ? blocks : sm_count()), kMoeThreads, down_smem, 0, st, a);
 }

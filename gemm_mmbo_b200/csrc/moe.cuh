@@ -11,7 +11,7 @@
 //   scores   one warp per (token, expert); also an aligned, zero-padded copy of the activations (for 4-bit experts in half
 //            precision with the groups' sums, as w4_tile_mma wants them)
 //   up       every block repeats the selection for itself (a microsecond, cheaper than another kernel and its launch), then
-//            works through its share of the units (expert, 16 rows of gate and up): sixteen warps split d
+//            teams of 4, 8 or 16 warps work through their shares of the units (expert, 16 rows of gate and up) and split d
 //   down     a block owns 16 rows of the output for all tokens, its warps split the list of (expert, part of f); the sums
 //            of the experts meet in shared memory in a fixed order
 // Each warp has a ring in shared memory that its lanes fill with 16-byte asynchronous copies of weights, every lane with
@@ -36,6 +36,7 @@ struct MoeArgs {
   const void *X, *router, *gate, *up, *down;
   size_t ldx, ldr, ldg, strideG, ldd, strideD;  // strides in elements, for packed experts in bytes
   float beta;
+  int team_log2;  // warps of a team of `up`
   void* Y;
   size_t ldy;
   int* ids;      // tokens x topk, the caller's or null
@@ -50,7 +51,8 @@ struct MoeArgs {
   int d_pad, f_pad; // multiples of 128
 };
 
-// The selection, sorted by expert: `order` holds the pairs (token * topk + slot) of expert 0's tokens, then expert 1's ..;
+// The selection, sorted by expert: `order` holds the pairs (token * topk + slot, and the token again in the upper half: a
+// division saved wherever a column is looked up) of expert 0's tokens, then expert 1's ..;
 // the a-th expert with tokens is expert[a], its pairs order[start[a] .. start[a + 1]).
 struct MoePlan {
   int* active;  // number of experts with tokens
@@ -240,6 +242,9 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], uint32_t
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool have) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most N of the groups committed are under way.
 template <int N>
@@ -256,7 +261,7 @@ template <typename T, int C>
 struct RowsFeed {
   const T *lo, *hi;  // this lane's place in rows r and r + 8
   int j, k;          // its column; a row's length
-  bool have_lo, have_hi, vec;
+  bool have_lo, have_hi, vec, plain;  // plain: everything is there and aligned
   __device__ __forceinline__ void start(const T* base, size_t ld, int rows, int k_, int step, bool vec_) {
     const int lane = threadIdx.x & 31, r = lane >> 2;
     have_lo = r < rows;
@@ -264,25 +269,34 @@ struct RowsFeed {
     j = step * 32 * C + (lane & 3) * 8;
     k = k_;
     vec = vec_;
+    plain = vec && rows >= 16 && k % (32 * C) == 0;
     lo = base + (have_lo ? r * ld : 0) + j;
     hi = base + (have_hi ? (r + 8) * ld : 0) + j;
   }
   __device__ __forceinline__ void fetch(uint32_t to) {
     to += (threadIdx.x & 31) * 16;
+    if (plain) {
 #pragma unroll
-    for (int u = 0; u < C; ++u) {
-      const bool in = j + 32 * u < k;
-      if (vec) {
-        copy16(to + u * 512, in ? lo + 32 * u : lo - j, in && have_lo);
-        copy16(to + (C + u) * 512, in ? hi + 32 * u : hi - j, in && have_hi);
-      } else {
-        sts128(to + u * 512, load8(lo - j, have_lo ? k : 0, j + 32 * u));
-        sts128(to + (C + u) * 512, load8(hi - j, have_hi ? k : 0, j + 32 * u));
+      for (int u = 0; u < C; ++u) {
+        copy16(to + u * 512, lo + 32 * u);
+        copy16(to + (C + u) * 512, hi + 32 * u);
       }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < C; ++u) {
+        const bool in = j + 32 * u < k;
+        if (vec) {
+          copy16(to + u * 512, in ? lo + 32 * u : lo - j, in && have_lo);
+          copy16(to + (C + u) * 512, in ? hi + 32 * u : hi - j, in && have_hi);
+        } else {
+          sts128(to + u * 512, load8(lo - j, have_lo ? k : 0, j + 32 * u));
+          sts128(to + (C + u) * 512, load8(hi - j, have_hi ? k : 0, j + 32 * u));
+        }
+      }
+      j += 32 * C;
     }
     lo += 32 * C;
     hi += 32 * C;
-    j += 32 * C;
   }
 };
 // acc += those weights * columns; b: this lane's 16 bytes of each 32 columns
@@ -313,9 +327,9 @@ struct TileFeed {
     scales = tile + scale_piece;
   }
   __device__ __forceinline__ void fetch(uint32_t to) {
-    copy16(to + piece, codes, true);
-    copy16(to + piece + 512, codes + 512, true);
-    if (has_scale) copy16(to + scale_piece, scales, true);
+    copy16(to + piece, codes);
+    copy16(to + piece + 512, codes + 512);
+    if (has_scale) copy16(to + scale_piece, scales);
     codes += bytes;
     scales += bytes;
   }
@@ -373,9 +387,9 @@ struct MoeHidden<__half> {
 // QG: quarters of a group of packed weights, 0: 16-bit weights.
 template <int QG>
 struct MoeUpShape {
-  static constexpr int kStep = QG ? 128 : 32;  // columns
-  static constexpr uint32_t kHalf = QG ? kTileRoom : 1024, kSlot = 2 * kHalf;  // gate, up
-  static constexpr int kSlots = QG ? 4 : 5;
+  static constexpr int kStep = QG ? 128 : 64;  // columns: whole 128-byte lines of 16-bit rows
+  static constexpr uint32_t kSlot = QG ? kTileRoom : 2048;  // gate and up take turns
+  static constexpr int kSlots = QG ? 8 : 5;
 };
 constexpr size_t kMoeUpSums = (size_t)2 * kMoeWarps * 256 * 4;
 
@@ -433,7 +447,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
   for (int i = threadIdx.x; i < active; i += kMoeThreads) {
     int at = plan.start[i];
     for (int p = 0; p < pairs; ++p)
-      if (ids[p] == plan.expert[i]) plan.order[at++] = p;
+      if (ids[p] == plan.expert[i]) plan.order[at++] = p | (p / a.topk) << 16;
   }
   __syncthreads();
   if (blockIdx.x == 0) {
@@ -444,11 +458,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
     }
   }
 
-  // units: expert, 16 rows, group of eight tokens
+  // units: expert, 16 rows, group of eight tokens; a team of warps shares a unit and cuts d
+  const int WK = 1 << a.team_log2, wk = warp & (WK - 1), team = warp >> a.team_log2, teams = kMoeWarps >> a.team_log2;
   const int blocks = (a.f + 15) / 16;
   int total = 0;
   for (int i = 0; i < active; ++i) total += blocks * ((plan.start[i + 1] - plan.start[i] + 7) / 8);
-  const int begin = (int)((long long)total * blockIdx.x / gridDim.x), end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+  const long long share = (long long)gridDim.x * teams, mine = (long long)blockIdx.x * teams + team;
+  const int begin = (int)(total * mine / share), end = (int)(total * (mine + 1) / share);
   struct Unit {
     int index, rows, group, groups;  // expert (of the active ones), row block, group of tokens
   };
@@ -474,12 +490,12 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
     if (++u.index < active) u.groups = (plan.start[u.index + 1] - plan.start[u.index] + 7) / 8;
   };
 
-  const int steps = (a.d + S::kStep - 1) / S::kStep, s0 = steps * warp / kMoeWarps, s1 = steps * (warp + 1) / kMoeWarps;
+  const int steps = (a.d + S::kStep - 1) / S::kStep, s0 = steps * wk >> a.team_log2, s1 = steps * (wk + 1) >> a.team_log2;
   const bool vec = !W4 && a.ldg % 8 == 0 && a.strideG % 8 == 0 && a.d % 8 == 0 &&
                    ((reinterpret_cast<uintptr_t>(a.gate) | reinterpret_cast<uintptr_t>(a.up)) & 15u) == 0;
   const uint32_t tile_bytes = W4 ? a.fmt.tile_bytes() : 0;
   // the copies run ahead of the products, through the same order
-  using Feed = typename std::conditional<W4, TileFeed, RowsFeed<T, 1>>::type;
+  using Feed = typename std::conditional<W4, TileFeed, RowsFeed<T, 2>>::type;
   Feed gate, up;
   Unit ahead = unit;
   int ahead_n = s0 < s1 ? begin : end, ahead_left = s1 - s0;
@@ -490,20 +506,22 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
     if constexpr (W4) {
       const size_t off = e * a.strideG + ((size_t)ahead.rows * steps + s0) * tile_bytes;
       gate.start(static_cast<const unsigned char*>(a.gate) + off, tile_bytes, 0);
-      up.start(static_cast<const unsigned char*>(a.up) + off, tile_bytes, 16);
+      up.start(static_cast<const unsigned char*>(a.up) + off, tile_bytes, 0);
     } else {
       const size_t off = e * a.strideG + (size_t)ahead.rows * 16 * a.ldg;
       gate.start(static_cast<const T*>(a.gate) + off, a.ldg, a.f - ahead.rows * 16, a.d, s0, vec);
       up.start(static_cast<const T*>(a.up) + off, a.ldg, a.f - ahead.rows * 16, a.d, s0, vec);
     }
   };
+  int turn = 0;  // gate's or up's
   auto fetch = [&]() {
     if (ahead_n < end) {
-      gate.fetch(ahead_at);
-      up.fetch(ahead_at + S::kHalf);
+      if (turn == 0) gate.fetch(ahead_at);
+      else up.fetch(ahead_at);
       ahead_at += S::kSlot;
       if (ahead_at == ring + S::kSlots * S::kSlot) ahead_at = ring;
-      if (--ahead_left == 0) {
+      turn ^= 1;
+      if (turn == 0 && --ahead_left == 0) {
         ahead_left = s1 - s0;
         if (++ahead_n < end) advance(ahead);
         start();
@@ -518,13 +536,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
   for (int n = begin; n < end; ++n) {
     const int p0 = plan.start[unit.index] + unit.group * 8, cols = min(8, plan.start[unit.index + 1] - p0);
     // columns past the last token repeat it; their sums are not used
-    const uint16_t* x = static_cast<const uint16_t*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] / a.topk) * a.d_pad +
+    const uint16_t* x = static_cast<const uint16_t*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] >> 16) * a.d_pad +
                         s0 * S::kStep + t * 8;
     const float *sums0 = nullptr, *sums1 = nullptr;
     if constexpr (W4) {
       const int per = a.d_pad / (32 * QG), at = s0 * (4 / QG);
-      sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] / a.topk) * per + at;
-      sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] / a.topk) * per + at;
+      sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] >> 16) * per + at;
+      sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] >> 16) * per + at;
     }
     float accg[4] = {0.f, 0.f, 0.f, 0.f}, accu[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s = s0; s < s1; ++s) {
@@ -538,42 +556,46 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a)
 #pragma unroll
         for (int g = 0; g < 4 / QG; ++g) xs[g] = make_float2(*sums0++, *sums1++);
       }
-      __syncwarp();
-      fetch();
-      copies_wait<S::kSlots - 1>();
-      if constexpr (W4) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
         __syncwarp();
-        w4_tile_mma<T, QG>(from, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, accg);
-        w4_tile_mma<T, QG>(from + S::kHalf, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, accu);
-      } else {
-        rows16_multiply<T, 1>(from, accg, b);
-        rows16_multiply<T, 1>(from + S::kHalf, accu, b);
+        fetch();
+        copies_wait<S::kSlots - 1>();
+        if constexpr (W4) {
+          __syncwarp();
+          w4_tile_mma<T, QG>(from, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, half ? accu : accg);
+        } else {
+          rows16_multiply<T, 2>(from, half ? accu : accg, b);
+        }
+        from += S::kSlot;
+        if (from == ring + S::kSlots * S::kSlot) from = ring;
       }
-      from += S::kSlot;
-      if (from == ring + S::kSlots * S::kSlot) from = ring;
     }
-    // [warp][gate, up][column][row]
-    float* mine = sums + ((n & 1) * kMoeWarps + warp) * 256;
+    // [turn][warp][gate, up][column][row]
+    float* ours = sums + ((n & 1) * kMoeWarps + (team << a.team_log2)) * 256;
+    float* mine_sums = ours + wk * 256;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = (t * 2 + (i & 1)) * 16 + r + 8 * (i >> 1);
-      mine[at] = accg[i];
-      mine[128 + at] = accu[i];
+      mine_sums[at] = accg[i];
+      mine_sums[128 + at] = accu[i];
     }
-    __syncthreads();
-    // finished by four warps, others' turn with every unit
-    const int i = (int)((threadIdx.x + 384 * (n & 3)) & (kMoeThreads - 1));
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(WK * 32) : "memory");
+    // finished by four warps, with larger teams others' turn with every unit
+    const int i = (wk * 32 + lane + 384 * (n & 3)) & (WK * 32 - 1);
     if (i < cols * 16) {
-      const float* p = sums + (n & 1) * kMoeWarps * 256 + i;
+      const float* p = ours + i;
       float g = 0.f, u = 0.f;
+      for (int w = 0; w < WK; w += 4) {
 #pragma unroll
-      for (int w = 0; w < kMoeWarps; ++w) {
-        g += p[w * 256];
-        u += p[w * 256 + 128];
+        for (int v = 0; v < 4; ++v) {
+          g += p[(w + v) * 256];
+          u += p[(w + v) * 256 + 128];
+        }
       }
-      const int row = unit.rows * 16 + (i & 15), pair = plan.order[p0 + i / 16];
+      const int row = unit.rows * 16 + (i & 15), entry = plan.order[p0 + i / 16], pair = entry & 0xffff;
       if (W4) {
-        const float2 undo = a.x_undo[pair / a.topk];
+        const float2 undo = a.x_undo[entry >> 16];
         g *= undo.x * undo.y;
         u *= undo.x * undo.y;
       }
@@ -697,18 +719,32 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs 
       const int p0 = plan.start[run.index] + run.group * 8, cols = min(8, plan.start[run.index + 1] - p0);
       const int length = (int)min((long long)(steps - run.step), w1 - n);
       n += length;
-      const uint16_t* h = static_cast<const uint16_t*>(a.hidden) + (size_t)plan.order[p0 + min(r, cols - 1)] * 2 * a.f_pad +
+      const uint16_t* h = static_cast<const uint16_t*>(a.hidden) + (size_t)(plan.order[p0 + min(r, cols - 1)] & 0xffff) * 2 * a.f_pad +
                           run.step * S::kStep + t * 8;
       float acc[4] = {0.f, 0.f, 0.f, 0.f}, rest[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int i = 0; i < length; ++i) {
-        constexpr int kQuarters = S::kStep / 32;
-        uint4 b[2][kQuarters];
+      constexpr int kQuarters = S::kStep / 32;
+      uint4 b[2][kQuarters], ahead_b[2][kQuarters];
+      auto columns = [&](uint4(&to)[2][kQuarters]) {
 #pragma unroll
         for (int q = 0; q < kQuarters; ++q) {
-          b[0][q] = *reinterpret_cast<const uint4*>(h + q * 32);
-          b[1][q] = *reinterpret_cast<const uint4*>(h + a.f_pad + q * 32);
+          to[0][q] = *reinterpret_cast<const uint4*>(h + q * 32);
+          to[1][q] = *reinterpret_cast<const uint4*>(h + a.f_pad + q * 32);
         }
         h += S::kStep;
+      };
+      if (!W4) columns(ahead_b);
+      for (int i = 0; i < length; ++i) {
+        // 16-bit weights: the columns of the next step, too (packed ones leave no registers for it)
+        if (W4) {
+          columns(b);
+        } else {
+#pragma unroll
+          for (int q = 0; q < kQuarters; ++q) {
+            b[0][q] = ahead_b[0][q];
+            b[1][q] = ahead_b[1][q];
+          }
+          if (i + 1 < length) columns(ahead_b);
+        }
         __syncwarp();
         fetch();
         copies_wait<S::kSlots - 1>();
@@ -726,9 +762,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs 
       for (int i = 0; i < 4; ++i) {
         const int col = t * 2 + (i & 1);
         if (col < cols) {
-          const int p = plan.order[p0 + col];
+          const int entry = plan.order[p0 + col];
           const float v = (acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest)) * (1.f / MoeHidden<U>::kScale);
-          sums[(warp * a.tokens + p / a.topk) * 16 + r + 8 * (i >> 1)] += plan.gate[p] * v;
+          sums[(warp * a.tokens + (entry >> 16)) * 16 + r + 8 * (i >> 1)] += plan.gate[entry & 0xffff] * v;
         }
       }
       __syncwarp();
