@@ -277,19 +277,14 @@ static int check_moe_sizes(int dtype, size_t tokens, size_t d, size_t f, size_t 
   return MMBO_OK;
 }
 
+// QG: quarters of a group of packed weights, 0: 16-bit weights.
 template <typename T, int QG>
-static int launch_moe(const MoeArgs& a, cudaStream_t st) {
-  using Up = MoeUpShape<QG>;
-  using Down = MoeDownShape<QG>;
+static int launch_moe(const MoeArgs& args, cudaStream_t st) {
+  MoeArgs a = args;
   const size_t pairs = (size_t)a.tokens * a.topk, words = MoePlan::words(a.experts, (int)pairs);
-  const size_t up_smem = (size_t)kMoeWarps * Up::kSlots * Up::kSlot + kMoeUpSums + (words + pairs + a.experts) * 4;
-  const size_t down_smem = (size_t)kMoeWarps * (Down::kSlots * Down::kSlot + a.tokens * 16 * 4) + words * 4;
-  if (up_smem > kGemvSmem || down_smem > kGemvSmem) return MMBO_ERR_TOO_LARGE;
-  auto up = moe_up_kernel<T, QG>;
-  auto down = moe_down_kernel<T, QG>;
-  static bool up_ready[kMaxDevices], down_ready[kMaxDevices];
-  int rc;
-  if ((rc = allow_smem(up, kGemvSmem, up_ready)) || (rc = allow_smem(down, kGemvSmem, down_ready))) return rc;
+  const size_t up_rest = kMoeUpSums + (words + pairs + a.experts) * 4;
+  const size_t down_rest = (size_t)kMoeWarps * a.tokens * 16 * 4 + words * 4;
+  const size_t rows = (a.d + 15) / 16, down_blocks = rows < (size_t)sm_count() ? rows : (size_t)sm_count();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((a.experts + 7) / 8 + 1), (unsigned)a.tokens);
   cfg.blockDim = dim3(256);
@@ -299,17 +294,38 @@ static int launch_moe(const MoeArgs& a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = settings().pdl ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
-  MMBO_COUNT_LAUNCH();
-  if (e != cudaSuccess) return (int)e;
-  // teams of `up`: small ones (fewer sums to join, fewer barriers) as long as every team has a unit
-  MoeArgs b = a;
-  const size_t experts = pairs < (size_t)a.experts ? pairs : (size_t)a.experts, units = experts * ((a.f + 15) / 16);
-  b.team_log2 = 4;
-  while (b.team_log2 > 2 && units >= (size_t)sm_count() * (kMoeWarps >> (b.team_log2 - 1)) * 3 / 4) --b.team_log2;
-  if ((rc = launch_clustered(up, (unsigned)sm_count(), kMoeThreads, up_smem, 0, st, b))) return rc;
-  const int blocks = (a.d + 15) / 16;
-  return launch_clustered(down, (unsigned)(blocks < sm_count() ? blocks : sm_count()), kMoeThreads, down_smem, 0, st, a);
+  static bool up_ready[kMaxDevices], down_ready[kMaxDevices];
+  int rc;
+  if constexpr (QG == 0) {
+    auto up = moe_up16_kernel<T>;
+    auto down = moe_down16_kernel<T>;
+    if ((rc = allow_smem(up, kGemvSmem, up_ready)) || (rc = allow_smem(down, kGemvSmem, down_ready))) return rc;
+    const size_t up_smem = kMoeUpStages * (size_t)(32 * kMoeRowBytes) + up_rest;
+    const size_t down_smem = kMoeDownStages * (size_t)(16 * kMoeRowBytes) + down_rest;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
+    MMBO_COUNT_LAUNCH();
+    if (e != cudaSuccess) return (int)e;
+    if ((rc = launch_clustered(up, (unsigned)sm_count(), kMoeFed16Threads, up_smem, 0, st, a)))
+      return rc;
+    return launch_clustered(down, (unsigned)down_blocks, kMoeFed16Threads, down_smem, 0, st, a);
+  } else {
+    auto up = moe_up4_kernel<T, QG>;
+    auto down = moe_down4_kernel<T, QG>;
+    if ((rc = allow_smem(up, kGemvSmem, up_ready)) || (rc = allow_smem(down, kGemvSmem, down_ready))) return rc;
+    // teams of `up`: small ones (fewer sums to join, fewer barriers) as long as every team has a unit
+    const size_t experts = pairs < (size_t)a.experts ? pairs : (size_t)a.experts, units = experts * ((a.f + 15) / 16);
+    a.team_log2 = 4;
+    while (a.team_log2 > 2 && units >= (size_t)sm_count() * (kMoeWarps >> (a.team_log2 - 1)) * 3 / 4) --a.team_log2;
+    const size_t tile = a.fmt.tile_bytes();
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
+    MMBO_COUNT_LAUNCH();
+    if (e != cudaSuccess) return (int)e;
+    if ((rc = launch_clustered(up, (unsigned)sm_count(), kMoeThreads, kMoeWarps * kMoeSlots * 2 * kMoeTiles * tile + up_rest, 0, st,
+                               a)))
+      return rc;
+    return launch_clustered(down, (unsigned)down_blocks, kMoeThreads, kMoeWarps * kMoeSlots * kMoeDownTiles * tile + down_rest, 0,
+                            st, a);
+  }
 }
 
 template <typename T>

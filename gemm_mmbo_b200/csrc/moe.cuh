@@ -14,12 +14,10 @@
 //            teams of 4, 8 or 16 warps work through their shares of the units (expert, 16 rows of gate and up) and split d
 //   down     a block owns 16 rows of the output for all tokens, its warps split the list of (expert, part of f); the sums
 //            of the experts meet in shared memory in a fixed order
-// Each warp has a ring in shared memory that its lanes fill with 16-byte asynchronous copies of weights, every lane with
-// the pieces that it will itself read as fragments of mma.sync.m16n8k16, so the ring needs no barrier and the copies in
-// flight no registers; the columns come straight from L2, the same 16 bytes' worth of k of a lane's token, asked for
-// before the wait for the weights.  (Weights loaded straight to registers one step ahead left 64 KB in flight an SM at
-// best: 255 us for the batch of 48 tokens in `up`, 2.9 TB/s.)  Tokens are the eight columns of the instruction; an expert with more tokens is taken in groups of
-// eight, the later ones finding its weights in L2.
+// Weights come through rings in shared memory that a feeding warp keeps full with bulk copies, long pieces of rows or tiles;
+// the columns, fragments of mma.sync.m16n8k16 (the same 16 bytes' worth of k of a lane's token), come straight from L2,
+// asked for before the wait for the weights.  Tokens are the eight columns of the instruction; an expert with more tokens
+// is taken in groups of eight, the later ones finding its weights in L2.
 #pragma once
 
 #include "w4_umma.cuh"
@@ -53,23 +51,26 @@ struct MoeArgs {
 
 // The selection, sorted by expert: `order` holds the pairs (token * topk + slot, and the token again in the upper half: a
 // division saved wherever a column is looked up) of expert 0's tokens, then expert 1's ..;
-// the a-th expert with tokens is expert[a], its pairs order[start[a] .. start[a + 1]).
+// the a-th expert with tokens is expert[a], its pairs order[start[a] .. start[a + 1]), in groups of eight, the first of which
+// is number base[a].
 struct MoePlan {
   int* active;  // number of experts with tokens
   int* expert;
   int* start;
+  int* base;
   int* order;
   float* gate;  // per pair
   __host__ __device__ static int words(int experts, int pairs) {
     const int a = experts < pairs ? experts : pairs;
-    return 1 + a + a + 1 + 2 * pairs;
+    return 1 + a + 2 * (a + 1) + 2 * pairs;
   }
   __device__ __forceinline__ MoePlan(int* at, int experts, int pairs) {
     const int a = min(experts, pairs);
     active = at;
     expert = at + 1;
     start = expert + a;
-    order = start + a + 1;
+    base = start + a + 1;
+    order = base + a + 1;
     gate = reinterpret_cast<float*>(order + pairs);
   }
 };
@@ -193,31 +194,28 @@ __device__ __forceinline__ void moe_select(const MoeArgs& a, const float* from, 
   for (int e = lane; e < a.experts; e += 32) sum += expf(scores[e] - top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  float chosen = 0.f;
-  uint64_t last = ~0ull;  // (key, ~index) of the expert taken before
+  uint32_t last_key = 0xffffffffu;
+  int last = -1;  // the expert taken before
   for (int s = 0; s < a.topk; ++s) {
-    uint64_t best = 0;
+    uint32_t key = 0;
+    int best = 0;
     for (int e = lane; e < a.experts; e += 32) {
-      const uint64_t c = ((uint64_t)moe_score_key(scores[e]) << 32) | (0xffffffffu - (uint32_t)e);
-      if (c < last && c > best) best = c;
+      const uint32_t k = moe_score_key(scores[e]);
+      if ((k < last_key || (k == last_key && e > last)) && k > key) {
+        key = k;
+        best = e;
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t c = __shfl_xor_sync(0xffffffffu, best, o);
-      best = c > best ? c : best;
-    }
-    last = best;
-    const uint32_t e = 0xffffffffu - (uint32_t)best;
-    const float p = expf(scores[e] - top) / sum;
-    chosen += p;
-    if (lane == 0) {
-      ids[s] = (int)e;
-      gates[s] = p;
-    }
+    last_key = __reduce_max_sync(0xffffffffu, key);
+    last = (int)__reduce_min_sync(0xffffffffu, key == last_key ? (uint32_t)best : 0xffffffffu);
+    if (lane == 0) ids[s] = last;
   }
   __syncwarp();
-  if (a.renorm)
-    for (int s = lane; s < a.topk; s += 32) gates[s] /= chosen;
+  const float p = lane < a.topk ? expf(scores[ids[lane]] - top) / sum : 0.f;
+  float chosen = p;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
+  if (lane < a.topk) gates[lane] = a.renorm ? p / chosen : p;
 }
 
 // ---------------------------------------------------------------- fragments -----------
@@ -237,103 +235,6 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// ---------------------------------------------------------------- rings ---------------
-// 16 bytes to shared memory, in the background; zeros where `have` is false.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool have) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Waits until at most N of the groups committed are under way.
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
-// Feeds a ring with sixteen rows of 16-bit weights, 32 C columns at a time: piece (h, u) of a lane, columns 32 u + 8 t ..
-// + 7 of row r + 8 h, goes to (h C + u) * 512 + lane * 16.  Rows that do not exist and columns behind k come as zeros.
-template <typename T, int C>
-struct RowsFeed {
-  const T *lo, *hi;  // this lane's place in rows r and r + 8
-  int j, k;          // its column; a row's length
-  bool have_lo, have_hi, vec, plain;  // plain: everything is there and aligned
-  __device__ __forceinline__ void start(const T* base, size_t ld, int rows, int k_, int step, bool vec_) {
-    const int lane = threadIdx.x & 31, r = lane >> 2;
-    have_lo = r < rows;
-    have_hi = r + 8 < rows;
-    j = step * 32 * C + (lane & 3) * 8;
-    k = k_;
-    vec = vec_;
-    plain = vec && rows >= 16 && k % (32 * C) == 0;
-    lo = base + (have_lo ? r * ld : 0) + j;
-    hi = base + (have_hi ? (r + 8) * ld : 0) + j;
-  }
-  __device__ __forceinline__ void fetch(uint32_t to) {
-    to += (threadIdx.x & 31) * 16;
-    if (plain) {
-#pragma unroll
-      for (int u = 0; u < C; ++u) {
-        copy16(to + u * 512, lo + 32 * u);
-        copy16(to + (C + u) * 512, hi + 32 * u);
-      }
-    } else {
-#pragma unroll 1
-      for (int u = 0; u < C; ++u) {
-        const bool in = j + 32 * u < k;
-        if (vec) {
-          copy16(to + u * 512, in ? lo + 32 * u : lo - j, in && have_lo);
-          copy16(to + (C + u) * 512, in ? hi + 32 * u : hi - j, in && have_hi);
-        } else {
-          sts128(to + u * 512, load8(lo - j, have_lo ? k : 0, j + 32 * u));
-          sts128(to + (C + u) * 512, load8(hi - j, have_hi ? k : 0, j + 32 * u));
-        }
-      }
-      j += 32 * C;
-    }
-    lo += 32 * C;
-    hi += 32 * C;
-  }
-};
-// acc += those weights * columns; b: this lane's 16 bytes of each 32 columns
-template <typename T, int C>
-__device__ __forceinline__ void rows16_multiply(uint32_t from, float (&acc)[4], const uint4 (&b)[C]) {
-  const uint32_t at = from + (threadIdx.x & 31) * 16;
-#pragma unroll
-  for (int u = 0; u < C; ++u) {
-    const uint4 lo = lds128(at + u * 512), hi = lds128(at + (C + u) * 512);
-    mma_16816<T>(acc, lo.x, hi.x, lo.y, hi.y, b[u].x, b[u].y);
-    mma_16816<T>(acc, lo.z, hi.z, lo.w, hi.w, b[u].z, b[u].w);
-  }
-}
-
-// The same with packed tiles, in their own layout: two pieces of codes a lane, scales and zero points by the lanes from
-// `first` on.  (Others read what a lane copied: __syncwarp() behind the wait.)
-struct TileFeed {
-  const unsigned char *codes, *scales;
-  uint32_t piece, scale_piece, bytes;
-  bool has_scale;
-  __device__ __forceinline__ void start(const unsigned char* tile, uint32_t tile_bytes, int first) {
-    const int lane = threadIdx.x & 31, i = lane - first;
-    bytes = tile_bytes;
-    piece = w4_piece(lane >> 2, lane & 3);
-    has_scale = i >= 0 && i * 16 < (int)tile_bytes - kW4Codes;
-    scale_piece = kW4Codes + (has_scale ? i * 16 : 0);
-    codes = tile + piece;
-    scales = tile + scale_piece;
-  }
-  __device__ __forceinline__ void fetch(uint32_t to) {
-    copy16(to + piece, codes);
-    copy16(to + piece + 512, codes + 512);
-    if (has_scale) copy16(to + scale_piece, scales);
-    codes += bytes;
-    scales += bytes;
-  }
-};
 // acc += a packed tile * two bfloat16 columns' worth (a value and its remainder, by quarters).  Codes become exact integers:
 // for w4_tile_mma a hidden vector would first have to be brought to half precision.
 template <typename T, int QG>
@@ -367,8 +268,6 @@ __device__ __forceinline__ void tile_multiply_bf16(uint32_t tile, const uint4 (&
     for (int i = 0; i < 4; ++i) acc[i] = fmaf(i < 2 ? s.x : s.y, part[0][i] + part[1][i], acc[i]);
   }
 }
-constexpr uint32_t kTileRoom = kW4Codes + 4 * 48;  // of a tile in a ring, whatever its groups
-
 // Hidden vectors as products take them: a 16-bit value and what its rounding left, so that 16 bits and more survive.
 // bfloat16 has the range of a float.  Half precision holds h / 64 and 2^11 times the remainder: magnitudes up to 4.19e6,
 // steps of 2^-30 near zero (results in half precision have steps of 2^-24).
@@ -383,410 +282,685 @@ struct MoeHidden<__half> {
   static constexpr float kScale = 0x1p-6f, kRest = 0x1p11f;
 };
 
-// ---------------------------------------------------------------- up ------------------
-// QG: quarters of a group of packed weights, 0: 16-bit weights.
-template <int QG>
-struct MoeUpShape {
-  static constexpr int kStep = QG ? 128 : 64;  // columns: whole 128-byte lines of 16-bit rows
-  static constexpr uint32_t kSlot = QG ? kTileRoom : 2048;  // gate and up take turns
-  static constexpr int kSlots = QG ? 8 : 5;
-};
+// The selection and its plan, by every block for itself; `scores`: kMoeUpSums bytes of shared memory.  The block's first
+// kMoeThreads threads take part, all of them pass the barriers.
 constexpr size_t kMoeUpSums = (size_t)2 * kMoeWarps * 256 * 4;
-
-template <typename T, int QG>
-__global__ void __launch_bounds__(kMoeThreads, 1) moe_up_kernel(const MoeArgs a) {
-  using S = MoeUpShape<QG>;
-  constexpr bool W4 = QG > 0;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  const int pairs = a.tokens * a.topk;
-  // shared memory: rings | partial sums (before that: scores) | plan | ids | count
-  const uint32_t ring = smem_u32(smem) + warp * S::kSlots * S::kSlot;
-  float* sums = reinterpret_cast<float*>(smem + kMoeWarps * S::kSlots * S::kSlot);
-  int* at_plan = reinterpret_cast<int*>(sums) + kMoeUpSums / 4;
-  MoePlan plan(at_plan, a.experts, pairs);
-  int* ids = at_plan + MoePlan::words(a.experts, pairs);
-  int* count = ids + pairs;  // experts
-  griddep_launch_dependents();
-  for (int e = threadIdx.x; e < a.experts; e += kMoeThreads) count[e] = 0;
-  griddep_wait();
-
-  // the selection, by every block for itself
+template <typename A>
+__device__ __forceinline__ void moe_make_plan(const A& a, MoePlan& plan, int* ids, int* count, float* scores) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, pairs = a.tokens * a.topk;
   const int selecting = min(kMoeWarps, (int)(kMoeUpSums / 4) / a.experts);  // warps that have room for a token's scores
+  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) count[e] = 0;
   for (int tok = warp; warp < selecting && tok < a.tokens; tok += selecting)
-    moe_select(a, a.scores + (size_t)tok * a.experts, sums + warp * a.experts, ids + tok * a.topk, plan.gate + tok * a.topk);
+    moe_select(a, a.scores + (size_t)tok * a.experts, scores + warp * a.experts, ids + tok * a.topk, plan.gate + tok * a.topk);
   __syncthreads();
-  for (int p = threadIdx.x; p < pairs; p += kMoeThreads) atomicAdd(&count[ids[p]], 1);
+  for (int p = threadIdx.x; p < pairs; p += blockDim.x) atomicAdd(&count[ids[p]], 1);
   __syncthreads();
   if (warp == 0) {  // experts with tokens, numbered in order, and where their pairs start
-    int n = 0, at = 0;
+    int n = 0, at = 0, groups = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
       const int e = e0 + lane, c = e < a.experts ? count[e] : 0;
-      int before = c;
+      int before = c, before_groups = (c + 7) / 8;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
+        const int v = __shfl_up_sync(0xffffffffu, before, o), w = __shfl_up_sync(0xffffffffu, before_groups, o);
+        if (lane >= o) {
+          before += v;
+          before_groups += w;
+        }
       }
       const unsigned live = __ballot_sync(0xffffffffu, c > 0);
       if (c > 0) {
         const int i = n + __popc(live & ((1u << lane) - 1u));
         plan.expert[i] = e;
         plan.start[i] = at + before - c;
+        plan.base[i] = groups + before_groups - (c + 7) / 8;
       }
       n += __popc(live);
       at += __shfl_sync(0xffffffffu, before, 31);
+      groups += __shfl_sync(0xffffffffu, before_groups, 31);
     }
     if (lane == 0) {
       *plan.active = n;
       plan.start[n] = at;
+      plan.base[n] = groups;
     }
   }
   __syncthreads();
   const int active = *plan.active;
-  for (int i = threadIdx.x; i < active; i += kMoeThreads) {
+  for (int i = warp; i < active; i += blockDim.x / 32) {
+    const int e = plan.expert[i];
     int at = plan.start[i];
-    for (int p = 0; p < pairs; ++p)
-      if (ids[p] == plan.expert[i]) plan.order[at++] = p | (p / a.topk) << 16;
+    for (int p0 = 0; p0 < pairs; p0 += 32) {
+      const int p = p0 + lane;
+      const bool its = p < pairs && ids[p] == e;
+      const unsigned which = __ballot_sync(0xffffffffu, its);
+      if (its) plan.order[at + __popc(which & ((1u << lane) - 1u))] = p | (p / a.topk) << 16;
+      at += __popc(which);
+    }
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < MoePlan::words(a.experts, pairs); i += kMoeThreads) a.plan[i] = at_plan[i];
-    for (int p = threadIdx.x; p < pairs; p += kMoeThreads) {
+    for (int i = threadIdx.x; i < MoePlan::words(a.experts, pairs); i += blockDim.x) a.plan[i] = plan.active[i];
+    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
       if (a.ids) a.ids[p] = ids[p];
       if (a.gates) a.gates[p] = plan.gate[p];
     }
   }
+}
 
-  // units: expert, 16 rows, group of eight tokens; a team of warps shares a unit and cuts d
-  const int WK = 1 << a.team_log2, wk = warp & (WK - 1), team = warp >> a.team_log2, teams = kMoeWarps >> a.team_log2;
-  const int blocks = (a.f + 15) / 16;
-  int total = 0;
-  for (int i = 0; i < active; ++i) total += blocks * ((plan.start[i + 1] - plan.start[i] + 7) / 8);
-  const long long share = (long long)gridDim.x * teams, mine = (long long)blockIdx.x * teams + team;
-  const int begin = (int)(total * mine / share), end = (int)(total * (mine + 1) / share);
-  struct Unit {
-    int index, rows, group, groups;  // expert (of the active ones), row block, group of tokens
-  };
-  Unit unit{0, 0, 0, 0};
-  {
-    int at = 0;
-    for (; unit.index < active; ++unit.index) {
-      const int g = (plan.start[unit.index + 1] - plan.start[unit.index] + 7) / 8;
-      if (begin < at + blocks * g) {
-        unit.groups = g;
-        unit.rows = (begin - at) / g;
-        unit.group = (begin - at) % g;
-        break;
-      }
-      at += blocks * g;
+// The units of `up`, in order: experts with tokens, row blocks of the hidden vector, groups of eight tokens.
+struct MoeUnit {
+  int index, rows, group, groups;
+  __device__ __forceinline__ static int total(const MoePlan& plan, int blocks) { return blocks * plan.base[*plan.active]; }
+  __device__ __forceinline__ void find(const MoePlan& plan, int blocks, int number) {
+    int lo = 0, hi = *plan.active;  // blocks * base[lo] <= number
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      (blocks * plan.base[mid] <= number ? lo : hi) = mid;
+    }
+    index = lo;
+    groups = plan.base[lo + 1] - plan.base[lo];
+    rows = (number - blocks * plan.base[lo]) / groups;
+    group = (number - blocks * plan.base[lo]) % groups;
+  }
+  __device__ __forceinline__ void advance(const MoePlan& plan, int blocks) {
+    if (++group < groups) return;
+    group = 0;
+    if (++rows < blocks) return;
+    rows = 0;
+    if (++index < *plan.active) groups = plan.base[index + 1] - plan.base[index];
+  }
+};
+
+// A hidden value into the workspace, as the products with `down` take it.
+template <typename U>
+__device__ __forceinline__ void moe_store_hidden(const MoeArgs& a, int pair, int row, float g, float u) {
+  const float h = row < a.f ? g / (1.f + expf(-g)) * u : 0.f;
+  U* out = static_cast<U*>(a.hidden) + (size_t)pair * 2 * a.f_pad + row;
+  const float scaled = h * MoeHidden<U>::kScale;
+  const U v = from_f32<U>(scaled);
+  const float rest = (scaled - to_f32(v)) * MoeHidden<U>::kRest;
+  out[0] = v;
+  out[a.f_pad] = from_f32<U>(isfinite(rest) ? rest : 0.f);
+}
+
+// ---------------------------------------------------------------- up ------------------
+// Joins a unit's sums, [warp][gate, up][column][row] of `warps` warps at `sums`, and stores the hidden values; thread i of
+// those that share the unit.
+template <typename U>
+__device__ __forceinline__ void moe_finish_unit(const MoeArgs& a, const float* sums, int warps, int i, int cols, int rows,
+                                                const int* order, bool packed) {
+  if (i >= cols * 16) return;
+  float g = 0.f, u = 0.f;
+  for (int w = 0; w < warps; w += 4) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      g += sums[(w + v) * 256 + i];
+      u += sums[(w + v) * 256 + 128 + i];
     }
   }
-  auto advance = [&](Unit& u) {
-    if (++u.group < u.groups) return;
-    u.group = 0;
-    if (++u.rows < blocks) return;
-    u.rows = 0;
-    if (++u.index < active) u.groups = (plan.start[u.index + 1] - plan.start[u.index] + 7) / 8;
-  };
+  const int entry = order[i / 16];
+  if (packed) {
+    const float2 undo = a.x_undo[entry >> 16];
+    g *= undo.x * undo.y;
+    u *= undo.x * undo.y;
+  }
+  moe_store_hidden<U>(a, entry & 0xffff, rows * 16 + (i & 15), g, u);
+}
+__device__ __forceinline__ void moe_keep_sums(float* to, const float (&gate)[4], const float (&up)[4]) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = (t * 2 + (i & 1)) * 16 + r + 8 * (i >> 1);
+    to[at] = gate[i];
+    to[128 + at] = up[i];
+  }
+}
 
-  const int steps = (a.d + S::kStep - 1) / S::kStep, s0 = steps * wk >> a.team_log2, s1 = steps * (wk + 1) >> a.team_log2;
-  const bool vec = !W4 && a.ldg % 8 == 0 && a.strideG % 8 == 0 && a.d % 8 == 0 &&
+// 16-bit weights.  A stage holds 512 columns of 16 rows of gate and of up, each row one copy of 1 KB (a warp's own copies of
+// 64 or 128 bytes a row left DRAM at 3.9 TB/s).  Teams of four warps take the stages in turn: with all sixteen in step on
+// every stage the columns' way from L2 was the bound (390 us instead of 241 for 48 tokens, 8 of 64 experts each, 2048 to 1408).  Rows lie 64 bytes out of step:
+// conflict-free 16-byte reads.
+constexpr int kMoeChunk = 512, kMoeTeam = 4;
+constexpr uint32_t kMoeRowBytes = kMoeChunk * 2 + 64;
+// Multiples of the teams: a team always waits at the same barriers, phase after phase (one that skipped phases could take an
+// older one for its own).
+constexpr int kMoeUpStages = 4, kMoeDownStages = 8;
+static_assert(kMoeUpStages % (kMoeWarps / kMoeTeam) == 0 && kMoeDownStages % (kMoeWarps / kMoeTeam) == 0, "");
+// Feeding warps, each for a part of the rows of a stage: a copy costs the warp that issues it some 30 clocks.
+constexpr int kMoeFeeders = 4, kMoeFed16Threads = kMoeThreads + kMoeFeeders * 32;
+
+// One warp's copies of `rows` rows into a stage.  One elected lane issues them: 100 clocks a copy with one row to a lane.
+template <typename T>
+__device__ __forceinline__ void moe_bring_rows(uint32_t to, const T* src, size_t ld, int rows, uint32_t bytes, uint32_t bar) {
+  if (elect_one()) {
+    mbar_expect_tx(bar, rows * bytes);
+#pragma unroll 4
+    for (int i = 0; i < rows; ++i) bulk_load(to + i * kMoeRowBytes, src + i * ld, bytes, bar);
+  }
+  __syncwarp();
+}
+
+// Sixteen bytes of a lane's row in a stage; zeros where the row ends before them.
+__device__ __forceinline__ uint4 moe_piece(uint32_t stage, int row, int column, int columns) {
+  return column < columns ? lds128(stage + row * kMoeRowBytes + column * 2) : make_uint4(0, 0, 0, 0);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const MoeArgs a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) unsigned long long full[kMoeUpStages], empty[kMoeUpStages], sums_full[2], sums_free[2];
+  __shared__ uint32_t abort_flag;
+  constexpr uint32_t kStage = 32 * kMoeRowBytes;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int pairs = a.tokens * a.topk;
+  // shared memory: stages | partial sums (before that: scores) | plan | ids | count
+  const uint32_t ring = smem_u32(smem);
+  float* sums = reinterpret_cast<float*>(smem + kMoeUpStages * kStage);
+  int* at_plan = reinterpret_cast<int*>(sums) + kMoeUpSums / 4;
+  MoePlan plan(at_plan, a.experts, pairs);
+  int* ids = at_plan + MoePlan::words(a.experts, pairs);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kMoeUpStages; ++i) {
+      mbar_init(smem_u32(&full[i]), kMoeFeeders);
+      mbar_init(smem_u32(&empty[i]), kMoeTeam);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sums_full[i]), kMoeWarps);
+      mbar_init(smem_u32(&sums_free[i]), kMoeTeam);
+    }
+  }
+  fence_mbar_init();
+  griddep_launch_dependents();
+  griddep_wait();
+  moe_make_plan(a, plan, ids, ids + pairs, sums);
+
+  const int blocks = (a.f + 15) / 16, total = MoeUnit::total(plan, blocks);
+  const int begin = (int)((long long)total * blockIdx.x / gridDim.x), end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
+  MoeUnit unit;
+  unit.find(plan, blocks, begin);
+  // rows that bulk copies can address; others are read by the multiplying warps themselves
+  const bool fed = a.ldg % 8 == 0 && a.strideG % 8 == 0 && a.d % 8 == 0 &&
                    ((reinterpret_cast<uintptr_t>(a.gate) | reinterpret_cast<uintptr_t>(a.up)) & 15u) == 0;
-  const uint32_t tile_bytes = W4 ? a.fmt.tile_bytes() : 0;
-  // the copies run ahead of the products, through the same order
-  using Feed = typename std::conditional<W4, TileFeed, RowsFeed<T, 2>>::type;
-  Feed gate, up;
-  Unit ahead = unit;
-  int ahead_n = s0 < s1 ? begin : end, ahead_left = s1 - s0;
-  uint32_t ahead_at = ring;
-  auto start = [&]() {
-    if (ahead_n >= end) return;
-    const size_t e = plan.expert[ahead.index];
-    if constexpr (W4) {
-      const size_t off = e * a.strideG + ((size_t)ahead.rows * steps + s0) * tile_bytes;
-      gate.start(static_cast<const unsigned char*>(a.gate) + off, tile_bytes, 0);
-      up.start(static_cast<const unsigned char*>(a.up) + off, tile_bytes, 0);
-    } else {
-      const size_t off = e * a.strideG + (size_t)ahead.rows * 16 * a.ldg;
-      gate.start(static_cast<const T*>(a.gate) + off, a.ldg, a.f - ahead.rows * 16, a.d, s0, vec);
-      up.start(static_cast<const T*>(a.up) + off, a.ldg, a.f - ahead.rows * 16, a.d, s0, vec);
-    }
-  };
-  int turn = 0;  // gate's or up's
-  auto fetch = [&]() {
-    if (ahead_n < end) {
-      if (turn == 0) gate.fetch(ahead_at);
-      else up.fetch(ahead_at);
-      ahead_at += S::kSlot;
-      if (ahead_at == ring + S::kSlots * S::kSlot) ahead_at = ring;
-      turn ^= 1;
-      if (turn == 0 && --ahead_left == 0) {
-        ahead_left = s1 - s0;
-        if (++ahead_n < end) advance(ahead);
-        start();
+  const int chunks = (a.d + kMoeChunk - 1) / kMoeChunk, units = end - begin;
+  constexpr int kTeams = kMoeWarps / kMoeTeam;
+  bool ok = true;
+  int count = 0;  // of stages
+  if (warp >= kMoeWarps) {
+    constexpr int kRows = 32 / kMoeFeeders;
+    const int first = (warp - kMoeWarps) * kRows;  // of the stage's rows, those that this warp brings
+    for (int n = 0; fed && ok && n < units; ++n) {
+      const int row = unit.rows * 16 + (first & 15), have = min(kRows, max(a.f - row, 0));
+      const T* src = static_cast<const T*>(first < 16 ? a.gate : a.up) + plan.expert[unit.index] * a.strideG + (size_t)row * a.ldg;
+      for (int c = 0; c < a.d; c += kMoeChunk, ++count) {
+        const int stage = count % kMoeUpStages;
+        ok = mbar_wait_together(smem_u32(&empty[stage]), (count / kMoeUpStages & 1) ^ 1u, &abort_flag, kFaultWaitEmpty, 0x4d00u);
+        if (!ok) break;
+        moe_bring_rows(ring + stage * kStage + first * kMoeRowBytes, src + c, a.ldg, have, min(kMoeChunk, a.d - c) * 2,
+                       smem_u32(&full[stage]));
       }
+      unit.advance(plan, blocks);
     }
-    copies_commit();
-  };
-  start();
-  for (int i = 0; i + 1 < S::kSlots; ++i) fetch();
+  } else {
+    const int team = warp / kMoeTeam, member = warp % kMoeTeam;
+    // A lane's columns of a stage, asked for a turn ahead; columns past the last token repeat it, their sums are not used.
+    uint4 b[4];
+    MoeUnit ahead = unit;
+    int ahead_n = -1;
+    const T* x = nullptr;
+    auto ask = [&](int at) {
+      if (at >= units * chunks) return;
+      const bool moved = at >= (ahead_n + 1) * chunks;
+      while (at >= (ahead_n + 1) * chunks)
+        if (++ahead_n > 0) ahead.advance(plan, blocks);
+      if (moved) {
+        const int p0 = plan.start[ahead.index] + ahead.group * 8, cols = min(8, plan.start[ahead.index + 1] - p0);
+        x = static_cast<const T*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] >> 16) * a.d_pad + t * 8;
+      }
+      const int c = (at - ahead_n * chunks) * kMoeChunk;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = c + (i * kMoeTeam + member) * 32;
+        if (j < a.d) b[i] = *reinterpret_cast<const uint4*>(x + j);
+      }
+    };
+    ask(count = team);
+    for (int n = 0; n < units; ++n) {
+      const int p0 = plan.start[unit.index] + unit.group * 8, cols = min(8, plan.start[unit.index + 1] - p0);
+      float gate[4] = {0.f, 0.f, 0.f, 0.f}, up[4] = {0.f, 0.f, 0.f, 0.f};
+      for (; count < (n + 1) * chunks; count += kTeams) {
+        const int stage = count % kMoeUpStages, c = (count - n * chunks) * kMoeChunk, columns = min(kMoeChunk, a.d - c);
+        if (fed && ok)
+          ok = mbar_wait_together(smem_u32(&full[stage]), count / kMoeUpStages & 1, &abort_flag, kFaultWaitFull, 0x4d01u);
+        const uint32_t at = ring + stage * kStage;
+        const size_t off = plan.expert[unit.index] * a.strideG + (size_t)(unit.rows * 16 + r) * a.ldg;
+        const int lo = unit.rows * 16 + r < a.f ? a.d : 0, hi = unit.rows * 16 + r + 8 < a.f ? a.d : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = (i * kMoeTeam + member) * 32;
+          if (j < columns) {
+            uint4 g0, g1, u0, u1;
+            if (fed) {
+              g0 = moe_piece(at, r, j + t * 8, columns);
+              g1 = moe_piece(at, r + 8, j + t * 8, columns);
+              u0 = moe_piece(at, r + 16, j + t * 8, columns);
+              u1 = moe_piece(at, r + 24, j + t * 8, columns);
+            } else {
+              g0 = load8(static_cast<const T*>(a.gate) + off, lo, c + j + t * 8);
+              g1 = load8(static_cast<const T*>(a.gate) + off + 8 * a.ldg, hi, c + j + t * 8);
+              u0 = load8(static_cast<const T*>(a.up) + off, lo, c + j + t * 8);
+              u1 = load8(static_cast<const T*>(a.up) + off + 8 * a.ldg, hi, c + j + t * 8);
+            }
+            mma_16816<T>(gate, g0.x, g1.x, g0.y, g1.y, b[i].x, b[i].y);
+            mma_16816<T>(up, u0.x, u1.x, u0.y, u1.y, b[i].x, b[i].y);
+            mma_16816<T>(gate, g0.z, g1.z, g0.w, g1.w, b[i].z, b[i].w);
+            mma_16816<T>(up, u0.z, u1.z, u0.w, u1.w, b[i].z, b[i].w);
+          }
+        }
+        __syncwarp();
+        if (fed && lane == 0) mbar_arrive(smem_u32(&empty[stage]));
+        ask(count + kTeams);
+      }
+      // the team that had the unit's last stage finishes it
+      const uint32_t which = n & 1, parity = n >> 1 & 1;
+      float* ours = sums + which * kMoeWarps * 256;
+      if (ok) ok = mbar_wait_together(smem_u32(&sums_free[which]), parity ^ 1u, &abort_flag, kFaultWaitEmpty, 0x4d02u);
+      moe_keep_sums(ours + warp * 256, gate, up);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sums_full[which]));
+      if (((n + 1) * chunks - 1) % kTeams == team) {
+        if (ok) ok = mbar_wait_together(smem_u32(&sums_full[which]), parity, &abort_flag, kFaultWaitFull, 0x4d03u);
+        moe_finish_unit<T>(a, ours, kMoeWarps, member * 32 + lane, cols, unit.rows, plan.order + p0, false);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sums_free[which]));
+      }
+      unit.advance(plan, blocks);
+    }
+  }
+  if (!ok) {  // a wait ran out: give the copies still in flight time to land
+    const uint64_t since = global_timer_ns();
+    while (global_timer_ns() - since < MMBO_DRAIN_LIMIT_NS) __nanosleep(1000);
+  }
+}
 
-  uint32_t from = ring;
+// Packed weights.  Every warp fills a ring of its own: a slot holds up to kMoeTiles consecutive tiles of gate and as many of
+// up.  Teams of warps share units and cut d.
+constexpr int kMoeTiles = 2, kMoeSlots = 2;
+
+template <typename T, int QG>
+__global__ void __launch_bounds__(kMoeThreads, 1) moe_up4_kernel(const MoeArgs a) {
+  constexpr int G = 4 / QG;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) unsigned long long full_bars[kMoeWarps * kMoeSlots];
+  __shared__ uint32_t abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int pairs = a.tokens * a.topk;
+  const uint32_t tile_bytes = a.fmt.tile_bytes(), half = kMoeTiles * tile_bytes, slot_bytes = 2 * half;
+  // shared memory: rings | partial sums (before that: scores) | plan | ids | count
+  float* sums = reinterpret_cast<float*>(smem + kMoeWarps * kMoeSlots * slot_bytes);
+  int* at_plan = reinterpret_cast<int*>(sums) + kMoeUpSums / 4;
+  MoePlan plan(at_plan, a.experts, pairs);
+  int* ids = at_plan + MoePlan::words(a.experts, pairs);
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (threadIdx.x < kMoeWarps * kMoeSlots) mbar_init(smem_u32(&full_bars[threadIdx.x]), 1);
+  fence_mbar_init();
+  griddep_launch_dependents();
+  griddep_wait();
+  moe_make_plan(a, plan, ids, ids + pairs, sums);
+
+  const int WK = 1 << a.team_log2, wk = warp & (WK - 1), team = warp >> a.team_log2, teams = kMoeWarps >> a.team_log2;
+  const int blocks = (a.f + 15) / 16, total = MoeUnit::total(plan, blocks);
+  const long long share = (long long)gridDim.x * teams, mine = (long long)blockIdx.x * teams + team;
+  const int begin = (int)(total * mine / share), end = (int)(total * (mine + 1) / share);
+  MoeUnit unit;
+  unit.find(plan, blocks, begin);
+  const int steps = (a.d + 127) / 128, s0 = steps * wk >> a.team_log2, s1 = steps * (wk + 1) >> a.team_log2;
+  const uint32_t full = smem_u32(&full_bars[warp * kMoeSlots]), ring = smem_u32(smem) + warp * kMoeSlots * slot_bytes;
+  // what the ring is filled with next
+  MoeUnit ahead = unit;
+  int units_left = s0 < s1 ? end - begin : 0, at_step = s0;
+  const unsigned char *from_gate = nullptr, *from_up = nullptr;
+  auto fill = [&](int slot) {
+    if (units_left <= 0) return;
+    if (at_step == s0) {
+      const size_t off = plan.expert[ahead.index] * a.strideG + ((size_t)ahead.rows * steps + s0) * tile_bytes;
+      from_gate = static_cast<const unsigned char*>(a.gate) + off;
+      from_up = static_cast<const unsigned char*>(a.up) + off;
+    }
+    const uint32_t bytes = min(kMoeTiles, s1 - at_step) * tile_bytes;
+    if (elect_one()) {
+      const uint32_t bar = full + slot * 8, to = ring + slot * slot_bytes;
+      mbar_expect_tx(bar, 2 * bytes);
+      bulk_load(to, from_gate, bytes, bar);
+      bulk_load(to + half, from_up, bytes, bar);
+    }
+    __syncwarp();
+    from_gate += bytes;
+    from_up += bytes;
+    if ((at_step += kMoeTiles) >= s1) {
+      at_step = s0;
+      --units_left;
+      ahead.advance(plan, blocks);
+    }
+  };
+  for (int i = 0; i < kMoeSlots; ++i) fill(i);
+  bool ok = true;
+  int slot = 0;
+  uint32_t phase = 0;
+  const int per = a.d_pad / (32 * QG);
   for (int n = begin; n < end; ++n) {
     const int p0 = plan.start[unit.index] + unit.group * 8, cols = min(8, plan.start[unit.index + 1] - p0);
     // columns past the last token repeat it; their sums are not used
     const uint16_t* x = static_cast<const uint16_t*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] >> 16) * a.d_pad +
-                        s0 * S::kStep + t * 8;
-    const float *sums0 = nullptr, *sums1 = nullptr;
-    if constexpr (W4) {
-      const int per = a.d_pad / (32 * QG), at = s0 * (4 / QG);
-      sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] >> 16) * per + at;
-      sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] >> 16) * per + at;
-    }
-    float accg[4] = {0.f, 0.f, 0.f, 0.f}, accu[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s < s1; ++s) {
-      constexpr int kQuarters = S::kStep / 32;
-      uint4 b[kQuarters];
+                        s0 * 128 + t * 8;
+    const float* sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] >> 16) * per + s0 * G;
+    const float* sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] >> 16) * per + s0 * G;
+    float gate[4] = {0.f, 0.f, 0.f, 0.f}, up[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = s0; s < s1; s += kMoeTiles) {
+      const int cnt = min(kMoeTiles, s1 - s);
+      uint32_t at = ring + slot * slot_bytes;
+      for (int i = 0; i < cnt; ++i) {
+        uint4 b[4];
+        float2 xs[G];
 #pragma unroll
-      for (int q = 0; q < kQuarters; ++q) b[q] = *reinterpret_cast<const uint4*>(x + q * 32);
-      x += S::kStep;
-      float2 xs[W4 ? 4 / (QG ? QG : 1) : 1];
-      if constexpr (W4) {
+        for (int q = 0; q < 4; ++q) b[q] = *reinterpret_cast<const uint4*>(x + q * 32);
 #pragma unroll
-        for (int g = 0; g < 4 / QG; ++g) xs[g] = make_float2(*sums0++, *sums1++);
+        for (int g = 0; g < G; ++g) xs[g] = make_float2(*sums0++, *sums1++);
+        x += 128;
+        if (i == 0 && ok) ok = mbar_wait_together(full + slot * 8, phase, &abort_flag, kFaultWaitFull, 0x4d10u + warp);
+        w4_tile_mma<T, QG>(at, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, gate);
+        w4_tile_mma<T, QG>(at + half, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, up);
+        at += tile_bytes;
       }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        __syncwarp();
-        fetch();
-        copies_wait<S::kSlots - 1>();
-        if constexpr (W4) {
-          __syncwarp();
-          w4_tile_mma<T, QG>(from, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, half ? accu : accg);
-        } else {
-          rows16_multiply<T, 2>(from, half ? accu : accg, b);
-        }
-        from += S::kSlot;
-        if (from == ring + S::kSlots * S::kSlot) from = ring;
+      __syncwarp();
+      fill(slot);
+      if (++slot == kMoeSlots) {
+        slot = 0;
+        phase ^= 1u;
       }
     }
-    // [turn][warp][gate, up][column][row]
     float* ours = sums + ((n & 1) * kMoeWarps + (team << a.team_log2)) * 256;
-    float* mine_sums = ours + wk * 256;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = (t * 2 + (i & 1)) * 16 + r + 8 * (i >> 1);
-      mine_sums[at] = accg[i];
-      mine_sums[128 + at] = accu[i];
-    }
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(WK * 32) : "memory");
-    // finished by four warps, with larger teams others' turn with every unit
-    const int i = (wk * 32 + lane + 384 * (n & 3)) & (WK * 32 - 1);
-    if (i < cols * 16) {
-      const float* p = ours + i;
-      float g = 0.f, u = 0.f;
-      for (int w = 0; w < WK; w += 4) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          g += p[(w + v) * 256];
-          u += p[(w + v) * 256 + 128];
-        }
-      }
-      const int row = unit.rows * 16 + (i & 15), entry = plan.order[p0 + i / 16], pair = entry & 0xffff;
-      if (W4) {
-        const float2 undo = a.x_undo[entry >> 16];
-        g *= undo.x * undo.y;
-        u *= undo.x * undo.y;
-      }
-      const float h = row < a.f ? g / (1.f + expf(-g)) * u : 0.f;
-      using U = typename std::conditional<W4, __nv_bfloat16, T>::type;  // type of the products with down
-      U* out = static_cast<U*>(a.hidden) + (size_t)pair * 2 * a.f_pad + row;
-      const float scaled = h * MoeHidden<U>::kScale;
-      const U v = from_f32<U>(scaled);
-      const float rest = (scaled - to_f32(v)) * MoeHidden<U>::kRest;
-      out[0] = v;
-      out[a.f_pad] = from_f32<U>(isfinite(rest) ? rest : 0.f);
-    }
-    if (n + 1 < end) advance(unit);
+    moe_keep_sums(ours + wk * 256, gate, up);
+    asm volatile("bar.sync %0, %1;" ::"r"(2 + team), "r"(WK * 32) : "memory");
+    moe_finish_unit<__nv_bfloat16>(a, ours, WK, (wk * 32 + lane + 384 * (n & 3)) & (WK * 32 - 1), cols, unit.rows,
+                                   plan.order + p0, true);
+    unit.advance(plan, blocks);
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!ok) {  // a wait ran out: give the copies still in flight time to land
+    const uint64_t since = global_timer_ns();
+    while (global_timer_ns() - since < MMBO_DRAIN_LIMIT_NS) __nanosleep(1000);
+  }
 }
 
 // ---------------------------------------------------------------- down ----------------
-template <int QG>
-struct MoeDownShape {
-  static constexpr int kStep = QG ? 128 : 64;
-  static constexpr uint32_t kSlot = QG ? kTileRoom : 2048;
-  static constexpr int kSlots = QG ? 6 : 4;
-};
+// Adds an expert's products with the tokens of a group, times their gates, to this warp's sums, [token][row].
+template <typename U>
+__device__ __forceinline__ void moe_add_products(const MoePlan& plan, float* sums, const int* order, int cols, const float (&acc)[4],
+                                                 const float (&rest)[4]) {
+  const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int col = t * 2 + (i & 1);
+    if (col < cols) {
+      const int entry = order[col];
+      const float v = (acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest)) * (1.f / MoeHidden<U>::kScale);
+      sums[(entry >> 16) * 16 + r + 8 * (i >> 1)] += plan.gate[entry & 0xffff] * v;
+    }
+  }
+  __syncwarp();
+}
+// Joins the warps' sums, stores 16 rows of the output and clears the sums; by the multiplying warps.
+template <typename T>
+__device__ __forceinline__ void moe_store_rows(const MoeArgs& a, float* sums, int rows) {
+  workers_sync();
+  for (int i = threadIdx.x; i < a.tokens * 16; i += kMoeThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMoeWarps; ++w) {
+      float* p = sums + w * a.tokens * 16 + i;
+      v += *p;
+      *p = 0.f;
+    }
+    const int row = rows * 16 + (i & 15);
+    if (row < a.d) {
+      T* y = static_cast<T*>(a.Y) + (size_t)(i / 16) * a.ldy + row;
+      *y = from_f32<T>(a.beta != 0.f ? fmaf(a.beta, to_f32(*y), v) : v);
+    }
+  }
+  workers_sync();
+}
 
-template <typename T, int QG>
-__global__ void __launch_bounds__(kMoeThreads, 1) moe_down_kernel(const MoeArgs a) {
-  using S = MoeDownShape<QG>;
-  constexpr bool W4 = QG > 0;
-  using U = typename std::conditional<W4, __nv_bfloat16, T>::type;  // type of the products
+// 16-bit weights: stages of 512 columns of the block's 16 rows, expert after expert; teams of four warps take
+// them in turn.
+template <typename T>
+__global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_down16_kernel(const MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) unsigned long long full[kMoeDownStages], empty[kMoeDownStages];
+  __shared__ uint32_t abort_flag;
+  constexpr uint32_t kStage = 16 * kMoeRowBytes;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int pairs = a.tokens * a.topk, words = MoePlan::words(a.experts, pairs);
-  const uint32_t ring = smem_u32(smem) + warp * S::kSlots * S::kSlot;
-  float* sums = reinterpret_cast<float*>(smem + kMoeWarps * S::kSlots * S::kSlot);  // [warp][token][row]
+  const uint32_t ring = smem_u32(smem);
+  float* sums = reinterpret_cast<float*>(smem + kMoeDownStages * kStage);  // [warp][token][row]
   int* at_plan = reinterpret_cast<int*>(sums + kMoeWarps * a.tokens * 16);
   MoePlan plan(at_plan, a.experts, pairs);
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kMoeDownStages; ++i) {
+      mbar_init(smem_u32(&full[i]), kMoeFeeders);
+      mbar_init(smem_u32(&empty[i]), kMoeTeam);
+    }
+  }
+  fence_mbar_init();
+  for (int i = threadIdx.x; i < kMoeWarps * a.tokens * 16; i += kMoeFed16Threads) sums[i] = 0.f;
+  griddep_launch_dependents();
+  griddep_wait();
+  for (int i = threadIdx.x; i < words; i += kMoeFed16Threads) at_plan[i] = a.plan[i];
+  __syncthreads();
+
+  const int active = *plan.active, row_blocks = (a.d + 15) / 16;
+  const bool fed = a.ldd % 8 == 0 && a.strideD % 8 == 0 && a.f % 8 == 0 && (reinterpret_cast<uintptr_t>(a.down) & 15u) == 0;
+  const int chunks = (a.f + kMoeChunk - 1) / kMoeChunk, row_stages = MoeUnit::total(plan, chunks);
+  constexpr int kTeams = kMoeWarps / kMoeTeam;
+  bool ok = true;
+  int count = 0;  // of stages
+  if (warp >= kMoeWarps) {
+    constexpr int kRows = 16 / kMoeFeeders;
+    const int first = (warp - kMoeWarps) * kRows;  // of the stage's rows, those that this warp brings
+    for (int rows = blockIdx.x; fed && ok && rows < row_blocks; rows += gridDim.x) {
+      const int row = rows * 16 + first, have = min(kRows, max(a.d - row, 0));
+      for (int i = 0; ok && i < active; ++i) {
+        const T* src = static_cast<const T*>(a.down) + plan.expert[i] * a.strideD + (size_t)row * a.ldd;
+        for (int g = plan.base[i]; ok && g < plan.base[i + 1]; ++g)
+          for (int c = 0; c < a.f; c += kMoeChunk, ++count) {
+            const int stage = count % kMoeDownStages;
+            ok = mbar_wait_together(smem_u32(&empty[stage]), (count / kMoeDownStages & 1) ^ 1u, &abort_flag, kFaultWaitEmpty,
+                                    0x4d20u);
+            if (!ok) break;
+            moe_bring_rows(ring + stage * kStage + first * kMoeRowBytes, src + c, a.ldd, have, min(kMoeChunk, a.f - c) * 2,
+                           smem_u32(&full[stage]));
+          }
+      }
+    }
+  } else {
+    const int team = warp / kMoeTeam, member = warp % kMoeTeam;
+    float* ours = sums + warp * a.tokens * 16;
+    // The stage that is next, as expert, pairs and first column; a lane's columns of it are asked for a turn ahead.
+    int e = 0, p0 = plan.start[0], c = 0;
+    uint4 b[4][2];
+    auto move = [&](int by) {
+      for (; by > 0; --by) {
+        if ((c += kMoeChunk) < a.f) continue;
+        c = 0;
+        if ((p0 += 8) < plan.start[e + 1]) continue;
+        if (++e == active) e = 0;
+        p0 = plan.start[e];
+      }
+    };
+    auto ask = [&] {
+      // columns past the last token repeat it; their sums are not used
+      const T* h = static_cast<const T*>(a.hidden) +
+                   (size_t)(plan.order[min(p0 + r, plan.start[e + 1] - 1)] & 0xffff) * 2 * a.f_pad + t * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = c + (i * kMoeTeam + member) * 32;
+        if (j < a.f) {
+          b[i][0] = *reinterpret_cast<const uint4*>(h + j);
+          b[i][1] = *reinterpret_cast<const uint4*>(h + a.f_pad + j);
+        }
+      }
+    };
+    move(count = team);
+    ask();
+    for (int rows = blockIdx.x, until = row_stages; rows < row_blocks; rows += gridDim.x, until += row_stages) {
+      const int lo = rows * 16 + r < a.d ? a.f : 0, hi = rows * 16 + r + 8 < a.d ? a.f : 0;
+      for (; count < until; count += kTeams) {
+        const int stage = count % kMoeDownStages, columns = min(kMoeChunk, a.f - c), cols = min(8, plan.start[e + 1] - p0);
+        const T* w = static_cast<const T*>(a.down) + plan.expert[e] * a.strideD + (size_t)(rows * 16 + r) * a.ldd + c;
+        const int* order = plan.order + p0;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f}, rest[4] = {0.f, 0.f, 0.f, 0.f};
+        if (fed && ok)
+          ok = mbar_wait_together(smem_u32(&full[stage]), count / kMoeDownStages & 1, &abort_flag, kFaultWaitFull, 0x4d21u);
+        const uint32_t at = ring + stage * kStage;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = (i * kMoeTeam + member) * 32;
+          if (j < columns) {
+            uint4 w0, w1;
+            if (fed) {
+              w0 = moe_piece(at, r, j + t * 8, columns);
+              w1 = moe_piece(at, r + 8, j + t * 8, columns);
+            } else {
+              w0 = load8(w, lo - c, j + t * 8);
+              w1 = load8(w + 8 * a.ldd, hi - c, j + t * 8);
+            }
+            mma_16816<T>(acc, w0.x, w1.x, w0.y, w1.y, b[i][0].x, b[i][0].y);
+            mma_16816<T>(rest, w0.x, w1.x, w0.y, w1.y, b[i][1].x, b[i][1].y);
+            mma_16816<T>(acc, w0.z, w1.z, w0.w, w1.w, b[i][0].z, b[i][0].w);
+            mma_16816<T>(rest, w0.z, w1.z, w0.w, w1.w, b[i][1].z, b[i][1].w);
+          }
+        }
+        __syncwarp();
+        if (fed && lane == 0) mbar_arrive(smem_u32(&empty[stage]));
+        move(kTeams);
+        ask();
+        moe_add_products<T>(plan, ours, order, cols, acc, rest);
+      }
+      moe_store_rows<T>(a, sums, rows);
+    }
+  }
+  if (!ok) {  // a wait ran out: give the copies still in flight time to land
+    const uint64_t since = global_timer_ns();
+    while (global_timer_ns() - since < MMBO_DRAIN_LIMIT_NS) __nanosleep(1000);
+  }
+}
+
+// Packed weights: the warps cut the list of (expert, group of tokens, tile) into equal parts and fill rings
+// of their own.
+constexpr int kMoeDownTiles = 3;
+
+template <typename T, int QG>
+__global__ void __launch_bounds__(kMoeThreads, 1) moe_down4_kernel(const MoeArgs a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) unsigned long long full_bars[kMoeWarps * kMoeSlots];
+  __shared__ uint32_t abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  const int pairs = a.tokens * a.topk, words = MoePlan::words(a.experts, pairs);
+  const uint32_t tile_bytes = a.fmt.tile_bytes(), slot_bytes = kMoeDownTiles * tile_bytes;
+  float* sums = reinterpret_cast<float*>(smem + kMoeWarps * kMoeSlots * slot_bytes);  // [warp][token][row]
+  int* at_plan = reinterpret_cast<int*>(sums + kMoeWarps * a.tokens * 16);
+  MoePlan plan(at_plan, a.experts, pairs);
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (threadIdx.x < kMoeWarps * kMoeSlots) mbar_init(smem_u32(&full_bars[threadIdx.x]), 1);
+  fence_mbar_init();
+  for (int i = threadIdx.x; i < kMoeWarps * a.tokens * 16; i += kMoeThreads) sums[i] = 0.f;
   griddep_launch_dependents();
   griddep_wait();
   for (int i = threadIdx.x; i < words; i += kMoeThreads) at_plan[i] = a.plan[i];
-  for (int i = threadIdx.x; i < kMoeWarps * a.tokens * 16; i += kMoeThreads) sums[i] = 0.f;
   __syncthreads();
-  const int active = *plan.active;
 
-  const int steps = (a.f + S::kStep - 1) / S::kStep;
-  int total = 0;
-  for (int i = 0; i < active; ++i) total += (plan.start[i + 1] - plan.start[i] + 7) / 8;
-  const long long all = (long long)total * steps;
-  const int row_blocks = (a.d + 15) / 16;
+  const int steps = (a.f + 127) / 128, row_blocks = (a.d + 15) / 16;
+  const long long all = (long long)MoeUnit::total(plan, 1) * steps;
   const long long w0 = all * warp / kMoeWarps, w1 = all * (warp + 1) / kMoeWarps;
-  const bool vec = !W4 && a.ldd % 8 == 0 && a.strideD % 8 == 0 && a.f % 8 == 0 &&
-                   (reinterpret_cast<uintptr_t>(a.down) & 15u) == 0;
-  const uint32_t tile_bytes = W4 ? a.fmt.tile_bytes() : 0;
-  // a run: what of this warp's part belongs to one expert and group of tokens
-  struct Run {
-    int index, group, groups, step;
-  };
-  Run first{0, 0, 0, 0};
-  {
-    long long at = 0;
-    for (; first.index < active; ++first.index) {
-      first.groups = (plan.start[first.index + 1] - plan.start[first.index] + 7) / 8;
-      if (w0 < at + (long long)first.groups * steps) {
-        first.group = (int)((w0 - at) / steps);
-        first.step = (int)((w0 - at) % steps);
-        break;
-      }
-      at += (long long)first.groups * steps;
+  // a run: what of a warp's part belongs to one expert and group of tokens
+  MoeUnit first;
+  first.find(plan, 1, (int)(w0 / steps));
+  const int first_step = (int)(w0 % steps);
+  const uint32_t full = smem_u32(&full_bars[warp * kMoeSlots]), ring = smem_u32(smem) + warp * kMoeSlots * slot_bytes;
+  // what the ring is filled with next
+  MoeUnit ahead = first;
+  int at_rows = blockIdx.x, at_step = first_step;
+  long long at = w0;
+  auto fill = [&](int slot) {
+    if (at_rows >= row_blocks || w0 == w1) return;
+    const int cnt = (int)min((long long)min(kMoeDownTiles, steps - at_step), w1 - at);
+    const uint32_t bytes = cnt * tile_bytes;
+    const unsigned char* src = static_cast<const unsigned char*>(a.down) + plan.expert[ahead.index] * a.strideD +
+                               ((size_t)at_rows * steps + at_step) * tile_bytes;
+    if (elect_one()) {
+      mbar_expect_tx(full + slot * 8, bytes);
+      bulk_load(ring + slot * slot_bytes, src, bytes, full + slot * 8);
     }
-  }
-  auto advance = [&](Run& p) {
-    p.step = 0;
-    if (++p.group < p.groups) return;
-    p.group = 0;
-    if (++p.index < active) p.groups = (plan.start[p.index + 1] - plan.start[p.index] + 7) / 8;
-  };
-  // the copies run ahead of the products, through the same order, on into the next row block
-  using Feed = typename std::conditional<W4, TileFeed, RowsFeed<T, 2>>::type;
-  Feed feed;
-  Run ahead = first;
-  int ahead_rows = w0 < w1 ? blockIdx.x : row_blocks, ahead_left = 0;
-  long long ahead_n = w0;
-  uint32_t ahead_at = ring;
-  auto start = [&]() {
-    if (ahead_rows >= row_blocks) return;
-    const size_t e = plan.expert[ahead.index];
-    ahead_left = (int)min((long long)(steps - ahead.step), w1 - ahead_n);
-    if constexpr (W4)
-      feed.start(static_cast<const unsigned char*>(a.down) + e * a.strideD + ((size_t)ahead_rows * steps + ahead.step) * tile_bytes,
-                 tile_bytes, 0);
-    else
-      feed.start(static_cast<const T*>(a.down) + e * a.strideD + (size_t)ahead_rows * 16 * a.ldd, a.ldd, a.d - ahead_rows * 16,
-                 a.f, ahead.step, vec);
-    ahead_n += ahead_left;
-  };
-  auto fetch = [&]() {
-    if (ahead_rows < row_blocks) {
-      feed.fetch(ahead_at);
-      ahead_at += S::kSlot;
-      if (ahead_at == ring + S::kSlots * S::kSlot) ahead_at = ring;
-      if (--ahead_left == 0) {
-        if (ahead_n == w1) {
-          ahead_n = w0;
-          ahead = first;
-          ahead_rows += gridDim.x;
-        } else {
-          advance(ahead);
-        }
-        start();
-      }
+    __syncwarp();
+    at += cnt;
+    if ((at_step += cnt) == steps) {
+      at_step = 0;
+      ahead.advance(plan, 1);
     }
-    copies_commit();
+    if (at == w1) {
+      at = w0;
+      at_step = first_step;
+      ahead = first;
+      at_rows += gridDim.x;
+    }
   };
-  start();
-  for (int i = 0; i + 1 < S::kSlots; ++i) fetch();
-
-  uint32_t from = ring;
+  for (int i = 0; i < kMoeSlots; ++i) fill(i);
+  bool ok = true;
+  int slot = 0;
+  uint32_t phase = 0;
+  float* ours = sums + warp * a.tokens * 16;
   for (int rows = blockIdx.x; rows < row_blocks; rows += gridDim.x) {
-    Run run = first;
-    for (long long n = w0; n < w1; advance(run)) {
-      const int p0 = plan.start[run.index] + run.group * 8, cols = min(8, plan.start[run.index + 1] - p0);
-      const int length = (int)min((long long)(steps - run.step), w1 - n);
+    MoeUnit run = first;
+    int step = first_step;
+    for (long long n = w0; n < w1; run.advance(plan, 1), step = 0) {
+      const int length = (int)min((long long)(steps - step), w1 - n);
       n += length;
-      const uint16_t* h = static_cast<const uint16_t*>(a.hidden) + (size_t)(plan.order[p0 + min(r, cols - 1)] & 0xffff) * 2 * a.f_pad +
-                          run.step * S::kStep + t * 8;
-      float acc[4] = {0.f, 0.f, 0.f, 0.f}, rest[4] = {0.f, 0.f, 0.f, 0.f};
-      constexpr int kQuarters = S::kStep / 32;
-      uint4 b[2][kQuarters], ahead_b[2][kQuarters];
-      auto columns = [&](uint4(&to)[2][kQuarters]) {
+      const int p0 = plan.start[run.index] + run.group * 8, cols = min(8, plan.start[run.index + 1] - p0);
+      const __nv_bfloat16* h = static_cast<const __nv_bfloat16*>(a.hidden) +
+                               (size_t)(plan.order[p0 + min(r, cols - 1)] & 0xffff) * 2 * a.f_pad + step * 128 + t * 8;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      const float none[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < length; s += kMoeDownTiles) {
+        const int cnt = min(kMoeDownTiles, length - s);
+        uint32_t tile = ring + slot * slot_bytes;
+        for (int i = 0; i < cnt; ++i) {
+          uint4 b[2][4];
 #pragma unroll
-        for (int q = 0; q < kQuarters; ++q) {
-          to[0][q] = *reinterpret_cast<const uint4*>(h + q * 32);
-          to[1][q] = *reinterpret_cast<const uint4*>(h + a.f_pad + q * 32);
-        }
-        h += S::kStep;
-      };
-      if (!W4) columns(ahead_b);
-      for (int i = 0; i < length; ++i) {
-        // 16-bit weights: the columns of the next step, too (packed ones leave no registers for it)
-        if (W4) {
-          columns(b);
-        } else {
-#pragma unroll
-          for (int q = 0; q < kQuarters; ++q) {
-            b[0][q] = ahead_b[0][q];
-            b[1][q] = ahead_b[1][q];
+          for (int q = 0; q < 4; ++q) {
+            b[0][q] = *reinterpret_cast<const uint4*>(h + q * 32);
+            b[1][q] = *reinterpret_cast<const uint4*>(h + a.f_pad + q * 32);
           }
-          if (i + 1 < length) columns(ahead_b);
+          h += 128;
+          if (i == 0 && ok) ok = mbar_wait_together(full + slot * 8, phase, &abort_flag, kFaultWaitFull, 0x4d30u + warp);
+          tile_multiply_bf16<T, QG>(tile, b, a.fmt.zeros, acc);
+          tile += tile_bytes;
         }
         __syncwarp();
-        fetch();
-        copies_wait<S::kSlots - 1>();
-        if constexpr (W4) {
-          __syncwarp();
-          tile_multiply_bf16<T, QG>(from, b, a.fmt.zeros, acc);
-        } else {
-          rows16_multiply<T, 2>(from, acc, b[0]);
-          rows16_multiply<T, 2>(from, rest, b[1]);
-        }
-        from += S::kSlot;
-        if (from == ring + S::kSlots * S::kSlot) from = ring;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = t * 2 + (i & 1);
-        if (col < cols) {
-          const int entry = plan.order[p0 + col];
-          const float v = (acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest)) * (1.f / MoeHidden<U>::kScale);
-          sums[(warp * a.tokens + (entry >> 16)) * 16 + r + 8 * (i >> 1)] += plan.gate[entry & 0xffff] * v;
+        fill(slot);
+        if (++slot == kMoeSlots) {
+          slot = 0;
+          phase ^= 1u;
         }
       }
-      __syncwarp();
+      moe_add_products<__nv_bfloat16>(plan, ours, plan.order + p0, cols, acc, none);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.tokens * 16; i += kMoeThreads) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kMoeWarps; ++w) {
-        float* p = sums + w * a.tokens * 16 + i;
-        v += *p;
-        *p = 0.f;
-      }
-      const int row = rows * 16 + (i & 15);
-      if (row < a.d) {
-        T* y = static_cast<T*>(a.Y) + (size_t)(i / 16) * a.ldy + row;
-        *y = from_f32<T>(a.beta != 0.f ? fmaf(a.beta, to_f32(*y), v) : v);
-      }
-    }
-    __syncthreads();
+    moe_store_rows<T>(a, sums, rows);
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!ok) {  // a wait ran out: give the copies still in flight time to land
+    const uint64_t since = global_timer_ns();
+    while (global_timer_ns() - since < MMBO_DRAIN_LIMIT_NS) __nanosleep(1000);
+  }
 }
 
 }  // namespace mmbo
