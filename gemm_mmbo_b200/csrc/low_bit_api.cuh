@@ -294,12 +294,14 @@ static int launch_moe(const MoeArgs& args, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = settings().pdl ? 1 : 0;
-  static bool up_ready[kMaxDevices], down_ready[kMaxDevices];
+  static bool up_ready[2][kMaxDevices], down_ready[2][kMaxDevices];
   int rc;
   if constexpr (QG == 0) {
-    auto up = moe_up16_kernel<T>;
-    auto down = moe_down16_kernel<T>;
-    if ((rc = allow_smem(up, kGemvSmem, up_ready)) || (rc = allow_smem(down, kGemvSmem, down_ready))) return rc;
+    const bool up_fed = a.ldg % 8 == 0 && a.strideG % 8 == 0 && a.d % 8 == 0 && aligned16(a.gate) && aligned16(a.up);
+    const bool down_fed = a.ldd % 8 == 0 && a.strideD % 8 == 0 && a.f % 8 == 0 && aligned16(a.down);
+    auto up = up_fed ? moe_up16_kernel<T, true> : moe_up16_kernel<T, false>;
+    auto down = down_fed ? moe_down16_kernel<T, true> : moe_down16_kernel<T, false>;
+    if ((rc = allow_smem(up, kGemvSmem, up_ready[up_fed])) || (rc = allow_smem(down, kGemvSmem, down_ready[down_fed]))) return rc;
     const size_t up_smem = kMoeUpStages * (size_t)(32 * kMoeRowBytes) + up_rest;
     const size_t down_smem = kMoeDownStages * (size_t)(16 * kMoeRowBytes) + down_rest;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, moe_scores_kernel<T>, a);
@@ -311,7 +313,7 @@ static int launch_moe(const MoeArgs& args, cudaStream_t st) {
   } else {
     auto up = moe_up4_kernel<T, QG>;
     auto down = moe_down4_kernel<T, QG>;
-    if ((rc = allow_smem(up, kGemvSmem, up_ready)) || (rc = allow_smem(down, kGemvSmem, down_ready))) return rc;
+    if ((rc = allow_smem(up, kGemvSmem, up_ready[0])) || (rc = allow_smem(down, kGemvSmem, down_ready[0]))) return rc;
     // teams of `up`: small ones (fewer sums to join, fewer barriers) as long as every team has a unit
     const size_t experts = pairs < (size_t)a.experts ? pairs : (size_t)a.experts, units = experts * ((a.f + 15) / 16);
     a.team_log2 = 4;

@@ -441,12 +441,27 @@ __device__ __forceinline__ void moe_bring_rows(uint32_t to, const T* src, size_t
   __syncwarp();
 }
 
+// A lane's quarters of a stage, f(which of the team's four, its first column): all of them, without a branch, when the stage
+// is whole.
+template <typename F>
+__device__ __forceinline__ void moe_quarters(int member, int columns, F f) {
+  if (columns >= kMoeChunk) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f(i, (i * kMoeTeam + member) * 32, std::true_type());
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if ((i * kMoeTeam + member) * 32 < columns) f(i, (i * kMoeTeam + member) * 32, std::false_type());
+  }
+}
 // Sixteen bytes of a lane's row in a stage; zeros where the row ends before them.
+template <bool WHOLE>
 __device__ __forceinline__ uint4 moe_piece(uint32_t stage, int row, int column, int columns) {
-  return column < columns ? lds128(stage + row * kMoeRowBytes + column * 2) : make_uint4(0, 0, 0, 0);
+  return WHOLE || column < columns ? lds128(stage + row * kMoeRowBytes + column * 2) : make_uint4(0, 0, 0, 0);
 }
 
-template <typename T>
+// FED: rows that bulk copies can address; others are read by the multiplying warps themselves.
+template <typename T, bool FED>
 __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) unsigned long long full[kMoeUpStages], empty[kMoeUpStages], sums_full[2], sums_free[2];
@@ -480,9 +495,6 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const Moe
   const int begin = (int)((long long)total * blockIdx.x / gridDim.x), end = (int)((long long)total * (blockIdx.x + 1) / gridDim.x);
   MoeUnit unit;
   unit.find(plan, blocks, begin);
-  // rows that bulk copies can address; others are read by the multiplying warps themselves
-  const bool fed = a.ldg % 8 == 0 && a.strideG % 8 == 0 && a.d % 8 == 0 &&
-                   ((reinterpret_cast<uintptr_t>(a.gate) | reinterpret_cast<uintptr_t>(a.up)) & 15u) == 0;
   const int chunks = (a.d + kMoeChunk - 1) / kMoeChunk, units = end - begin;
   constexpr int kTeams = kMoeWarps / kMoeTeam;
   bool ok = true;
@@ -490,7 +502,7 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const Moe
   if (warp >= kMoeWarps) {
     constexpr int kRows = 32 / kMoeFeeders;
     const int first = (warp - kMoeWarps) * kRows;  // of the stage's rows, those that this warp brings
-    for (int n = 0; fed && ok && n < units; ++n) {
+    for (int n = 0; FED && ok && n < units; ++n) {
       const int row = unit.rows * 16 + (first & 15), have = min(kRows, max(a.f - row, 0));
       const T* src = static_cast<const T*>(first < 16 ? a.gate : a.up) + plan.expert[unit.index] * a.strideG + (size_t)row * a.ldg;
       for (int c = 0; c < a.d; c += kMoeChunk, ++count) {
@@ -519,11 +531,7 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const Moe
         x = static_cast<const T*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] >> 16) * a.d_pad + t * 8;
       }
       const int c = (at - ahead_n * chunks) * kMoeChunk;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = c + (i * kMoeTeam + member) * 32;
-        if (j < a.d) b[i] = *reinterpret_cast<const uint4*>(x + j);
-      }
+      moe_quarters(member, a.d - c, [&](int i, int j, auto) { b[i] = *reinterpret_cast<const uint4*>(x + c + j); });
     };
     ask(count = team);
     for (int n = 0; n < units; ++n) {
@@ -531,35 +539,32 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const Moe
       float gate[4] = {0.f, 0.f, 0.f, 0.f}, up[4] = {0.f, 0.f, 0.f, 0.f};
       for (; count < (n + 1) * chunks; count += kTeams) {
         const int stage = count % kMoeUpStages, c = (count - n * chunks) * kMoeChunk, columns = min(kMoeChunk, a.d - c);
-        if (fed && ok)
+        if (FED && ok)
           ok = mbar_wait_together(smem_u32(&full[stage]), count / kMoeUpStages & 1, &abort_flag, kFaultWaitFull, 0x4d01u);
         const uint32_t at = ring + stage * kStage;
         const size_t off = plan.expert[unit.index] * a.strideG + (size_t)(unit.rows * 16 + r) * a.ldg;
         const int lo = unit.rows * 16 + r < a.f ? a.d : 0, hi = unit.rows * 16 + r + 8 < a.f ? a.d : 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = (i * kMoeTeam + member) * 32;
-          if (j < columns) {
-            uint4 g0, g1, u0, u1;
-            if (fed) {
-              g0 = moe_piece(at, r, j + t * 8, columns);
-              g1 = moe_piece(at, r + 8, j + t * 8, columns);
-              u0 = moe_piece(at, r + 16, j + t * 8, columns);
-              u1 = moe_piece(at, r + 24, j + t * 8, columns);
-            } else {
-              g0 = load8(static_cast<const T*>(a.gate) + off, lo, c + j + t * 8);
-              g1 = load8(static_cast<const T*>(a.gate) + off + 8 * a.ldg, hi, c + j + t * 8);
-              u0 = load8(static_cast<const T*>(a.up) + off, lo, c + j + t * 8);
-              u1 = load8(static_cast<const T*>(a.up) + off + 8 * a.ldg, hi, c + j + t * 8);
-            }
-            mma_16816<T>(gate, g0.x, g1.x, g0.y, g1.y, b[i].x, b[i].y);
-            mma_16816<T>(up, u0.x, u1.x, u0.y, u1.y, b[i].x, b[i].y);
-            mma_16816<T>(gate, g0.z, g1.z, g0.w, g1.w, b[i].z, b[i].w);
-            mma_16816<T>(up, u0.z, u1.z, u0.w, u1.w, b[i].z, b[i].w);
+        moe_quarters(member, columns, [&](int i, int j, auto whole) {
+          uint4 g0, g1, u0, u1;
+          if (FED) {
+            constexpr bool kWhole = decltype(whole)::value;
+            g0 = moe_piece<kWhole>(at, r, j + t * 8, columns);
+            g1 = moe_piece<kWhole>(at, r + 8, j + t * 8, columns);
+            u0 = moe_piece<kWhole>(at, r + 16, j + t * 8, columns);
+            u1 = moe_piece<kWhole>(at, r + 24, j + t * 8, columns);
+          } else {
+            g0 = load8(static_cast<const T*>(a.gate) + off, lo, c + j + t * 8);
+            g1 = load8(static_cast<const T*>(a.gate) + off + 8 * a.ldg, hi, c + j + t * 8);
+            u0 = load8(static_cast<const T*>(a.up) + off, lo, c + j + t * 8);
+            u1 = load8(static_cast<const T*>(a.up) + off + 8 * a.ldg, hi, c + j + t * 8);
           }
-        }
+          mma_16816<T>(gate, g0.x, g1.x, g0.y, g1.y, b[i].x, b[i].y);
+          mma_16816<T>(up, u0.x, u1.x, u0.y, u1.y, b[i].x, b[i].y);
+          mma_16816<T>(gate, g0.z, g1.z, g0.w, g1.w, b[i].z, b[i].w);
+          mma_16816<T>(up, u0.z, u1.z, u0.w, u1.w, b[i].z, b[i].w);
+        });
         __syncwarp();
-        if (fed && lane == 0) mbar_arrive(smem_u32(&empty[stage]));
+        if (FED && lane == 0) mbar_arrive(smem_u32(&empty[stage]));
         ask(count + kTeams);
       }
       // the team that had the unit's last stage finishes it
@@ -699,15 +704,16 @@ template <typename U>
 __device__ __forceinline__ void moe_add_products(const MoePlan& plan, float* sums, const int* order, int cols, const float (&acc)[4],
                                                  const float (&rest)[4]) {
   const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+  float v[4], *to[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int col = t * 2 + (i & 1);
-    if (col < cols) {
-      const int entry = order[col];
-      const float v = (acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest)) * (1.f / MoeHidden<U>::kScale);
-      sums[(entry >> 16) * 16 + r + 8 * (i >> 1)] += plan.gate[entry & 0xffff] * v;
-    }
+  for (int i = 0; i < 4; ++i) {  // all read before one is written: a lane's four are different ones
+    const int entry = order[min(t * 2 + (i & 1), cols - 1)];
+    to[i] = sums + (entry >> 16) * 16 + r + 8 * (i >> 1);
+    v[i] = fmaf(plan.gate[entry & 0xffff], (acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest)) * (1.f / MoeHidden<U>::kScale), *to[i]);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (t * 2 + (i & 1) < cols) *to[i] = v[i];
   __syncwarp();
 }
 // Joins the warps' sums, stores 16 rows of the output and clears the sums; by the multiplying warps.
@@ -733,7 +739,7 @@ __device__ __forceinline__ void moe_store_rows(const MoeArgs& a, float* sums, in
 
 // 16-bit weights: stages of 512 columns of the block's 16 rows, expert after expert; teams of four warps take
 // them in turn.
-template <typename T>
+template <typename T, bool FED>
 __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_down16_kernel(const MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) unsigned long long full[kMoeDownStages], empty[kMoeDownStages];
@@ -760,7 +766,6 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_down16_kernel(const M
   __syncthreads();
 
   const int active = *plan.active, row_blocks = (a.d + 15) / 16;
-  const bool fed = a.ldd % 8 == 0 && a.strideD % 8 == 0 && a.f % 8 == 0 && (reinterpret_cast<uintptr_t>(a.down) & 15u) == 0;
   const int chunks = (a.f + kMoeChunk - 1) / kMoeChunk, row_stages = MoeUnit::total(plan, chunks);
   constexpr int kTeams = kMoeWarps / kMoeTeam;
   bool ok = true;
@@ -768,7 +773,7 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_down16_kernel(const M
   if (warp >= kMoeWarps) {
     constexpr int kRows = 16 / kMoeFeeders;
     const int first = (warp - kMoeWarps) * kRows;  // of the stage's rows, those that this warp brings
-    for (int rows = blockIdx.x; fed && ok && rows < row_blocks; rows += gridDim.x) {
+    for (int rows = blockIdx.x; FED && ok && rows < row_blocks; rows += gridDim.x) {
       const int row = rows * 16 + first, have = min(kRows, max(a.d - row, 0));
       for (int i = 0; ok && i < active; ++i) {
         const T* src = static_cast<const T*>(a.down) + plan.expert[i] * a.strideD + (size_t)row * a.ldd;
@@ -786,13 +791,12 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_down16_kernel(const M
   } else {
     const int team = warp / kMoeTeam, member = warp % kMoeTeam;
     float* ours = sums + warp * a.tokens * 16;
-    // The stage that is next, as expert, pairs and first column; a lane's columns of it are asked for a turn ahead.
+    // The stage that is next, as expert, pairs and piece of f; a lane's columns of it are asked for a turn ahead.
     int e = 0, p0 = plan.start[0], c = 0;
     uint4 b[4][2];
     auto move = [&](int by) {
-      for (; by > 0; --by) {
-        if ((c += kMoeChunk) < a.f) continue;
-        c = 0;
+      for (c += by; c >= chunks;) {
+        c -= chunks;
         if ((p0 += 8) < plan.start[e + 1]) continue;
         if (++e == active) e = 0;
         p0 = plan.start[e];
@@ -802,47 +806,42 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_down16_kernel(const M
       // columns past the last token repeat it; their sums are not used
       const T* h = static_cast<const T*>(a.hidden) +
                    (size_t)(plan.order[min(p0 + r, plan.start[e + 1] - 1)] & 0xffff) * 2 * a.f_pad + t * 8;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = c + (i * kMoeTeam + member) * 32;
-        if (j < a.f) {
-          b[i][0] = *reinterpret_cast<const uint4*>(h + j);
-          b[i][1] = *reinterpret_cast<const uint4*>(h + a.f_pad + j);
-        }
-      }
+      h += c * kMoeChunk;
+      moe_quarters(member, a.f - c * kMoeChunk, [&](int i, int j, auto) {
+        b[i][0] = *reinterpret_cast<const uint4*>(h + j);
+        b[i][1] = *reinterpret_cast<const uint4*>(h + a.f_pad + j);
+      });
     };
     move(count = team);
     ask();
     for (int rows = blockIdx.x, until = row_stages; rows < row_blocks; rows += gridDim.x, until += row_stages) {
-      const int lo = rows * 16 + r < a.d ? a.f : 0, hi = rows * 16 + r + 8 < a.d ? a.f : 0;
       for (; count < until; count += kTeams) {
-        const int stage = count % kMoeDownStages, columns = min(kMoeChunk, a.f - c), cols = min(8, plan.start[e + 1] - p0);
-        const T* w = static_cast<const T*>(a.down) + plan.expert[e] * a.strideD + (size_t)(rows * 16 + r) * a.ldd + c;
+        const int stage = count % kMoeDownStages, columns = min(kMoeChunk, a.f - c * kMoeChunk);
+        const int cols = min(8, plan.start[e + 1] - p0);
+        const T* w = static_cast<const T*>(a.down) + plan.expert[e] * a.strideD + (size_t)(rows * 16 + r) * a.ldd + c * kMoeChunk;
+        const int lo = rows * 16 + r < a.d ? columns : 0, hi = rows * 16 + r + 8 < a.d ? columns : 0;
         const int* order = plan.order + p0;
         float acc[4] = {0.f, 0.f, 0.f, 0.f}, rest[4] = {0.f, 0.f, 0.f, 0.f};
-        if (fed && ok)
+        if (FED && ok)
           ok = mbar_wait_together(smem_u32(&full[stage]), count / kMoeDownStages & 1, &abort_flag, kFaultWaitFull, 0x4d21u);
         const uint32_t at = ring + stage * kStage;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = (i * kMoeTeam + member) * 32;
-          if (j < columns) {
-            uint4 w0, w1;
-            if (fed) {
-              w0 = moe_piece(at, r, j + t * 8, columns);
-              w1 = moe_piece(at, r + 8, j + t * 8, columns);
-            } else {
-              w0 = load8(w, lo - c, j + t * 8);
-              w1 = load8(w + 8 * a.ldd, hi - c, j + t * 8);
-            }
-            mma_16816<T>(acc, w0.x, w1.x, w0.y, w1.y, b[i][0].x, b[i][0].y);
-            mma_16816<T>(rest, w0.x, w1.x, w0.y, w1.y, b[i][1].x, b[i][1].y);
-            mma_16816<T>(acc, w0.z, w1.z, w0.w, w1.w, b[i][0].z, b[i][0].w);
-            mma_16816<T>(rest, w0.z, w1.z, w0.w, w1.w, b[i][1].z, b[i][1].w);
+        moe_quarters(member, columns, [&](int i, int j, auto whole) {
+          uint4 w0, w1;
+          if (FED) {
+            constexpr bool kWhole = decltype(whole)::value;
+            w0 = moe_piece<kWhole>(at, r, j + t * 8, columns);
+            w1 = moe_piece<kWhole>(at, r + 8, j + t * 8, columns);
+          } else {
+            w0 = load8(w, lo, j + t * 8);
+            w1 = load8(w + 8 * a.ldd, hi, j + t * 8);
           }
-        }
+          mma_16816<T>(acc, w0.x, w1.x, w0.y, w1.y, b[i][0].x, b[i][0].y);
+          mma_16816<T>(rest, w0.x, w1.x, w0.y, w1.y, b[i][1].x, b[i][1].y);
+          mma_16816<T>(acc, w0.z, w1.z, w0.w, w1.w, b[i][0].z, b[i][0].w);
+          mma_16816<T>(rest, w0.z, w1.z, w0.w, w1.w, b[i][1].z, b[i][1].w);
+        });
         __syncwarp();
-        if (fed && lane == 0) mbar_arrive(smem_u32(&empty[stage]));
+        if (FED && lane == 0) mbar_arrive(smem_u32(&empty[stage]));
         move(kTeams);
         ask();
         moe_add_products<T>(plan, ours, order, cols, acc, rest);
