@@ -342,6 +342,22 @@ static int run_moe(const MoeArgs& a, cudaStream_t st) {
 
 }  // namespace mmbo
 
+// f(a zero of the type, quarters of a group, whether there are zero points), the latter two as types.
+template <typename F>
+static void for_w4_kind(int dtype, int group, int zeros, F f) {
+  auto with_group = [&](auto zero, auto has_zeros) {
+    if (group == 32) f(zero, std::integral_constant<int, 1>(), has_zeros);
+    else if (group == 64) f(zero, std::integral_constant<int, 2>(), has_zeros);
+    else f(zero, std::integral_constant<int, 4>(), has_zeros);
+  };
+  auto with_zeros = [&](auto zero) {
+    if (zeros) with_group(zero, std::true_type());
+    else with_group(zero, std::false_type());
+  };
+  if (dtype == MMBO_DTYPE_F16) with_zeros(__half());
+  else with_zeros(__nv_bfloat16());
+}
+
 extern "C" {
 
 int mmbo_w4_bytes(size_t m, size_t k, int group, int zeros, size_t* bytes) {
@@ -364,13 +380,11 @@ int mmbo_w4_quantize(int dtype, size_t m, size_t k, int group, int zeros, const 
   unsigned grid = 0;
   if ((rc = w4_tile_grid(m, k, &grid))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const W4Format f{group, zeros};
-  if (dtype == MMBO_DTYPE_F16)
-    w4_quantize_kernel<__half><<<grid, 256, 0, st>>>(m, k, f, static_cast<const __half*>(W), ldw,
-                                                     static_cast<unsigned char*>(packed));
-  else
-    w4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m, k, f, static_cast<const __nv_bfloat16*>(W), ldw,
-                                                            static_cast<unsigned char*>(packed));
+  for_w4_kind(dtype, group, zeros, [&](auto zero, auto quarters, auto has_zeros) {
+    using T = decltype(zero);
+    w4_quantize_kernel<T, decltype(quarters)::value, decltype(has_zeros)::value>
+        <<<grid, 256, 0, st>>>(m, k, static_cast<const T*>(W), ldw, static_cast<unsigned char*>(packed));
+  });
   MMBO_COUNT_LAUNCH();
   return (int)cudaGetLastError();
 }
@@ -416,12 +430,11 @@ int mmbo_w4_unpack(int dtype, size_t m, size_t k, int group, int zeros, const vo
   unsigned grid = 0;
   if ((rc = w4_tile_grid(m, k, &grid))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const W4Format f{group, zeros};
-  const unsigned char* in = static_cast<const unsigned char*>(packed);
-  if (dtype == MMBO_DTYPE_F16)
-    w4_unpack_kernel<__half><<<grid, 256, 0, st>>>(m, k, f, in, static_cast<__half*>(W), ldw);
-  else
-    w4_unpack_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m, k, f, in, static_cast<__nv_bfloat16*>(W), ldw);
+  for_w4_kind(dtype, group, zeros, [&](auto zero, auto quarters, auto has_zeros) {
+    using T = decltype(zero);
+    w4_unpack_kernel<T, decltype(quarters)::value, decltype(has_zeros)::value>
+        <<<grid, 256, 0, st>>>(m, k, static_cast<const unsigned char*>(packed), static_cast<T*>(W), ldw);
+  });
   MMBO_COUNT_LAUNCH();
   return (int)cudaGetLastError();
 }

@@ -56,6 +56,16 @@ __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two 16-bit floats (as stored, low half first) widened.
+template <typename T>
+__device__ __forceinline__ float2 widen2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 widen2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+template <>
+__device__ __forceinline__ float2 widen2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
 // Elements at .. at + 7 of an array of `len`, zero behind its end, as they lie in memory; the array starts on any 2-byte
 // boundary.  Off the 16-byte boundaries two aligned loads are shifted together (eight loads of two bytes took four times
 // as long); nothing outside the array is read.  In two steps, so that several can be under way at a time.
@@ -99,6 +109,69 @@ __device__ __forceinline__ uint4 load8(const T* array, long long len, long long 
   return l.finish(array, len, at);
 }
 
+// ---------------------------------------------------------------- codes ---------------
+// Tile layout known at compile time.
+template <int QG, bool ZEROS>
+struct W4Tile {
+  static constexpr int kGroups = 4 / QG;  // QG: quarters of 32 columns in a group
+  static constexpr int kScales = kW4Codes, kZeros = kW4Codes + kGroups * kW4Rows * 2;
+  static constexpr int kBytes = kZeros + (ZEROS ? kGroups * kW4Rows : 0);
+};
+
+constexpr uint32_t kLowCodes = 0x000f000fu, kHighCodes = 0x00f000f0u;
+// Eight codes of a word as four registers of two 16-bit floats with the zero point subtracted, all exact.
+//   half precision: 0x6400 | q is 1024 + q and 0x6400 | 16 q is 1024 + 16 q, of which a fused multiply-add makes q - z
+//   bfloat16: 0x4300 | q is 128 + q (the 16 q form would spill into the exponent)
+template <typename T>
+struct W4Unpacker;
+// (x & mask) | with in one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t with) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(with));
+  return r;
+}
+// A constant the compiler keeps in a register: as an immediate beside the mask it would need a second instruction.
+__device__ __forceinline__ uint32_t in_register(uint32_t c) {
+  asm volatile("" : "+r"(c));
+  return c;
+}
+template <>
+struct W4Unpacker<__half> {
+  uint32_t bias, z1, z16;
+  __device__ __forceinline__ W4Unpacker() : bias(in_register(0x64006400u)) {}
+  __device__ __forceinline__ void set_zero(uint32_t z) {
+    z1 = (0x6400u | z) * 0x10001u;
+    z16 = (0xd400u | (z << 4)) * 0x10001u;  // -(64 + z)
+  }
+  __device__ __forceinline__ static __half2 h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+  __device__ __forceinline__ static uint32_t u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+  __device__ __forceinline__ void unpack(uint32_t w, uint32_t* a) const {
+    const uint32_t v = w >> 8;
+    const __half2 c16 = __half2half2(__ushort_as_half(0x2c00));  // 1 / 16
+    a[0] = u32(__hsub2(h2(and_or(w, kLowCodes, bias)), h2(z1)));
+    a[1] = u32(__hsub2(h2(and_or(v, kLowCodes, bias)), h2(z1)));
+    a[2] = u32(__hfma2(h2(and_or(w, kHighCodes, bias)), c16, h2(z16)));
+    a[3] = u32(__hfma2(h2(and_or(v, kHighCodes, bias)), c16, h2(z16)));
+  }
+};
+template <>
+struct W4Unpacker<__nv_bfloat16> {
+  uint32_t bias, z1;
+  __device__ __forceinline__ W4Unpacker() : bias(in_register(0x43004300u)) {}
+  __device__ __forceinline__ void set_zero(uint32_t z) { z1 = (0x4300u | z) * 0x10001u; }
+  __device__ __forceinline__ uint32_t one(uint32_t w) const {
+    uint32_t x = and_or(w, kLowCodes, bias);
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&z1));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
+  __device__ __forceinline__ void unpack(uint32_t w, uint32_t* a) const {
+    a[0] = one(w);
+    a[1] = one(w >> 8);
+    a[2] = one(w >> 4);
+    a[3] = one(w >> 12);
+  }
+};
+
 // ---------------------------------------------------------------- writing the format --
 // One warp per tile; lane 4 r + t (r 0..7, t 0..3) owns rows r and r + 8 of the block and, in each quarter u, the
 // columns 32 u + 8 t .. + 7: its eight words are two 16-byte stores, and the loads of four lanes are 64 contiguous
@@ -107,77 +180,120 @@ __device__ __forceinline__ uint4 load8(const T* array, long long len, long long 
 // Symmetric: s = max|w| / 7 rounded to the weights' type, z = 8.  With zero points: lo = min(w, 0), hi = max(w, 0),
 // s = (hi - lo) / 15 rounded to the weights' type, z = rint(-lo / s).  q = rint(w / s) + z, held to 0..15; ties to
 // even.  A group whose scale rounds to zero becomes zeros; one with an infinity or a NaN becomes NaN (its scale is).
+//
+// rint(w / s) without a division per element (a division bound the kernel: 53 us instead of 21 for a round trip of
+// 4096 x 4096): w * (1 / s) is within 2^-18 of w / s, and one fused multiply-add rounds it to a multiple of 2^-14.  With
+// significands of 11 bits at most w / s is either a tie, n + 1/2, which that rounding restores, or at least 2^-13 away from
+// one, which it keeps on its side.  A second addition rounds to an integer, ties to even.
+constexpr float kSnap = 768.f;             // adding it leaves multiples of 2^-14
+constexpr float kToInteger = 12582144.f;   // 1.5 * 2^23 - kSnap: adding it then leaves integers, in the low bits
+constexpr uint32_t kIntegerBits = 0x4b400000u;
 template <typename T>
-__global__ void w4_quantize_kernel(size_t m, size_t k, W4Format f, const T* __restrict__ W, size_t ldw,
-                                   unsigned char* __restrict__ packed) {
-  const size_t tiles = w4_k_tiles(k);
-  const size_t unit = (size_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (unit >= w4_row_blocks(m) * tiles) return;
-  const size_t block = unit / tiles, tile = unit % tiles;
+struct W4Pair {
+  using type = __half2;
+};
+template <>
+struct W4Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+};
+
+template <typename T, int QG, bool ZEROS>
+__global__ void __launch_bounds__(256) w4_quantize_kernel(size_t m, size_t k, const T* __restrict__ W, size_t ldw,
+                                                          unsigned char* __restrict__ packed) {
+  using L = W4Tile<QG, ZEROS>;
+  using Pair = typename W4Pair<T>::type;
+  const unsigned tiles = (unsigned)w4_k_tiles(k), unit = blockIdx.x * 8 + threadIdx.x / 32;
+  const unsigned block = unit / tiles, tile = unit % tiles;
+  if (block >= w4_row_blocks(m)) return;
   const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  unsigned char* out = packed + unit * f.tile_bytes();
-  const int per = f.group / 32;  // quarters in a group
+  unsigned char* out = packed + (size_t)unit * L::kBytes;
+  const size_t j0 = (size_t)tile * kW4Cols + 8 * t;
+  const bool whole = ldw % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15u) == 0 && (size_t)(tile + 1) * kW4Cols <= k;
+  uint4 w[2][4];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const size_t i = (size_t)block * kW4Rows + r + 8 * half;
+    const T* row = W + i * ldw;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (whole)
+        w[half][u] = i < m ? *reinterpret_cast<const uint4*>(row + j0 + 32 * u) : make_uint4(0, 0, 0, 0);
+      else
+        w[half][u] = load8(row, i < m ? (long long)k : 0, (long long)(j0 + 32 * u));
+    }
+  }
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int row = r + 8 * half;
-    const size_t i = block * kW4Rows + row;
-    __align__(16) T w[4][8];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      *reinterpret_cast<uint4*>(w[u]) =
-          load8(W + i * ldw, i < m ? (long long)k : 0, (long long)(tile * kW4Cols + 32 * u + 8 * t));
-    float lo[4], hi[4];
-    bool bad[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      lo[u] = hi[u] = 0.f;
-      bad[u] = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = to_f32(w[u][e]);
-        lo[u] = fminf(lo[u], v);
-        hi[u] = fmaxf(hi[u], v);
-        bad[u] |= !(fabsf(v) <= 3.4e38f);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int x = 1; x <= 2; x <<= 1) {
-        lo[u] = fminf(lo[u], __shfl_xor_sync(0xffffffffu, lo[u], x));
-        hi[u] = fmaxf(hi[u], __shfl_xor_sync(0xffffffffu, hi[u], x));
-        bad[u] |= __shfl_xor_sync(0xffffffffu, (int)bad[u], x) != 0;
-      }
-    }
     uint32_t word[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int first = u / per * per;
-      float l = lo[u], h = hi[u];
-      bool b = bad[u];
+    for (int g = 0; g < L::kGroups; ++g) {
+      // (lo, -hi) of the group; a NaN stays
+      const uint32_t none = 0;
+      Pair lo = *reinterpret_cast<const Pair*>(&none), hi = lo;
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        if (v >= first && v < first + per) {
-          l = fminf(l, lo[v]);
-          h = fmaxf(h, hi[v]);
-          b |= bad[v];
+      for (int q = 0; q < QG; ++q) {
+        const uint4 v = w[half][g * QG + q];
+        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Pair p = *reinterpret_cast<const Pair*>(&e[i]);
+          lo = __hmin2_nan(lo, p);
+          hi = __hmax2_nan(hi, p);
         }
-      // halves first: the span of two bfloat16 values may pass the largest float
-      const float wide = f.zeros ? (0.5f * h - 0.5f * l) / 7.5f : fmaxf(-l, h) / 7.f;
-      float s = to_f32(from_f32<T>(wide));
-      if (b || !(s <= 3.4e38f)) s = __int_as_float(0x7fc00000);
-      const bool live = s > 0.f;
-      const float z = f.zeros ? (live ? fminf(fmaxf(rintf(-l / s), 0.f), 15.f) : 0.f) : 8.f;
-      word[u] = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float q = live ? fminf(fmaxf(rintf(to_f32(w[u][e]) / s) + z, 0.f), 15.f) : z;
-        word[u] |= (uint32_t)q << (4 * w4_nibble(e));
       }
-      if (t == 0 && u % per == 0) {
-        const int g = u / per;
-        *reinterpret_cast<T*>(out + f.scale_at(g, row)) = from_f32<T>(s);
-        if (f.zeros) out[f.zero_at(g, row)] = (unsigned char)z;
+      hi = __hneg2(hi);
+      const uint32_t lows = *reinterpret_cast<const uint32_t*>(&lo), highs = *reinterpret_cast<const uint32_t*>(&hi);
+      const uint32_t first = __byte_perm(lows, highs, 0x5410), second = __byte_perm(lows, highs, 0x7632);
+      Pair ends = __hmin2_nan(*reinterpret_cast<const Pair*>(&first), *reinterpret_cast<const Pair*>(&second));
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&ends), x);
+        ends = __hmin2_nan(ends, *reinterpret_cast<const Pair*>(&other));
+      }
+      const float2 range = widen2<T>(*reinterpret_cast<const uint32_t*>(&ends));
+      const float l = range.x, h = -range.y;
+      // halves first: the span of two bfloat16 values may pass the largest float
+      const float wide = ZEROS ? (0.5f * h - 0.5f * l) / 7.5f : fmaxf(-l, h) / 7.f;
+      float s = to_f32(from_f32<T>(wide));
+      if (!(s <= 3.4e38f)) s = __int_as_float(0x7fc00000);
+      const bool live = s > 0.f;
+      // scales whose reciprocal might overflow (bfloat16 only) are divided by
+      const bool tiny = std::is_same<T, __nv_bfloat16>::value && live && s < 0x1p-100f;
+      const float inverse = __frcp_rn(s);
+      int z = 8;
+      if (ZEROS) {
+        const float y = tiny ? -l / s + kSnap : fmaf(-l, inverse, kSnap);
+        z = live ? (int)(__float_as_uint(fminf(y, kSnap + 15.f) + kToInteger) - kIntegerBits) : 0;
+      }
+      const float least = kSnap - (float)z, most = kSnap + (float)(15 - z);
+#pragma unroll
+      for (int q = 0; q < QG; ++q) {
+        const uint4 v = w[half][g * QG + q];
+        const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+        uint32_t bits[8], all = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 p = widen2<T>(e[i]);
+          float y0, y1;
+          if (tiny) {
+            y0 = p.x / s + kSnap;
+            y1 = p.y / s + kSnap;
+          } else {
+            y0 = fmaf(p.x, inverse, kSnap);
+            y1 = fmaf(p.y, inverse, kSnap);
+          }
+          bits[2 * i] = __float_as_uint(fminf(fmaxf(y0, least), most) + kToInteger);
+          bits[2 * i + 1] = __float_as_uint(fminf(fmaxf(y1, least), most) + kToInteger);
+        }
+#pragma unroll
+        for (int n = 7; n >= 0; --n) all = all * 16u + bits[w4_nibble(n)];  // nibble n holds column w4_nibble(n)
+        const uint32_t zeros = (uint32_t)z * 0x11111111u;
+        word[g * QG + q] = live ? all + (zeros - kIntegerBits * 0x11111111u) : zeros;
+      }
+      if (t == 0) {
+        *reinterpret_cast<T*>(out + L::kScales + (g * kW4Rows + W4Format::slot(row)) * 2) = from_f32<T>(s);
+        if (ZEROS) out[L::kZeros + g * kW4Rows + W4Format::slot(row)] = (unsigned char)z;
       }
     }
     *reinterpret_cast<uint4*>(out + w4_piece(row, t)) = make_uint4(word[0], word[1], word[2], word[3]);
@@ -232,42 +348,47 @@ __global__ void w4_pack_kernel(size_t m, size_t k, W4Format f, const unsigned ch
 
 // The weights that a packed matrix stands for, rounded to the 16-bit type (the product of a 4-bit difference and a
 // 16-bit scale has up to 15 bits): the mirror of w4_quantize_kernel.
-template <typename T>
-__global__ void w4_unpack_kernel(size_t m, size_t k, W4Format f, const unsigned char* __restrict__ packed,
-                                 T* __restrict__ W, size_t ldw) {
-  const size_t tiles = w4_k_tiles(k);
-  const size_t unit = (size_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (unit >= w4_row_blocks(m) * tiles) return;
-  const size_t block = unit / tiles, tile = unit % tiles;
+template <typename T, int QG, bool ZEROS>
+__global__ void __launch_bounds__(256) w4_unpack_kernel(size_t m, size_t k, const unsigned char* __restrict__ packed,
+                                                        T* __restrict__ W, size_t ldw) {
+  using L = W4Tile<QG, ZEROS>;
+  using Pair = typename W4Pair<T>::type;
+  const unsigned tiles = (unsigned)w4_k_tiles(k), unit = blockIdx.x * 8 + threadIdx.x / 32;
+  const unsigned block = unit / tiles, tile = unit % tiles;
+  if (block >= w4_row_blocks(m)) return;
   const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  const unsigned char* in = packed + unit * f.tile_bytes();
+  const unsigned char* in = packed + (size_t)unit * L::kBytes;
   const bool vec = ldw % 8 == 0 && (reinterpret_cast<uintptr_t>(W) & 15u) == 0;
-  const int per = f.group / 32;
+  W4Unpacker<T> unpacker;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int row = r + 8 * half;
-    const size_t i = block * kW4Rows + row;
+    const size_t i = (size_t)block * kW4Rows + row;
     if (i >= m) continue;
     const uint4 c = __ldg(reinterpret_cast<const uint4*>(in + w4_piece(row, t)));
     const uint32_t word[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const size_t j = tile * kW4Cols + 32 * u + 8 * t;
-      if (j >= k) continue;
-      const int g = u / per;
-      const float s = to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row)));
-      const int z = f.zeros ? in[f.zero_at(g, row)] : 8;
-      T v[8];
+      const size_t j = (size_t)tile * kW4Cols + 32 * u + 8 * t;
+      const int g = u / QG;
+      const uint32_t scale = *reinterpret_cast<const uint16_t*>(in + L::kScales + (g * kW4Rows + W4Format::slot(row)) * 2);
+      const uint32_t scales = scale * 0x10001u;
+      unpacker.set_zero(ZEROS ? in[L::kZeros + g * kW4Rows + W4Format::slot(row)] : 8u);
+      uint32_t v[4];
+      unpacker.unpack(word[u], v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[e] = from_f32<T>((float)((int)((word[u] >> (4 * w4_nibble(e))) & 15u) - z) * s);
+      for (int e = 0; e < 4; ++e) {
+        const Pair p = __hmul2(*reinterpret_cast<const Pair*>(&v[e]), *reinterpret_cast<const Pair*>(&scales));
+        v[e] = *reinterpret_cast<const uint32_t*>(&p);
+      }
       T* dst = W + i * ldw + j;
       if (vec && j + 8 <= k) {
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
       } else {
+        const T* from = reinterpret_cast<const T*>(v);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (j + e < k) dst[e] = v[e];
+          if (j + e < k) dst[e] = from[e];
       }
     }
   }

@@ -25,7 +25,6 @@
 
 namespace mmbo {
 
-constexpr uint32_t kLowCodes = 0x000f000fu, kHighCodes = 0x00f000f0u;
 
 // c (16 x 8) = a (16 x 16) * b (16 x 8) + c (or + 0), fp32 sums.
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -61,24 +60,6 @@ __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
-// Two 16-bit floats (as stored, low half first) widened.
-template <typename T>
-__device__ __forceinline__ float2 widen2(uint32_t v);
-template <>
-__device__ __forceinline__ float2 widen2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-template <>
-__device__ __forceinline__ float2 widen2<__nv_bfloat16>(uint32_t v) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-}
-
-// Tile layout known at compile time.
-template <int QG, bool ZEROS>
-struct W4Tile {
-  static constexpr int kGroups = 4 / QG;  // QG: quarters of 32 columns in a group
-  static constexpr int kScales = kW4Codes, kZeros = kW4Codes + kGroups * kW4Rows * 2;
-  static constexpr int kBytes = kZeros + (ZEROS ? kGroups * kW4Rows : 0);
-};
-
 // acc += the products of a tile with 128 rows of 8 columns: b(q) is this lane's 16 bytes of quarter q of its column, xs(g)
 // the sums of group g of the columns 2 t and 2 t + 1.  Sums are in units of 2^20.
 //

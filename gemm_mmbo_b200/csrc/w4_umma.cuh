@@ -17,59 +17,6 @@
 
 namespace mmbo {
 
-// Eight codes of a word as four registers of two 16-bit floats with the zero point subtracted, all exact.
-//   half precision: 0x6400 | q is 1024 + q and 0x6400 | 16 q is 1024 + 16 q, of which a fused multiply-add makes q - z
-//   bfloat16: 0x4300 | q is 128 + q (the 16 q form would spill into the exponent)
-template <typename T>
-struct W4Unpacker;
-// (x & mask) | with in one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t with) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(with));
-  return r;
-}
-// A constant the compiler keeps in a register: as an immediate beside the mask it would need a second instruction.
-__device__ __forceinline__ uint32_t in_register(uint32_t c) {
-  asm volatile("" : "+r"(c));
-  return c;
-}
-template <>
-struct W4Unpacker<__half> {
-  uint32_t bias, z1, z16;
-  __device__ __forceinline__ W4Unpacker() : bias(in_register(0x64006400u)) {}
-  __device__ __forceinline__ void set_zero(uint32_t z) {
-    z1 = (0x6400u | z) * 0x10001u;
-    z16 = (0xd400u | (z << 4)) * 0x10001u;  // -(64 + z)
-  }
-  __device__ __forceinline__ static __half2 h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
-  __device__ __forceinline__ static uint32_t u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
-  __device__ __forceinline__ void unpack(uint32_t w, uint32_t* a) const {
-    const uint32_t v = w >> 8;
-    const __half2 c16 = __half2half2(__ushort_as_half(0x2c00));  // 1 / 16
-    a[0] = u32(__hsub2(h2(and_or(w, kLowCodes, bias)), h2(z1)));
-    a[1] = u32(__hsub2(h2(and_or(v, kLowCodes, bias)), h2(z1)));
-    a[2] = u32(__hfma2(h2(and_or(w, kHighCodes, bias)), c16, h2(z16)));
-    a[3] = u32(__hfma2(h2(and_or(v, kHighCodes, bias)), c16, h2(z16)));
-  }
-};
-template <>
-struct W4Unpacker<__nv_bfloat16> {
-  uint32_t bias, z1;
-  __device__ __forceinline__ W4Unpacker() : bias(in_register(0x43004300u)) {}
-  __device__ __forceinline__ void set_zero(uint32_t z) { z1 = (0x4300u | z) * 0x10001u; }
-  __device__ __forceinline__ uint32_t one(uint32_t w) const {
-    uint32_t x = and_or(w, kLowCodes, bias);
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&z1));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  }
-  __device__ __forceinline__ void unpack(uint32_t w, uint32_t* a) const {
-    a[0] = one(w);
-    a[1] = one(w >> 8);
-    a[2] = one(w >> 4);
-    a[3] = one(w >> 12);
-  }
-};
-
 // 32 lanes x 32 consecutive 32-bit columns of tensor memory, thread t of the warp writing lane (base lane + t).
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
