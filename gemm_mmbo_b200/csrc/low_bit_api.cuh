@@ -342,13 +342,17 @@ static int run_moe(const MoeArgs& a, cudaStream_t st) {
 
 }  // namespace mmbo
 
-// f(a zero of the type, quarters of a group, whether there are zero points), the latter two as types.
+// f(a zero of the type, quarters of a group, whether there are zero points, whether the rows are aligned), all as types.
 template <typename F>
-static void for_w4_kind(int dtype, int group, int zeros, F f) {
+static void for_w4_kind(int dtype, int group, int zeros, bool aligned, F f) {
+  auto with_aligned = [&](auto zero, auto quarters, auto has_zeros) {
+    if (aligned) f(zero, quarters, has_zeros, std::true_type());
+    else f(zero, quarters, has_zeros, std::false_type());
+  };
   auto with_group = [&](auto zero, auto has_zeros) {
-    if (group == 32) f(zero, std::integral_constant<int, 1>(), has_zeros);
-    else if (group == 64) f(zero, std::integral_constant<int, 2>(), has_zeros);
-    else f(zero, std::integral_constant<int, 4>(), has_zeros);
+    if (group == 32) with_aligned(zero, std::integral_constant<int, 1>(), has_zeros);
+    else if (group == 64) with_aligned(zero, std::integral_constant<int, 2>(), has_zeros);
+    else with_aligned(zero, std::integral_constant<int, 4>(), has_zeros);
   };
   auto with_zeros = [&](auto zero) {
     if (zeros) with_group(zero, std::true_type());
@@ -380,9 +384,9 @@ int mmbo_w4_quantize(int dtype, size_t m, size_t k, int group, int zeros, const 
   unsigned grid = 0;
   if ((rc = w4_tile_grid(m, k, &grid))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  for_w4_kind(dtype, group, zeros, [&](auto zero, auto quarters, auto has_zeros) {
+  for_w4_kind(dtype, group, zeros, ldw % 8 == 0 && aligned16(W), [&](auto zero, auto quarters, auto has_zeros, auto aligned) {
     using T = decltype(zero);
-    w4_quantize_kernel<T, decltype(quarters)::value, decltype(has_zeros)::value>
+    w4_quantize_kernel<T, decltype(quarters)::value, decltype(has_zeros)::value, decltype(aligned)::value>
         <<<grid, 256, 0, st>>>(m, k, static_cast<const T*>(W), ldw, static_cast<unsigned char*>(packed));
   });
   MMBO_COUNT_LAUNCH();
@@ -430,9 +434,9 @@ int mmbo_w4_unpack(int dtype, size_t m, size_t k, int group, int zeros, const vo
   unsigned grid = 0;
   if ((rc = w4_tile_grid(m, k, &grid))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  for_w4_kind(dtype, group, zeros, [&](auto zero, auto quarters, auto has_zeros) {
+  for_w4_kind(dtype, group, zeros, ldw % 8 == 0 && aligned16(W), [&](auto zero, auto quarters, auto has_zeros, auto aligned) {
     using T = decltype(zero);
-    w4_unpack_kernel<T, decltype(quarters)::value, decltype(has_zeros)::value>
+    w4_unpack_kernel<T, decltype(quarters)::value, decltype(has_zeros)::value, decltype(aligned)::value>
         <<<grid, 256, 0, st>>>(m, k, static_cast<const unsigned char*>(packed), static_cast<T*>(W), ldw);
   });
   MMBO_COUNT_LAUNCH();

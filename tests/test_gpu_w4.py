@@ -169,6 +169,14 @@ def test_offsets_past_32_bits(cuda, mm):
 # ---------------------------------------------------------------- packing and rounding --
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(40, 8, 70001), (24, 5, 40000), (17, 1, 200000), (20001, 8, 256), (150000, 3, 64),
+                                   (1024, 1, 16384), (16, 16, 60000), (40000, 9, 130)])
+def test_product_of_long_and_tall_matrices(cuda, mm, dtype, m, n, k):
+    """Activations that do not fit a block's shared memory, contractions cut over blocks, several batches of rows a block."""
+    product(mm, dtype, m, n, k, 128, True)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("group,zeros", [(32, True), (32, False), (64, True), (128, False), (128, True)])
 def test_round_trip_is_the_formula(cuda, mm, dtype, group, zeros):
     """Rounding and unpacking against 64 bits: equal to the last bit, ties and short last groups included."""
@@ -196,6 +204,26 @@ def test_round_trip_is_the_formula(cuda, mm, dtype, group, zeros):
         assert torch.equal(out[:, :k].cpu(), want), (m, k)
         before[64:64 + out.numel()].view(out.shape)[:, :k] = out[:, :k]
         assert torch.equal(before.view(torch.int16), obuf.view(torch.int16)), "written outside W"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("ld", [700, 701, 702, 704])
+def test_round_trip_with_rows_at_any_address(cuda, mm, dtype, ld):
+    """Rows that start on any 2-byte boundary, tiles inside the rows and at their ends; the columns between them stay."""
+    dt, m, k, group = TYPES[dtype], 19, 700, 64
+    w = (torch.randn(m, k, generator=torch.Generator().manual_seed(ld)) * 0.02).to(dt)
+    want = round64(w, group, True, dt).to(dt)
+    for off in range(8):
+        flat = torch.full((m * ld + 16,), float("nan"), dtype=dt, device="cuda")
+        flat[off:off + m * ld].view(m, ld)[:, :k] = w.cuda()
+        packed = torch.zeros(mm.w4_bytes(m, k, group, True), dtype=torch.uint8, device="cuda")
+        mm.w4_quantize(dtype, m, k, group, True, flat[off:], ld, packed)
+        back = torch.full_like(flat, float("nan"))
+        mm.w4_unpack(dtype, m, k, group, True, packed, back[off:], ld)
+        out = back[off:off + m * ld].view(m, ld)
+        assert torch.equal(out[:, :k].cpu(), want), off
+        out[:, :k] = float("nan")
+        assert torch.isnan(back.float()).all(), "written outside W"
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
