@@ -105,8 +105,8 @@ static int launch_clustered(K kernel, unsigned grid, unsigned threads, size_t sm
 }
 
 // How w4_gemv_kernel cuts a problem: the cheapest of all (warps along k, blocks along k), by a sum of what was measured
-// (B200, us): 0.022 a tile of the busiest SM, 0.3 a slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join clusters of two / four.  8192 x 28672, one
-// column: 28.4 us with the chosen 16 x 2, 30.7 with 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
+// (B200, us): 0.022 a tile of the busiest SM, 0.3 a slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join
+// clusters of two / four, 1 a batch of row groups.  8192 x 28672, one column: 28.4 us with the chosen 16 x 2, 30.7 with 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
 template <int QG>
 static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3], size_t* smem) {
   const size_t k_tiles = w4_k_tiles(a.k), blocks = w4_row_blocks(a.m);
@@ -115,10 +115,14 @@ static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3]
     for (int split_log2 = 0; split_log2 <= 2; ++split_log2) {
       const size_t wk = (size_t)1 << wk_log2, split = (size_t)1 << split_log2, wm = kGemvWarps / wk;
       if (split > 1 && k_tiles < split) continue;
-      const size_t groups = (blocks + wm - 1) / wm, span = (k_tiles + split - 1) / split, part = (span + wk - 1) / wk;
+      const size_t groups = (blocks + wm - 1) >> (4 - wk_log2), span = (k_tiles + split - 1) >> split_log2, part = (span + wk - 1) >> wk_log2;
       const size_t cl = groups < (size_t)clusters[split_log2] ? groups : (size_t)clusters[split_log2];
       const size_t rounds = (groups + cl - 1) / cl;
       const int slot_tiles = part < 4 ? (int)(part ? part : 1) : 4;
+      const double staged = (double)a.n * span * 0.25;
+      double cost = rounds * wm * span * 0.022 + rounds * ((part + slot_tiles - 1) / slot_tiles) * 0.3 + staged * 0.05 +
+                    (split == 1 ? 0.0 : split == 2 ? 1.8 : 2.5);
+      if (cost >= best) continue;
       const size_t ring = (size_t)kGemvWarps * 2 * slot_tiles * tile_bytes;
       const size_t one = gemv_sums_bytes((int)wk, (int)split, a.n, 1);
       if (ring + one + gemv_x_bytes(a.n, 1, 4 / QG) > kGemvSmem) continue;
@@ -130,9 +134,7 @@ static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3]
       if (batch > rounds) batch = rounds;
       if (batch == 0 || (split > 1 && batch < rounds)) continue;
       const size_t batches = (rounds + batch - 1) / batch;
-      const double staged = (double)a.n * span * 0.25 * (x_tiles < span ? batches : 1);
-      const double cost = rounds * wm * span * 0.022 + rounds * ((part + slot_tiles - 1) / slot_tiles) * 0.3 +
-                          staged * 0.05 + (split == 1 ? 0.0 : split == 2 ? 1.8 : 2.5) + (batches - 1) * 1.0;
+      cost += (x_tiles < span ? (batches - 1) * staged * 0.05 : 0.0) + (batches - 1) * 1.0;
       if (cost < best) {
         best = cost;
         a.wk_log2 = wk_log2;

@@ -353,11 +353,27 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
       for (int col = 0; col < n && whole > 0; ++col)
         bulk_load(smem_u32(xs) + col * x_stride, static_cast<const T*>(a.B) + col * a.ldb + k0, whole * 16, smem_u32(&x_bar));
     }
-    for (int col = 0; col < n; ++col)
-#pragma unroll 2
-      for (int piece = whole + threadIdx.x; piece < pieces; piece += kWorkers)
-        *reinterpret_cast<uint4*>(xs + col * x_stride + piece * 16) =
-            load8(static_cast<const T*>(a.B) + col * a.ldb, (long long)a.k, (long long)k0 + piece * 8);
+    // what bulk copies cannot bring: four pieces of a thread under way at a time
+    int col = whole < pieces ? 0 : n, piece = whole + threadIdx.x;
+    while (col < n) {
+      Load8 load[4];
+      int cols[4], at[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i, piece += kWorkers) {
+        while (piece >= pieces && col < n) {
+          piece -= pieces - whole;
+          ++col;
+        }
+        cols[i] = col;
+        at[i] = piece;
+        if (col < n) load[i].issue(static_cast<const T*>(a.B) + col * a.ldb, (long long)a.k, (long long)k0 + piece * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (cols[i] < n)
+          *reinterpret_cast<uint4*>(xs + cols[i] * x_stride + at[i] * 16) =
+              load[i].finish(static_cast<const T*>(a.B) + cols[i] * a.ldb, (long long)a.k, (long long)k0 + at[i] * 8);
+    }
   };
   if (warp < kGemvWarps) request_x(0);
 
