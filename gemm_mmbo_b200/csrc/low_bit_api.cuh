@@ -204,6 +204,8 @@ static int launch_w4_umma(UmmaArgs a, cudaStream_t st) {
   if (rc) return rc;
   constexpr uint32_t kTile = W4Tile<QG, ZEROS>::kBytes;
   const size_t stage = S::kXBytes + umma_code_bytes(kTile), fixed = 1024 + (a.split_log2 ? NT * 512 : 0);
+  static_assert(S::kUnpackSets == 1 || (kGemvSmem - 1024 - NT * 512) / (S::kXBytes + umma_code_bytes(kTile)) >=
+                                           S::kUnpackSets + kUmmaASlots, "");  // see the unpackers
   a.stages = (int)((kGemvSmem - fixed) / stage);
   if (a.stages > kUmmaMaxStages) a.stages = kUmmaMaxStages;
   a.col_tiles = (int)((a.n + NT - 1) / NT);

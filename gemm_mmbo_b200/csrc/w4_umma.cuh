@@ -209,7 +209,9 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
         }
       }
   } else if (warp >= 4 && warp < 4 + 4 * S::kUnpackSets) {
-    // ---- unpackers: thread = row of the tile
+    // ---- unpackers: thread = row of the tile.  A set skips phases of the ring's barriers, those of the other set's tiles.  It
+    // cannot take an older phase for its own: tile i - kUnpackSets had its place in tensor memory only after the products of
+    // the tile kUmmaASlots before it, so what was loaded up to there is complete, and the ring has that many stages or more.
     const int set = (warp - 4) / 4, row = (warp & 3) * 32 + lane, r = row & 15;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     int stage = set % a.stages;
