@@ -26,7 +26,7 @@ static size_t w4_total_bytes(size_t m, size_t k, const W4Format& f) {
 // One warp per tile, eight to a block.
 static int w4_tile_grid(size_t m, size_t k, unsigned* grid) {
   const size_t blocks = (w4_row_blocks(m) * w4_k_tiles(k) + 7) / 8;
-  if (blocks > 0x7fffffffull) return MMBO_ERR_TOO_LARGE;
+  if (blocks > 0x1fffffffull) return MMBO_ERR_TOO_LARGE;  // tiles are counted in 32 bits
   *grid = (unsigned)blocks;
   return MMBO_OK;
 }
@@ -106,7 +106,8 @@ static int launch_clustered(K kernel, unsigned grid, unsigned threads, size_t sm
 
 // How w4_gemv_kernel cuts a problem: the cheapest of all (warps along k, blocks along k), by a sum of what was measured
 // (B200, us): 0.022 a tile of the busiest SM, 0.3 a slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join
-// clusters of two / four, 1 a batch of row groups.  8192 x 28672, one column: 28.4 us with the chosen 16 x 2, 30.7 with 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
+// clusters of two / four, 1 a batch of row groups.  8192 x 28672, one column: 28.4 us with the chosen 16 x 2, 30.7 with
+// 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
 template <int QG>
 static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3], size_t* smem) {
   const size_t k_tiles = w4_k_tiles(a.k), blocks = w4_row_blocks(a.m);
@@ -115,7 +116,8 @@ static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3]
     for (int split_log2 = 0; split_log2 <= 2; ++split_log2) {
       const size_t wk = (size_t)1 << wk_log2, split = (size_t)1 << split_log2, wm = kGemvWarps / wk;
       if (split > 1 && k_tiles < split) continue;
-      const size_t groups = (blocks + wm - 1) >> (4 - wk_log2), span = (k_tiles + split - 1) >> split_log2, part = (span + wk - 1) >> wk_log2;
+      const size_t groups = (blocks + wm - 1) >> (4 - wk_log2), span = (k_tiles + split - 1) >> split_log2;
+      const size_t part = (span + wk - 1) >> wk_log2;
       const size_t cl = groups < (size_t)clusters[split_log2] ? groups : (size_t)clusters[split_log2];
       const size_t rounds = (groups + cl - 1) / cl;
       const int slot_tiles = part < 4 ? (int)(part ? part : 1) : 4;
@@ -185,7 +187,8 @@ static void plan_umma(size_t m, size_t n, size_t k, bool x_tma, int* nt, int* sp
       const size_t tiles = row_tiles * ((n + w - 1) / w), slots = (size_t)cluster_slots(log2);
       if (log2 && (tiles > slots || k_tiles < ((size_t)1 << log2))) continue;
       const size_t rounds = (tiles + slots - 1) / slots, span = (k_tiles + ((size_t)1 << log2) - 1) >> log2;
-      const double cost = (double)rounds * span * (w == 32 ? (x_tma ? 500.0 : 700.0) : w == 64 ? (x_tma ? 620.0 : 1100.0) : 900.0) + (double)rounds * w * 10 +
+      const double tile = w == 32 ? (x_tma ? 500.0 : 700.0) : w == 64 ? (x_tma ? 620.0 : 1100.0) : 900.0;
+      const double cost = (double)rounds * span * tile + (double)rounds * w * 10 +
                           (log2 == 0 ? 0.0 : log2 == 1 ? 2500.0 : 3500.0);
       if (cost < best) {
         best = cost;

@@ -19,9 +19,9 @@
 // 16 bytes' worth of k of a lane's token), come straight from L2.  Tokens are the eight columns of the instruction; an expert
 // with more tokens is taken in groups of eight, the later ones finding its weights in L2.
 //
-// Measured (whole layer, B200): 48 tokens, 8 of 64 fp16 experts, 2048 to 1408: 232 us, up 131 us (740 MB, 5.6 TB/s), down 100 us
+// Measured (whole layer, B200): 48 tokens, 8 of 64 fp16 experts, 2048 to 1408: 231 us, up 131 us (740 MB, 5.6 TB/s), down 100 us
 // (371 MB on 128 of 148 SMs; 76 us without its arithmetic); one token, 6 of 64 bf16 experts of that size: 36 us, of which
-// scores 8, up 22, down 13 one by one; 8 tokens, 4 of 32 packed experts, 4096 to 1800: 89 us, up 45 us and down 43 us (3.9 and
+// scores 8, up 22, down 13 one by one; 8 tokens, 4 of 32 packed experts, 4096 to 1800: 86 us, up 45 us and down 43 us (3.9 and
 // 2.2 TB/s: instructions, about 170 a tile in up and 230 in down).  Asking for packed experts' columns a tile ahead made both
 // slower (97 us): the added instructions cost more than the wait.
 #pragma once
@@ -425,8 +425,8 @@ __device__ __forceinline__ void moe_keep_sums(float* to, const float (&gate)[4],
 
 // 16-bit weights.  A stage holds 512 columns of 16 rows of gate and of up, each row one copy of 1 KB (a warp's own copies of
 // 64 or 128 bytes a row left DRAM at 3.9 TB/s).  Teams of four warps take the stages in turn: with all sixteen in step on
-// every stage the columns' way from L2 was the bound (390 us instead of 241 for 48 tokens, 8 of 64 experts each, 2048 to 1408).  Rows lie 64 bytes out of step:
-// conflict-free 16-byte reads.
+// every stage the columns' way from L2 was the bound (390 us instead of 241 for 48 tokens, 8 of 64 experts each, 2048 to
+// 1408).  Rows lie 64 bytes out of step: conflict-free 16-byte reads.
 constexpr int kMoeChunk = 512, kMoeTeam = 4;
 constexpr uint32_t kMoeRowBytes = kMoeChunk * 2 + 64;
 // Multiples of the teams: a team always waits at the same barriers, phase after phase (one that skipped phases could take an

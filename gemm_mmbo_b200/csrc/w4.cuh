@@ -189,7 +189,8 @@ struct W4Unpacker<__nv_bfloat16> {
 // rint(w / s) without a division per element (a division bound the kernel: 53 us instead of 21 for a round trip of
 // 4096 x 4096): w * (1 / s) is within 2^-18 of w / s, and one fused multiply-add rounds it to a multiple of 2^-14.  With
 // significands of 11 bits at most w / s is either a tie, n + 1/2, which that rounding restores, or at least 2^-13 away from
-// one, which it keeps on its side (all pairs of significands were compared with the quotient).  A second addition rounds to an integer, ties to even.
+// one, which it keeps on its side (all pairs of significands were compared with the quotient).  A second
+// addition rounds to an integer, ties to even.
 // A group's scale, too, is computed by one of its four lanes instead of all (ragged 11001 x 8200 in groups of 32 with zero
 // points: 83 us before, 54 us after).
 constexpr float kSnap = 768.f;             // adding it leaves multiples of 2^-14
@@ -271,8 +272,10 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(size_t m, size_t k, co
     // A group's multiplier; -s for a scale whose reciprocal might overflow (bfloat16 only): these divide.
     const float by = !(s > 0.f) ? 0.f : std::is_same<T, __nv_bfloat16>::value && s < 0x1p-100f ? -s : __frcp_rn(s);
     int zero = 8;
-    if (ZEROS) zero = (int)(__float_as_uint(fminf(by < 0.f ? -l / s + kSnap : fmaf(-l, by, kSnap), kSnap + 15.f) + kToInteger) - kIntegerBits);
-    if (ZEROS && !(s > 0.f)) zero = 0;
+    if (ZEROS) {
+      const float y = by < 0.f ? -l / s + kSnap : fmaf(-l, by, kSnap);
+      zero = s > 0.f ? (int)(__float_as_uint(fminf(y, kSnap + 15.f) + kToInteger) - kIntegerBits) : 0;
+    }
     if (t % QG == 0) {
       const int at = t / QG * kW4Rows + W4Format::slot(row);
       *reinterpret_cast<T*>(out + L::kScales + at * 2) = from_f32<T>(s);

@@ -357,6 +357,8 @@ int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, const float* alpha, co
  * of gate_e at gate + e * strideG + i * ldg elements (ldg >= d; up the same), of down_e at
  * down + e * strideD + i * ldd (ldd >= f).  group != 0: packed experts (the format above), expert e
  * at e * strideG (strideD) BYTES, multiples of 16; ldg and ldd are not used.
+ * Sums, scores and gates are fp32; a hidden value (silu(gate) o up) keeps 16 bits and more, with 16-bit
+ * fp16 experts up to a magnitude of 4.19e6 (larger ones become infinite).
  * ids (tokens x topk, int) and gates (tokens x topk, float) receive the choice and may be NULL.
  * tokens <= MMBO_MOE_MAX_TOKENS, topk <= MMBO_MOE_MAX_TOPK, experts <= MMBO_MOE_MAX_EXPERTS, d and f
  * <= MMBO_MOE_MAX_WIDTH.  workspace: 256-byte aligned device memory of at least

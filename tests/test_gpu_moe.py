@@ -1,5 +1,8 @@
 """A whole mixture-of-experts layer for a few tokens against its formula in 64 bits."""
 import math
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -90,6 +93,29 @@ SIZES = [(1, 64, 32, 4, 1), (1, 256, 384, 8, 2), (2, 130, 70, 5, 5), (3, 200, 12
 def test_layer(cuda, mm, dtype, group, zeros):
     for i, s in enumerate(SIZES):
         Layer(mm, dtype, *s, renorm=bool(i % 2), group=group, zeros=zeros, seed=i).check()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("group", [0, 32, 128])
+def test_long_rows(cuda, mm, dtype, group):
+    """Rows of several pieces with a ragged last one, experts with more tokens than a group takes, many rows of units to a
+    block and blocks without any."""
+    for i, s in enumerate(((20, 1096, 1544, 3, 1), (7, 2048, 520, 5, 3), (1, 3000, 2056, 2, 2), (64, 640, 1032, 2, 1),
+                           (33, 513, 1025, 4, 2), (3, 5000, 16, 3, 1))):
+        Layer(mm, dtype, *s, renorm=bool(i % 2), group=group, zeros=group == 32, seed=40 + i).check()
+
+
+def test_the_widest_layers(cuda, mm):
+    Layer(mm, "f16", 2, 65536, 24, 2, 1).check()
+    Layer(mm, "f16", 2, 24, 65536, 2, 1).check()
+    Layer(mm, "bf16", 1, 65536, 40, 2, 2, group=64).check()
+    Layer(mm, "bf16", 1, 40, 65536, 2, 2, group=128).check()
+
+
+def test_the_most_tokens(cuda, mm):
+    """Four passes of 64 tokens, with one expert and with several."""
+    Layer(mm, "f16", 256, 64, 48, 1, 1).check()
+    Layer(mm, "bf16", 256, 72, 40, 3, 2, renorm=True, group=32).check()
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
@@ -243,3 +269,49 @@ def test_decoding_step(cuda, mm):
     # three results rounded to half precision (2^-11 of their size each), each passing through a product whose rows
     # have norm about one: eight half steps of the largest logit
     assert (logits.cpu().double() - want).abs().max() <= 8 * 2.0 ** -11 * want.abs().max()
+
+
+FIRST_CALLS = """
+import torch
+import gemm_mmbo_b200 as mm
+t, d, f, E, k, g = 3, 320, 200, 6, 2, 64
+gen = torch.Generator().manual_seed(0)
+r = lambda *s: (torch.randn(*s, generator=gen) * 0.1).half().cuda()
+x, router, W = r(t, d), r(E, d), r(E * f, d)
+gate, up, down = r(E, f, d), r(E, f, d), r(E, d, f)
+per, perd = mm.w4_bytes(f, d, g, True), mm.w4_bytes(d, f, g, True)
+pg, pu, pd = [torch.zeros(E * b, dtype=torch.uint8, device="cuda") for b in (per, per, perd)]
+packed = torch.zeros(mm.w4_bytes(E * f, d, g, True), dtype=torch.uint8, device="cuda")
+ws = torch.empty(mm.moe_workspace_bytes("f16", t, d, f, E, k), dtype=torch.uint8, device="cuda")
+many = r(40, d)
+outs = [torch.zeros(t, d).half().cuda(), torch.zeros(t, d).half().cuda(), torch.zeros(1, E * f).half().cuda(),
+        torch.zeros(40, E * f).half().cuda(), torch.zeros(E * f, d).half().cuda()]
+def step(o):
+    mm.w4_quantize("f16", E * f, d, g, True, W, d, packed)
+    for e in range(E):
+        mm.w4_quantize("f16", f, d, g, True, gate[e], d, pg[e * per:])
+        mm.w4_quantize("f16", f, d, g, True, up[e], d, pu[e * per:])
+        mm.w4_quantize("f16", d, f, g, True, down[e], f, pd[e * perd:])
+    mm.moe("f16", t, d, f, E, k, x, d, router, d, gate, up, d, f * d, down, f, d * f, o[0], d, workspace=ws)
+    mm.moe("f16", t, d, f, E, k, x, d, router, d, pg, pu, 0, per, pd, 0, perd, o[1], d, group=g, zeros=True, workspace=ws)
+    mm.gemm_w4("f16", E * f, 1, d, 1.0, packed, g, True, x, d, 0.0, o[2], E * f)
+    mm.gemm_w4("f16", E * f, 40, d, 1.0, packed, g, True, many, d, 0.0, o[3], E * f)
+    mm.w4_unpack("f16", E * f, d, g, True, packed, o[4], d)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step(outs)
+graph.replay()
+torch.cuda.synchronize()
+eager = [torch.zeros_like(o) for o in outs]
+step(eager)
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) and bool(a.abs().sum() > 0) for a, b in zip(outs, eager))
+assert mm.device_status() == 0
+"""
+
+
+def test_first_calls_of_a_process_captured(cuda):
+    """Nothing has to run before it can be captured."""
+    subprocess.run([sys.executable, "-c", FIRST_CALLS], check=True, timeout=300,
+                   cwd=pathlib.Path(__file__).resolve().parent.parent)
