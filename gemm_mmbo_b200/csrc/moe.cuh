@@ -407,9 +407,9 @@ __device__ __forceinline__ void moe_finish_unit(const MoeArgs& a, const float* s
   }
   const int entry = order[i / 16];
   if (packed) {
-    const float2 undo = a.x_undo[entry >> 16];
-    g *= undo.x * undo.y;
-    u *= undo.x * undo.y;
+    const float2 undo = a.x_undo[entry >> 16];  // one after the other: their product may pass the largest float
+    g = g * undo.x * undo.y;
+    u = u * undo.x * undo.y;
   }
   moe_store_hidden<U>(a, entry & 0xffff, rows * 16 + (i & 15), g, u);
 }

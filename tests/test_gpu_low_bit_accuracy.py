@@ -1,0 +1,55 @@
+"""Inputs on which the 4-bit and mixture-of-experts entry points could lose what their formulas keep: values far apart, sums near
+the ends of a type's range, codes equal to their zero points, results that nearly cancel."""
+import pytest
+import torch
+
+from low_bit import TYPES, check16, make_w4, moe64, pack, weights64
+
+pytestmark = pytest.mark.gpu
+
+
+def expert_layer(mm, dtype, x, router, experts, group, topk, renorm=False, beta=0.0, Y=None):
+    """One call with packed experts (a dict of lists of (codes, scales, zero points)); returns Y, ids and gates on the CPU."""
+    (tokens, d), E = x.shape, router.shape[0]
+    f = experts["gate"][0][0].shape[0]
+    zeros = experts["gate"][0][2] is not None
+    dev = {n: torch.stack([pack(mm, dtype, *p, group) for p in v]) for n, v in experts.items()}
+    Y = torch.full((tokens, d), float("nan"), dtype=TYPES[dtype], device="cuda") if Y is None else Y
+    ids = torch.full((tokens, topk), -1, dtype=torch.int32, device="cuda")
+    gates = torch.full((tokens, topk), float("nan"), device="cuda")
+    ws = torch.full((mm.moe_workspace_bytes(dtype, tokens, d, f, E, topk),), 0xFF, dtype=torch.uint8, device="cuda")
+    mm.moe(dtype, tokens, d, f, E, topk, x.cuda(), d, router.cuda(), d, dev["gate"], dev["up"], ldg=0,
+           strideG=dev["gate"].stride(0), down=dev["down"], ldd=0, strideD=dev["down"].stride(0), Y=Y, ldy=d, group=group,
+           zeros=zeros, renorm=renorm, beta=beta, ids=ids, gates=gates, workspace=ws)
+    torch.cuda.synchronize()
+    assert mm.device_status() == 0
+    return Y.cpu(), ids.cpu(), gates.cpu()
+
+
+def expert_weights(gen, E, d, f, group, zeros, dt):
+    return {n: [make_w4(gen, r, c, group, zeros, dt) for _ in range(E)] for n, r, c in (("gate", f, d), ("up", f, d), ("down", d, f))}
+
+
+def in64(experts, group):
+    return [torch.stack([weights64(*p, group) for p in experts[n]]) for n in ("gate", "up", "down")]
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+def test_packed_layer_with_activations_near_the_end_of_the_range(cuda, mm, zeros):
+    """A bfloat16 token of 2^123 whose gate and up weights bring it back to ordinary hidden values."""
+    gen = torch.Generator().manual_seed(31)
+    tokens, d, f, E, group, dt = 3, 96, 64, 4, 32, torch.bfloat16
+    x = torch.randn(tokens, d, generator=gen).to(dt)
+    x[1] = 0
+    x[1, 40] = 2.0 ** 123
+    router = torch.randn(E, d, generator=gen).to(dt)
+    router[:, 40] = 0
+    experts = expert_weights(gen, E, d, f, group, zeros, dt)
+    for n in ("gate", "up"):
+        for codes, scales, zps in experts[n]:
+            scales[:, 1] = 2.0 ** -122  # the group of column 40
+            codes[::3, 32:64] = 8 if zps is None else zps[::3, 1:2]  # some rows have no weight there
+    Y, ids, _ = expert_layer(mm, "bf16", x, router, experts, group, 2)
+    y, want_ids, _, bound, _ = moe64(x.double(), router.double(), *in64(experts, group), 2, False)
+    assert torch.equal(ids.long(), want_ids)
+    check16(Y, y, bound, "bf16")
