@@ -198,6 +198,20 @@ static void plan_umma(size_t m, size_t n, size_t k, bool x_tma, int* nt, int* sp
     }
 }
 
+// Packed tiles as 64-bit words: word of a tile, k-tile, row block; one load takes a k-tile of eight row blocks.  (With a row
+// block's tiles as one axis the coordinate of a word would pass 2^31 for k above 1.8e9.)
+static int make_tile_map(CUtensorMap* map, const unsigned char* packed, uint32_t tile_bytes, size_t k_tiles, size_t row_blocks) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return MMBO_ERR_NO_DRIVER_ENTRY;
+  const cuuint64_t dims[3] = {tile_bytes / 8, k_tiles, row_blocks};
+  const cuuint64_t strides[2] = {tile_bytes, k_tiles * tile_bytes};
+  const cuuint32_t box[3] = {tile_bytes / 8, 1, 8}, steps[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_INT64, 3, const_cast<unsigned char*>(packed), dims, strides, box, steps,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MMBO_OK : MMBO_ERR_TENSOR_MAP;
+}
+
 template <typename T, int NT, int QG, bool ZEROS>
 static int launch_w4_umma(UmmaArgs a, cudaStream_t st) {
   using S = UmmaShape<NT>;
@@ -215,14 +229,10 @@ static int launch_w4_umma(UmmaArgs a, cudaStream_t st) {
   const size_t tiles = (a.m + 127) / 128 * (size_t)a.col_tiles;
   if (tiles > 0x3fffffffull) return MMBO_ERR_TOO_LARGE;
   a.tiles = (int)tiles;
-  // packed tiles as 64-bit words: a row block is a row of the map, one load takes a k-tile of eight
   CUtensorMap w_map, map;
   memset(&w_map, 0, sizeof w_map);
   memset(&map, 0, sizeof map);
-  const size_t row_words = w4_k_tiles(a.k) * kTile / 8;
-  if (a.k > 0 && (rc = make_map(&w_map, CU_TENSOR_MAP_DATA_TYPE_INT64, 8, a.packed, row_words, w4_row_blocks(a.m), row_words,
-                                kTile / 8, 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
-    return rc;
+  if (a.k > 0 && (rc = make_tile_map(&w_map, a.packed, kTile, w4_k_tiles(a.k), w4_row_blocks(a.m)))) return rc;
   if (a.x_tma &&
       (rc = make_map(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                      2, a.B, a.k, a.n, a.ldb, 64, NT)))

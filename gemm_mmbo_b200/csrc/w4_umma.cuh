@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
         if (elect_one()) {
           const uint32_t bar = smem_u32(&full_bars[stage]), x = smem + stage * S::kXBytes;
           mbar_expect_tx(bar, 8 * TILE + (a.x_tma ? S::kXBytes : 0));
-          tma_load_2d(codes_at + stage * CODES, &w_map, bar, (t0 + i) * (int)(TILE / 8), row_tile * 8);
+          tma_load_3d(codes_at + stage * CODES, &w_map, bar, 0, t0 + i, row_tile * 8);
           if (a.x_tma) {
             tma_load_2d(x, &x_map, bar, (t0 + i) * kW4Cols, col0);
             tma_load_2d(x + NT * 128, &x_map, bar, (t0 + i) * kW4Cols + 64, col0);

@@ -3,7 +3,7 @@ the ends of a type's range, codes equal to their zero points, results that nearl
 import pytest
 import torch
 
-from low_bit import TYPES, check16, make_w4, moe64, pack, weights64
+from low_bit import TYPES, chain, check16, make_w4, moe64, pack, weights64
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,30 @@ def test_packed_layer_with_activations_near_the_end_of_the_range(cuda, mm, zeros
     y, want_ids, _, bound, _ = moe64(x.double(), router.double(), *in64(experts, group), 2, False)
     assert torch.equal(ids.long(), want_ids)
     check16(Y, y, bound, "bf16")
+
+
+def test_contractions_past_the_32_bit_words_of_a_row_block(cuda, mm):
+    """One row of 1.82e9 weights in groups of 32 with zero points: 2.16e9 64-bit words of packed tiles.  B is zero but for 200
+    places on both sides of word 2^31 and at the ends, so that at most 200 groups' sums are inexact additions."""
+    k, n, group = 1_820_000_000, 9, 32
+    if torch.cuda.mem_get_info()[0] < 60 * 2 ** 30:
+        pytest.skip("needs 60 GB")
+    g, gen = k // group, torch.Generator().manual_seed(3)
+    edge = 2 ** 31 // 152 * 128  # first column of the tile with word 2^31
+    at = torch.cat([torch.arange(a, a + 50) * 3 for a in (0, edge // 3 - 60, edge // 3 + 200, k // 3 - 50)])
+    codes = torch.randint(0, 256, (1, k // 2), dtype=torch.uint8, device="cuda")
+    scales = (0.002 + 0.01 * torch.rand(1, g, device="cuda")).half()
+    zps = torch.randint(0, 16, (1, g), dtype=torch.uint8, device="cuda")
+    packed = torch.empty(mm.w4_bytes(1, k, group, True), dtype=torch.uint8, device="cuda")
+    mm.w4_pack("f16", 1, k, group, codes, k // 2, scales, g, zps, g, packed)
+    x = torch.randn(n, at.numel(), generator=gen).half()
+    B = torch.zeros(n, k, dtype=torch.float16, device="cuda")
+    B[:, at.cuda()] = x.cuda()
+    C = torch.empty(n, 1, dtype=torch.float16, device="cuda")
+    mm.gemm_w4("f16", 1, n, k, 1.0, packed, group, True, B, k, 0.0, C, 1)
+    torch.cuda.synchronize()
+    assert mm.device_status() == 0
+    both, where = codes[0, at.cuda() // 2].cpu(), at // group
+    q = torch.where(at % 2 == 0, both & 15, both >> 4).double()
+    w = (q - zps[0, where.cuda()].cpu().double()) * scales[0, where.cuda()].cpu().double()
+    check16(C[:, 0].cpu(), x.double() @ w, chain(200 * 128) * (x.double().abs() @ w.abs()), "f16")
