@@ -241,8 +241,8 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// acc += a packed tile * two bfloat16 columns' worth (a value and its remainder, by quarters).  Codes become exact integers:
-// for w4_tile_mma a hidden vector would first have to be brought to half precision.
+// acc += a packed tile * two bfloat16 columns' worth (a value and its remainder, by quarters).  Codes become exact integers
+// times 2^-11, see W4Operand: for w4_tile_mma a hidden vector would first have to be brought to half precision.
 template <typename T, int QG>
 __device__ __forceinline__ void tile_multiply_bf16(uint32_t tile, const uint4 (&b)[2][4], bool zeros, float (&acc)[4]) {
   using L = W4Tile<QG, true>;
@@ -250,7 +250,7 @@ __device__ __forceinline__ void tile_multiply_bf16(uint32_t tile, const uint4 (&
   const uint32_t codes = tile + w4_piece(r, lane & 3);
   const uint4 c0 = lds128(codes), c1 = lds128(codes + 512);
   const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
-  W4Unpacker<__nv_bfloat16> lo, hi;
+  W4Operand<__nv_bfloat16> lo, hi;
 #pragma unroll
   for (int g = 0; g < L::kGroups; ++g) {
     const uint32_t z = zeros ? lds16(tile + L::kZeros + g * 16 + r * 2) : 0x0808u;
@@ -705,17 +705,17 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up4_kernel(const MoeArgs a
 }
 
 // ---------------------------------------------------------------- down ----------------
-// Adds an expert's products with the tokens of a group, times their gates, to this warp's sums, [token][row].
+// Adds an expert's products with the tokens of a group, times their gates and `unit`, to this warp's sums, [token][row].
 template <typename U>
 __device__ __forceinline__ void moe_add_products(const MoePlan& plan, float* sums, const int* order, int cols, const float (&acc)[4],
-                                                 const float (&rest)[4]) {
+                                                 const float (&rest)[4], float unit) {
   const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   float v[4], *to[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {  // all read before one is written: a lane's four are different ones
     const int entry = order[min(t * 2 + (i & 1), cols - 1)];
     to[i] = sums + (entry >> 16) * 16 + r + 8 * (i >> 1);
-    v[i] = fmaf(plan.gate[entry & 0xffff], (acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest)) * (1.f / MoeHidden<U>::kScale), *to[i]);
+    v[i] = fmaf(plan.gate[entry & 0xffff] * unit, acc[i] + rest[i] * (1.f / MoeHidden<U>::kRest), *to[i]);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_down16_kernel(const M
         if (FED && lane == 0) mbar_arrive(smem_u32(&empty[stage]));
         move(kTeams);
         ask();
-        moe_add_products<T>(plan, ours, order, cols, acc, rest);
+        moe_add_products<T>(plan, ours, order, cols, acc, rest, 1.f / MoeHidden<T>::kScale);
       }
       moe_store_rows<T>(a, sums, rows);
     }
@@ -958,7 +958,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down4_kernel(const MoeArgs
           phase ^= 1u;
         }
       }
-      moe_add_products<__nv_bfloat16>(plan, ours, plan.order + p0, cols, acc, none);
+      moe_add_products<__nv_bfloat16>(plan, ours, plan.order + p0, cols, acc, none, W4Operand<__nv_bfloat16>::kUnit);
     }
     moe_store_rows<T>(a, sums, rows);
   }

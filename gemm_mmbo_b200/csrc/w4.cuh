@@ -159,11 +159,13 @@ struct W4Unpacker<__half> {
     a[3] = u32(__hfma2(h2(and_or(v, kHighCodes, bias)), c16, h2(z16)));
   }
 };
-template <>
-struct W4Unpacker<__nv_bfloat16> {
+// DOWN: bfloat16 codes come times 2^-DOWN, by another exponent in the same constants.
+template <int DOWN = 0>
+struct W4UnpackerBf16 {
+  static constexpr uint32_t kBias = 0x4300u - (DOWN << 7);
   uint32_t bias, z1;
-  __device__ __forceinline__ W4Unpacker() : bias(in_register(0x43004300u)) {}
-  __device__ __forceinline__ void set_zero(uint32_t z) { z1 = (0x4300u | z) * 0x10001u; }
+  __device__ __forceinline__ W4UnpackerBf16() : bias(in_register(kBias * 0x10001u)) {}
+  __device__ __forceinline__ void set_zero(uint32_t z) { z1 = (kBias | z) * 0x10001u; }
   __device__ __forceinline__ uint32_t one(uint32_t w) const {
     uint32_t x = and_or(w, kLowCodes, bias);
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&z1));
@@ -175,6 +177,21 @@ struct W4Unpacker<__nv_bfloat16> {
     a[2] = one(w >> 4);
     a[3] = one(w >> 12);
   }
+};
+template <>
+struct W4Unpacker<__nv_bfloat16> : W4UnpackerBf16<> {};
+
+// Codes as the products take them, kUnit times too small.  A group's sum of bfloat16 activations could pass the largest float
+// where the scale would bring it back: up to 128 products with differences up to 15, so below 2^11 times the largest
+// activation.  With differences times 2^-11 it cannot; results get the factor back at the end.  What that costs: results
+// below 2^-115 are held to steps of 2^-138 (bfloat16's are 2^-133).
+template <typename T>
+struct W4Operand : W4Unpacker<T> {
+  static constexpr float kUnit = 1.f;
+};
+template <>
+struct W4Operand<__nv_bfloat16> : W4UnpackerBf16<11> {
+  static constexpr float kUnit = 0x1p11f;
 };
 
 // ---------------------------------------------------------------- writing the format --

@@ -3,8 +3,9 @@
 // A block computes 128 rows x NT columns.  The weights never exist in 16 bits outside tensor memory:
 //   warp 0      feeds: TMA loads of the packed tiles (8 row blocks in one) and of the activations (128 x NT) into a ring
 //   warp 1      issues the products: A (the unpacked weights) from tensor memory, B (the activations) from shared memory
-//   unpackers   (4 or 8 warps) turn codes into exact integers q - z in the activations' type and write them to tensor
-//               memory, thread = row; where the activations are not aligned for TMA they bring those, too
+//   unpackers   (4 or 8 warps) turn codes into exact integers q - z (bfloat16: times 2^-11, see W4Operand) in the activations'
+//               type and write them to tensor memory, thread = row; where the activations are not aligned for TMA they bring
+//               those, too
 //   drainers    (4 or 8 warps) take each group's sums out of tensor memory, multiply by the group's scale and add them to
 //               the tile's sums in fp32 registers: the scales never meet a 16-bit rounding
 // Bounds: with few columns the codes' bytes (a 128 x 128 tile is 8.4 KB, 365 cycles of an SM's share of the memory); with
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
         z[g] = 8u;
         if (ZEROS) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z[g]) : "r"(block + L::kZeros + g * 16 + W4Format::slot(r)));
       }
-      W4Unpacker<T> un;
+      W4Operand<T> un;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
       auto store = [&](int col, float v) {
         if (grow < a.m && (size_t)col < a.n) {
           T* c = static_cast<T*>(a.C) + (size_t)col * a.ldc + grow;
-          v *= a.alpha;
+          v = v * a.alpha * W4Operand<T>::kUnit;
           *c = from_f32<T>(a.beta != 0.f ? fmaf(a.beta, to_f32(*c), v) : v);
         }
       };

@@ -80,3 +80,56 @@ def test_contractions_past_the_32_bit_words_of_a_row_block(cuda, mm):
     q = torch.where(at % 2 == 0, both & 15, both >> 4).double()
     w = (q - zps[0, where.cuda()].cpu().double()) * scales[0, where.cuda()].cpu().double()
     check16(C[:, 0].cpu(), x.double() @ w, chain(200 * 128) * (x.double().abs() @ w.abs()), "f16")
+
+
+@pytest.mark.parametrize("n", [1, 8, 9, 70, 300])
+@pytest.mark.parametrize("group", [32, 128])
+def test_group_sums_past_the_largest_float(cuda, mm, n, group):
+    """bfloat16 activations around 2^120 with equal signs and the largest codes: a group's sum of (q - z) x passes 2^128, its
+    product with the scale does not."""
+    gen = torch.Generator().manual_seed(n + group)
+    m, k, dt = 150, 520, torch.bfloat16
+    codes, scales, zps = make_w4(gen, m, k, group, True, dt)
+    codes[::2], zps[::2] = 15, 0
+    x = (torch.randn(n, k, generator=gen).abs() * 2.0 ** 120).to(dt)
+    packed = pack(mm, "bf16", codes, scales, zps, group)
+    C = torch.empty(n, m, dtype=dt, device="cuda")
+    mm.gemm_w4("bf16", m, n, k, 1.0, packed, group, True, x.cuda(), k, 0.0, C, m)
+    w = weights64(codes, scales, zps, group)
+    check16(C.cpu(), x.double() @ w.t(), chain(k) * (x.double().abs() @ w.abs().t()), "bf16")
+
+
+@pytest.mark.parametrize("n", [1, 9, 70])
+def test_results_near_the_smallest_bfloat16(cuda, mm, n):
+    """The other end: results around 2^-126, where a step is 2^-133."""
+    gen = torch.Generator().manual_seed(n)
+    m, k, group, dt = 150, 520, 64, torch.bfloat16
+    codes, scales, zps = make_w4(gen, m, k, group, True, dt)
+    x = (torch.randn(n, k, generator=gen) * 2.0 ** -123).to(dt)
+    packed = pack(mm, "bf16", codes, scales, zps, group)
+    C = torch.empty(n, m, dtype=dt, device="cuda")
+    mm.gemm_w4("bf16", m, n, k, 1.0, packed, group, True, x.cuda(), k, 0.0, C, m)
+    w = weights64(codes, scales, zps, group)
+    # 9 groups and the joints of their sums, each rounded to steps of 2^-138
+    check16(C.cpu(), x.double() @ w.t(), chain(k) * (x.double().abs() @ w.abs().t()) + 30 * 2.0 ** -139, "bf16")
+
+
+def test_packed_hidden_vectors_near_the_end_of_the_range(cuda, mm):
+    """Hidden values of 2^116 and more that down's scales bring back."""
+    gen = torch.Generator().manual_seed(9)
+    tokens, d, f, E, group, dt = 4, 64, 128, 2, 128, torch.bfloat16
+    x = torch.randn(tokens, d, generator=gen).abs().to(dt)
+    router = torch.randn(E, d, generator=gen).to(dt)
+    experts = expert_weights(gen, E, d, f, group, True, dt)
+    for e in range(E):
+        for n, size in (("gate", 2.0 ** 50), ("up", 2.0 ** 50), ("down", 2.0 ** -118)):
+            codes, scales, zps = experts[n][e]
+            scales.fill_(size)
+            zps.fill_(0)
+            codes.clamp_(min=1)
+            if n == "down":
+                codes[::2] = 15
+    Y, ids, _ = expert_layer(mm, "bf16", x, router, experts, group, 1)
+    y, want_ids, _, bound, _ = moe64(x.double(), router.double(), *in64(experts, group), 1, False)
+    assert torch.equal(ids.long(), want_ids)
+    check16(Y, y, bound, "bf16")
