@@ -108,7 +108,6 @@ static int launch_clustered(K kernel, unsigned grid, unsigned threads, size_t sm
 // (B200, us): 0.022 a tile of the busiest SM, 0.3 a slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join
 // clusters of two / four, 1 a batch of row groups.  8192 x 28672, one column: 28.4 us with the chosen 16 x 2, 30.7 with
 // 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
-template <int QG>
 static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3], size_t* smem) {
   const size_t k_tiles = w4_k_tiles(a.k), blocks = w4_row_blocks(a.m);
   double best = 1e30;
@@ -127,11 +126,11 @@ static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3]
       if (cost >= best) continue;
       const size_t ring = (size_t)kGemvWarps * 2 * slot_tiles * tile_bytes;
       const size_t one = gemv_sums_bytes((int)wk, (int)split, a.n, 1);
-      if (ring + one + gemv_x_bytes(a.n, 1, 4 / QG) > kGemvSmem) continue;
-      size_t x_tiles = (kGemvSmem - ring - one - a.n * 64) / (a.n * 256 + (size_t)(4 / QG) * 32);
+      if (ring + one + gemv_x_bytes(a.n, 1) > kGemvSmem) continue;
+      size_t x_tiles = (kGemvSmem - ring - one - a.n * 64) / (a.n * 256);
       if (x_tiles > span) x_tiles = span ? span : 1;
       if (x_tiles == 0) continue;
-      const size_t x = gemv_x_bytes(a.n, x_tiles, 4 / QG);
+      const size_t x = gemv_x_bytes(a.n, x_tiles);
       size_t batch = (kGemvSmem - ring - x) / one;
       if (batch > rounds) batch = rounds;
       if (batch == 0 || (split > 1 && batch < rounds)) continue;
@@ -160,7 +159,7 @@ static int launch_w4_gemv(GemvArgs a, cudaStream_t st) {
   if (rc) return rc;
   const int clusters[3] = {cluster_slots(0), cluster_slots(1), cluster_slots(2)};
   size_t smem = 0;
-  if (!plan_gemv<QG>(a, W4Tile<QG, ZEROS>::kBytes, clusters, &smem)) return MMBO_ERR_TOO_LARGE;
+  if (!plan_gemv(a, W4Tile<QG, ZEROS>::kBytes, clusters, &smem)) return MMBO_ERR_TOO_LARGE;
   return launch_clustered(kernel, (unsigned)a.clusters << a.split_log2, kGemvThreads, smem, a.split_log2, st, a);
 }
 
@@ -270,7 +269,7 @@ static int run_w4_gemm(size_t m, size_t n, size_t k, float alpha, const void* pa
 
 // Workspace of the expert layer, for one pass.
 struct MoeWorkspace {
-  size_t scores, x, x_sums, x_undo, hidden, plan, total;
+  size_t scores, x, hidden, plan, total;
 };
 static MoeWorkspace moe_workspace(size_t tokens, size_t d, size_t f, size_t experts, size_t topk) {
   if (tokens > (size_t)moe_pass_tokens((int)topk)) tokens = moe_pass_tokens((int)topk);
@@ -278,9 +277,7 @@ static MoeWorkspace moe_workspace(size_t tokens, size_t d, size_t f, size_t expe
   MoeWorkspace w;
   w.scores = 0;
   w.x = w.scores + align_up(tokens * experts * 4, 256);
-  w.x_sums = w.x + align_up(tokens * align_up(d, 128) * 2, 256);
-  w.x_undo = w.x_sums + align_up(tokens * (align_up(d, 128) / 32) * 4, 256);
-  w.hidden = w.x_undo + align_up(tokens * 8, 256);
+  w.hidden = w.x + align_up(tokens * align_up(d, 128) * 2, 256);
   w.plan = w.hidden + align_up(pairs * align_up(f, 128) * 4, 256);
   w.total = w.plan + align_up((size_t)MoePlan::words((int)experts, (int)pairs) * 4, 256);
   return w;
@@ -551,8 +548,6 @@ int mmbo_moe(int dtype, size_t tokens, size_t d, size_t f, size_t experts, size_
     a.gates = gates ? gates + t0 * topk : nullptr;
     a.scores = reinterpret_cast<float*>(base + ws.scores);
     a.x = base + ws.x;
-    a.x_sums = reinterpret_cast<float*>(base + ws.x_sums);
-    a.x_undo = reinterpret_cast<float2*>(base + ws.x_undo);
     a.hidden = base + ws.hidden;
     a.plan = reinterpret_cast<int*>(base + ws.plan);
     a.d_pad = (int)align_up(d, 128);

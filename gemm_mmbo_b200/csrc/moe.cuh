@@ -8,8 +8,7 @@
 //
 // What bounds it: the bytes of the experts that the tokens choose, and for one token the chain of three kernels.  They run in
 // one stream, each started while the one in front drains (programmatic dependent launch):
-//   scores   one warp per (token, expert); also an aligned, zero-padded copy of the activations (for 4-bit experts in half
-//            precision with the groups' sums, as w4_tile_mma wants them)
+//   scores   one warp per (token, expert); also an aligned, zero-padded copy of the activations
 //   up       every block repeats the selection for itself (one to eight microseconds, cheaper than another kernel and its
 //            launch), then its share of the units (expert, 16 rows of gate and up, group of up to eight tokens)
 //   down     a block owns 16 rows of the output for all tokens, its warps split the list of (expert, part of f); the sums
@@ -47,9 +46,7 @@ struct MoeArgs {
   float* gates;  // tokens x topk, the caller's or null
   // workspace
   float* scores;    // tokens x experts
-  void* x;          // tokens x d_pad: the activations, zero behind d (4-bit experts: in half precision, scaled)
-  float* x_sums;    // 4-bit experts: tokens x (d_pad / group) sums of these, in units of 2^20
-  float2* x_undo;   // 4-bit experts: two factors a token that undo its scale and the unit of 2^20
+  void* x;          // tokens x d_pad: the activations, zero behind d
   void* hidden;     // pairs x 2 x f_pad, zero behind f: hidden vectors as a 16-bit value and what its rounding left, see MoeHidden
   int* plan;        // what `up` found out for `down`, see MoePlan
   int d_pad, f_pad; // multiples of 128
@@ -91,10 +88,7 @@ __device__ __forceinline__ uint32_t moe_score_key(float v) {
 
 template <typename T>
 __global__ void __launch_bounds__(256) moe_scores_kernel(const MoeArgs a) {
-  __shared__ uint32_t peak;
   griddep_launch_dependents();
-  if (threadIdx.x == 0) peak = 0;
-  __syncthreads();
   griddep_wait();
   const int t = blockIdx.y, lane = threadIdx.x & 31;
   const T* x = static_cast<const T*>(a.X) + (size_t)t * a.ldx;
@@ -102,56 +96,8 @@ __global__ void __launch_bounds__(256) moe_scores_kernel(const MoeArgs a) {
     uint16_t* h = static_cast<uint16_t*>(a.hidden) + (size_t)t * a.topk * a.f_pad * 2;
     const int pad = a.f_pad - a.f;
     for (int i = threadIdx.x; i < a.topk * 2 * pad; i += 256) h[(size_t)(i / pad) * a.f_pad + a.f + i % pad] = 0;
-    if (!a.fmt.group) {
-      T* copy = static_cast<T*>(a.x) + (size_t)t * a.d_pad;
-      for (int j = threadIdx.x * 8; j < a.d_pad; j += 256 * 8) *reinterpret_cast<uint4*>(copy + j) = load8(x, a.d, j);
-      return;
-    }
-    float f1 = 1.f, f2 = 1.f;
-    if (!std::is_same<T, __half>::value) {
-      // exponent of the largest magnitude (below the normal range: the smallest normal one), 2^(14 - e) as a product
-      uint32_t top = 0;
-      for (int j = threadIdx.x * 8; j < a.d; j += 256 * 8) {
-        const uint4 v = load8(x, a.d, j);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max(w[i] << 16 & 0x7fffffffu, w[i] & 0x7fff0000u));
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) atomicMax(&peak, top);
-      __syncthreads();
-      const int up = 14 - ((int)max(peak >> 23, 1u) - 127), up1 = min(max(up, -100), 100), up2 = up - up1;
-      f1 = __uint_as_float((uint32_t)(up1 + 127) << 23);
-      f2 = __uint_as_float((uint32_t)(up2 + 127) << 23);
-      if (threadIdx.x == 0)
-        a.x_undo[t] = peak < 0x7f800000u ? make_float2(__uint_as_float((uint32_t)(127 - up1) << 23),
-                                                       __uint_as_float((uint32_t)(127 - up2 + 20) << 23))
-                                         : make_float2(__int_as_float(0x7fc00000), 0.f);
-    } else if (threadIdx.x == 0) {
-      a.x_undo[t] = make_float2(1.f, 0x1p20f);
-    }
-    __half* copy = static_cast<__half*>(a.x) + (size_t)t * a.d_pad;
-    const int lanes = a.fmt.group / 8;  // neighbouring threads that hold a group
-    for (int j0 = 0; j0 < a.d_pad; j0 += 256 * 8) {
-      const int j = j0 + threadIdx.x * 8;
-      const uint4 v = load8(x, a.d, j);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      uint32_t out[4];
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 e = widen2<T>(w[i]);
-        const __half2 c = __floats2half2_rn(e.x * f1 * f2, e.y * f1 * f2);
-        out[i] = *reinterpret_cast<const uint32_t*>(&c);
-        const float2 back = __half22float2(c);
-        sum += back.x + back.y;
-      }
-      for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (j < a.d_pad) {
-        *reinterpret_cast<uint4*>(copy + j) = make_uint4(out[0], out[1], out[2], out[3]);
-        if (threadIdx.x % lanes == 0) a.x_sums[(size_t)t * (a.d_pad / a.fmt.group) + j / a.fmt.group] = sum * 0x1p-20f;
-      }
-    }
+    T* copy = static_cast<T*>(a.x) + (size_t)t * a.d_pad;
+    for (int j = threadIdx.x * 8; j < a.d_pad; j += 256 * 8) *reinterpret_cast<uint4*>(copy + j) = load8(x, a.d, j);
     return;
   }
   const int e = blockIdx.x * 8 + threadIdx.x / 32;
@@ -224,56 +170,7 @@ __device__ __forceinline__ void moe_select(const MoeArgs& a, const float* from, 
   if (lane < a.topk) gates[lane] = a.renorm ? p / chosen : p;
 }
 
-// ---------------------------------------------------------------- fragments -----------
-template <typename T>
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1);
-template <>
-__device__ __forceinline__ void mma_16816<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                  uint32_t b0, uint32_t b1) {
-  mma_f16(c, a0, a1, a2, a3, b0, b1);
-}
-template <>
-__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                         uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// acc += a packed tile * two bfloat16 columns' worth (a value and its remainder, by quarters).  Codes become exact integers
-// times 2^-11, see W4Operand: for w4_tile_mma a hidden vector would first have to be brought to half precision.
-template <typename T, int QG>
-__device__ __forceinline__ void tile_multiply_bf16(uint32_t tile, const uint4 (&b)[2][4], bool zeros, float (&acc)[4]) {
-  using L = W4Tile<QG, true>;
-  const int lane = threadIdx.x & 31, r = lane >> 2;
-  const uint32_t codes = tile + w4_piece(r, lane & 3);
-  const uint4 c0 = lds128(codes), c1 = lds128(codes + 512);
-  const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
-  W4Operand<__nv_bfloat16> lo, hi;
-#pragma unroll
-  for (int g = 0; g < L::kGroups; ++g) {
-    const uint32_t z = zeros ? lds16(tile + L::kZeros + g * 16 + r * 2) : 0x0808u;
-    lo.set_zero(z & 15u);
-    hi.set_zero(z >> 8 & 15u);
-    float part[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (int qq = 0; qq < QG; ++qq) {
-      const int q = g * QG + qq;
-      uint32_t p[4], s[4];
-      lo.unpack(w0[q], p);
-      hi.unpack(w1[q], s);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mma_16816<__nv_bfloat16>(part[i], p[0], s[0], p[1], s[1], b[i][q].x, b[i][q].y);
-        mma_16816<__nv_bfloat16>(part[i], p[2], s[2], p[3], s[3], b[i][q].z, b[i][q].w);
-      }
-    }
-    const float2 s = widen2<T>(lds32(tile + L::kScales + g * 32 + r * 4));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(i < 2 ? s.x : s.y, part[0][i] + part[1][i], acc[i]);
-  }
-}
+// ---------------------------------------------------------------- hidden vectors ------
 // Hidden vectors as products take them: a 16-bit value and what its rounding left, so that 16 bits and more survive.
 // bfloat16 has the range of a float.  Half precision holds h / 64 and 2^11 times the remainder: magnitudes up to 4.19e6,
 // steps of 2^-30 near zero (results in half precision have steps of 2^-24).
@@ -391,11 +288,11 @@ __device__ __forceinline__ void moe_store_hidden(const MoeArgs& a, int pair, int
 }
 
 // ---------------------------------------------------------------- up ------------------
-// Joins a unit's sums, [warp][gate, up][column][row] of `warps` warps at `sums`, and stores the hidden values; thread i of
-// those that share the unit.
+// Joins a unit's sums, [warp][gate, up][column][row] of `warps` warps at `sums`, `unit` times too small, and stores the hidden
+// values; thread i of those that share the unit.
 template <typename U>
 __device__ __forceinline__ void moe_finish_unit(const MoeArgs& a, const float* sums, int warps, int i, int cols, int rows,
-                                                const int* order, bool packed) {
+                                                const int* order, float unit) {
   if (i >= cols * 16) return;
   float g = 0.f, u = 0.f;
   for (int w = 0; w < warps; w += 4) {
@@ -405,13 +302,7 @@ __device__ __forceinline__ void moe_finish_unit(const MoeArgs& a, const float* s
       u += sums[(w + v) * 256 + 128 + i];
     }
   }
-  const int entry = order[i / 16];
-  if (packed) {
-    const float2 undo = a.x_undo[entry >> 16];  // one after the other: their product may pass the largest float
-    g = g * undo.x * undo.y;
-    u = u * undo.x * undo.y;
-  }
-  moe_store_hidden<U>(a, entry & 0xffff, rows * 16 + (i & 15), g, u);
+  moe_store_hidden<U>(a, order[i / 16] & 0xffff, rows * 16 + (i & 15), g * unit, u * unit);
 }
 __device__ __forceinline__ void moe_keep_sums(float* to, const float (&gate)[4], const float (&up)[4]) {
   const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
@@ -582,7 +473,7 @@ __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const Moe
       if (lane == 0) mbar_arrive(smem_u32(&sums_full[which]));
       if (((n + 1) * chunks - 1) % kTeams == team) {
         if (ok) ok = mbar_wait_together(smem_u32(&sums_full[which]), parity, &abort_flag, kFaultWaitFull, 0x4d03u);
-        moe_finish_unit<T>(a, ours, kMoeWarps, member * 32 + lane, cols, unit.rows, plan.order + p0, false);
+        moe_finish_unit<T>(a, ours, kMoeWarps, member * 32 + lane, cols, unit.rows, plan.order + p0, 1.f);
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sums_free[which]));
       }
@@ -601,7 +492,6 @@ constexpr int kMoeTiles = 2, kMoeSlots = 2;
 
 template <typename T, int QG>
 __global__ void __launch_bounds__(kMoeThreads, 1) moe_up4_kernel(const MoeArgs a) {
-  constexpr int G = 4 / QG;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) unsigned long long full_bars[kMoeWarps * kMoeSlots];
   __shared__ uint32_t abort_flag;
@@ -659,29 +549,22 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up4_kernel(const MoeArgs a
   bool ok = true;
   int slot = 0;
   uint32_t phase = 0;
-  const int per = a.d_pad / (32 * QG);
   for (int n = begin; n < end; ++n) {
     const int p0 = plan.start[unit.index] + unit.group * 8, cols = min(8, plan.start[unit.index + 1] - p0);
     // columns past the last token repeat it; their sums are not used
-    const uint16_t* x = static_cast<const uint16_t*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] >> 16) * a.d_pad +
-                        s0 * 128 + t * 8;
-    const float* sums0 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t, cols - 1)] >> 16) * per + s0 * G;
-    const float* sums1 = a.x_sums + (size_t)(plan.order[p0 + min(2 * t + 1, cols - 1)] >> 16) * per + s0 * G;
+    const T* x = static_cast<const T*>(a.x) + (size_t)(plan.order[p0 + min(r, cols - 1)] >> 16) * a.d_pad + s0 * 128 + t * 8;
     float gate[4] = {0.f, 0.f, 0.f, 0.f}, up[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s = s0; s < s1; s += kMoeTiles) {
       const int cnt = min(kMoeTiles, s1 - s);
       uint32_t at = ring + slot * slot_bytes;
       for (int i = 0; i < cnt; ++i) {
         uint4 b[4];
-        float2 xs[G];
 #pragma unroll
         for (int q = 0; q < 4; ++q) b[q] = *reinterpret_cast<const uint4*>(x + q * 32);
-#pragma unroll
-        for (int g = 0; g < G; ++g) xs[g] = make_float2(*sums0++, *sums1++);
         x += 128;
         if (i == 0 && ok) ok = mbar_wait_together(full + slot * 8, phase, &abort_flag, kFaultWaitFull, 0x4d10u + warp);
-        w4_tile_mma<T, QG>(at, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, gate);
-        w4_tile_mma<T, QG>(at + half, [&](int q) { return b[q]; }, [&](int g) { return xs[g]; }, a.fmt.zeros, up);
+        w4_tile_mma<T, T, QG>(at, [&](int, int q) { return b[q]; }, a.fmt.zeros, gate);
+        w4_tile_mma<T, T, QG>(at + half, [&](int, int q) { return b[q]; }, a.fmt.zeros, up);
         at += tile_bytes;
       }
       __syncwarp();
@@ -695,7 +578,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up4_kernel(const MoeArgs a
     moe_keep_sums(ours + wk * 256, gate, up);
     asm volatile("bar.sync %0, %1;" ::"r"(2 + team), "r"(WK * 32) : "memory");
     moe_finish_unit<__nv_bfloat16>(a, ours, WK, (wk * 32 + lane + 384 * (n & 3)) & (WK * 32 - 1), cols, unit.rows,
-                                   plan.order + p0, true);
+                                   plan.order + p0, W4Operand<T>::kUnit);
     unit.advance(plan, blocks);
   }
   if (!ok) {  // a wait ran out: give the copies still in flight time to land
@@ -948,7 +831,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_down4_kernel(const MoeArgs
           }
           h += 128;
           if (i == 0 && ok) ok = mbar_wait_together(full + slot * 8, phase, &abort_flag, kFaultWaitFull, 0x4d30u + warp);
-          tile_multiply_bf16<T, QG>(tile, b, a.fmt.zeros, acc);
+          w4_tile_mma<__nv_bfloat16, T, QG, 2>(tile, [&](int i, int q) { return b[i][q]; }, a.fmt.zeros, acc);
           tile += tile_bytes;
         }
         __syncwarp();

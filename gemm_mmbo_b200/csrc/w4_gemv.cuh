@@ -26,28 +26,35 @@
 namespace mmbo {
 
 
-// c (16 x 8) = a (16 x 16) * b (16 x 8) + c (or + 0), fp32 sums.
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// c (16 x 8) = a (16 x 16) * b (16 x 8) + c (or + 0), fp32 sums, operands of type T.
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16_from_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                  uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+template <typename T>
+__device__ __forceinline__ void mma_16816_from_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                    uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
@@ -60,49 +67,48 @@ __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
-// acc += the products of a tile with 128 rows of 8 columns: b(q) is this lane's 16 bytes of quarter q of its column, xs(g)
-// the sums of group g of the columns 2 t and 2 t + 1.  Sums are in units of 2^20.
+// acc += the products of a tile with 128 rows of 8 columns, PARTS of them added (a vector kept as a value and its remainder):
+// column(i, q) is this lane's 16 bytes of quarter q of its column in part i.  U: type of the columns, T: of the scales.  Sums
+// are W4Operand<U>::kUnit times too small.
 //
-// A code is used as the bits of a half-precision number: q in the lowest four bits is the subnormal q 2^-24, q in the
-// next four is q 2^-20, both exact, so a word becomes four operand registers with a shift and four masks.  The two kinds
-// have a sum each, and the zero point comes off once a group:  sum (q - z) x = sum q x - z sum x.  (Forming the sums of
-// x with the same instruction and a matrix of ones made the tensor pipe the bound: 16 instructions a tile, 32 cycles;
-// subtracting the zero point from each code costs as much again as unpacking it.)
-template <typename T, int QG, typename Columns, typename Sums>
-__device__ __forceinline__ void w4_tile_mma(uint32_t tile, Columns column, Sums sums, bool zeros, float (&acc)[4]) {
+// Every code becomes the exact difference q - z before it is multiplied, so that an error is measured by the terms
+// |q - z| |x| of the formula: a large activation at a weight of zero drops out.  (Taking z times the sum of x off a group's
+// sum of q x saves four of nine instructions a word, but leaves that activation's rounding behind.)
+template <typename U, typename T, int QG, int PARTS = 1, typename Columns>
+__device__ __forceinline__ void w4_tile_mma(uint32_t tile, Columns column, bool zeros, float (&acc)[4]) {
   using L = W4Tile<QG, true>;  // (where there are zero points does not depend on whether there are)
   const int lane = threadIdx.x & 31, r = lane >> 2;
   const uint32_t codes = tile + w4_piece(r, lane & 3);
   const uint4 c0 = lds128(codes), c1 = lds128(codes + 512);  // rows r and r + 8
   const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+  W4Operand<U> lo, hi;
 #pragma unroll
   for (int g = 0; g < L::kGroups; ++g) {
-    float low[4], high[4];
+    const uint32_t z = zeros ? lds16(tile + L::kZeros + g * 16 + r * 2) : 0x0808u;
+    lo.set_zero(z & 15u);
+    hi.set_zero(z >> 8 & 15u);
+    float part[PARTS][4];
 #pragma unroll
     for (int qq = 0; qq < QG; ++qq) {
       const int q = g * QG + qq;
-      const uint32_t v0 = w0[q] >> 8, v1 = w1[q] >> 8;
-      const uint4 b = column(q);
-      if (qq == 0) {
-        mma_f16_from_zero(low, w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
-        mma_f16_from_zero(high, w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
-      } else {
-        mma_f16(low, w0[q] & kLowCodes, w1[q] & kLowCodes, v0 & kLowCodes, v1 & kLowCodes, b.x, b.y);
-        mma_f16(high, w0[q] & kHighCodes, w1[q] & kHighCodes, v0 & kHighCodes, v1 & kHighCodes, b.z, b.w);
+      uint32_t p[4], s[4];
+      lo.unpack(w0[q], p);
+      hi.unpack(w1[q], s);
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        const uint4 b = column(i, q);
+        if (qq == 0) mma_16816_from_zero<U>(part[i], p[0], s[0], p[1], s[1], b.x, b.y);
+        else mma_16816<U>(part[i], p[0], s[0], p[1], s[1], b.x, b.y);
+        mma_16816<U>(part[i], p[2], s[2], p[3], s[3], b.z, b.w);
       }
     }
     const float2 s = widen2<T>(lds32(tile + L::kScales + g * 32 + r * 4));
-    float z0 = 8.f, z1 = 8.f;
-    if (zeros) {
-      const uint32_t z = lds16(tile + L::kZeros + g * 16 + r * 2);
-      z0 = (float)(z & 15u);
-      z1 = (float)((z >> 8) & 15u);
-    }
-    const float2 xs = sums(g);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float dot = fmaf(16.f, low[i], high[i]);
-      acc[i] = fmaf(i < 2 ? s.x : s.y, fmaf(i < 2 ? -z0 : -z1, i & 1 ? xs.y : xs.x, dot), acc[i]);
+      float sum = part[0][i];
+#pragma unroll
+      for (int j = 1; j < PARTS; ++j) sum += part[j][i];
+      acc[i] = fmaf(i < 2 ? s.x : s.y, sum, acc[i]);
     }
   }
 }
@@ -112,105 +118,6 @@ constexpr int kGemvThreads = (kGemvWarps + 1) * 32;  // and one that feeds them
 constexpr int kGemvMaxSlots = 4;
 // Barrier of the multiplying warps.
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kGemvWarps * 32) : "memory"); }
-
-// What w4_tile_mma reads: `n` columns of `tiles` k-tiles in half precision and the sums of every group in the codes' units
-// of 2^-20.  Half-precision columns are used as they came.  A bfloat16 column is scaled by the power of two that brings
-// its largest magnitude into [2^14, 2^15); this is exact but for elements 2^-38 of that magnitude and less, whose
-// rounding is far below the last bit of any fp32 sum they enter, and one tile product serves both types.  The sums get
-// their true size again by two factors a column; those of a bfloat16 column with an infinity or a NaN are NaN, so that
-// they are noticed.
-//   xs: the columns as they came, x_stride bytes apart; sums: [tile][group][8] floats; peak: bits of the largest
-//   magnitudes (bfloat16), zero before the call.
-template <typename T, int QG>
-__device__ __forceinline__ void w4_stage(int n, int tiles, unsigned char* xs, uint32_t x_stride, float* sums,
-                                         uint32_t* peak, float2* undo) {
-  constexpr bool kScale = !std::is_same<T, __half>::value;
-  constexpr int kLanes = 4 * QG;  // pieces of 16 bytes in a group, held by as many neighbouring lanes
-  const int pieces = tiles * 16, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-  const int strips = (pieces + 63) / 64;  // a warp takes 64 pieces of a column at a time
-  if (kScale) {
-    for (int i = warp; i < strips * n; i += kGemvWarps) {
-      const int col = i / strips, piece = i % strips * 64 + lane;
-      uint32_t top = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (piece + 32 * h < pieces) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(xs + col * x_stride + (piece + 32 * h) * 16);
-          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top = max(top, max(w[j] << 16 & 0x7fffffffu, w[j] & 0x7fff0000u));
-        }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) atomicMax(&peak[col], top);
-    }
-    workers_sync();
-  }
-  for (int i = warp; i < strips * n; i += kGemvWarps) {
-    const int col = i / strips, first = i % strips * 64 + lane;
-    float f1 = 1.f, f2 = 1.f;
-    if (kScale) {
-      // exponent of the largest magnitude (below the normal range: the smallest normal one), 2^(14 - e) as a product
-      const uint32_t top = peak[col];
-      const int up = 14 - ((int)max(top >> 23, 1u) - 127), up1 = min(max(up, -100), 100), up2 = up - up1;
-      f1 = __uint_as_float((uint32_t)(up1 + 127) << 23);
-      f2 = __uint_as_float((uint32_t)(up2 + 127) << 23);
-      if (i % strips == 0 && lane == 0)
-        undo[col] = top < 0x7f800000u ? make_float2(__uint_as_float((uint32_t)(127 - up1) << 23),
-                                                    __uint_as_float((uint32_t)(127 - up2 + 20) << 23))
-                                      : make_float2(__int_as_float(0x7fc00000), 0.f);
-    }
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int piece = first + 32 * h;
-      if (piece < pieces) {
-        uint4* at = reinterpret_cast<uint4*>(xs + col * x_stride + piece * 16);
-        const uint4 raw = *at;
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        uint32_t out[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float2 v = widen2<T>(w[j]);
-          if (kScale) {
-            const __half2 h2 = __floats2half2_rn(v.x * f1 * f2, v.y * f1 * f2);
-            out[j] = *reinterpret_cast<const uint32_t*>(&h2);
-            v = __half22float2(h2);
-          }
-          sum[h] += v.x + v.y;
-        }
-        if (kScale) *at = make_uint4(out[0], out[1], out[2], out[3]);
-      }
-    }
-#pragma unroll
-    for (int x = 1; x < kLanes; x <<= 1) {
-      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], x);
-      sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], x);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int piece = first + 32 * h;
-      if (piece < pieces && (piece & (kLanes - 1)) == 0) sums[piece / kLanes * 8 + col] = sum[h] * 0x1p-20f;
-    }
-  }
-  workers_sync();
-}
-
-// Sum over k of row i times the column x, element by element.
-template <typename T>
-__device__ __noinline__ float w4_slow_dot(const unsigned char* __restrict__ packed, W4Format f, size_t i, size_t k,
-                                          const T* __restrict__ x) {
-  const size_t tiles = w4_k_tiles(k);
-  const int row = (int)(i % kW4Rows);
-  float acc = 0.f;
-  for (size_t j = 0; j < k; ++j) {
-    const unsigned char* in = packed + (i / kW4Rows * tiles + j / kW4Cols) * f.tile_bytes();
-    const int c = (int)(j % kW4Cols), g = c / f.group;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(in + w4_piece(row, c % 32 / 8) + c / 32 * 4);
-    const int q = (w >> (4 * w4_nibble(c % 8))) & 15u, z = f.zeros ? in[f.zero_at(g, row)] : 8;
-    acc = fmaf((float)(q - z) * to_f32(*reinterpret_cast<const T*>(in + f.scale_at(g, row))), to_f32(x[j]), acc);
-  }
-  return acc;
-}
 
 // Untiled bulk copy, completion on an mbarrier of this CTA (addresses and size multiples of 16 bytes), and the request
 // to have the bytes brought into L2.
@@ -274,10 +181,8 @@ struct GemvArgs {
   int clusters;
 };
 
-// Staged columns with their group sums (groups: in a tile).
-__host__ __device__ inline size_t gemv_x_bytes(size_t n, size_t tiles, int groups) {
-  return n * (tiles * 256 + 64) + tiles * groups * 32;
-}
+// Staged columns.
+__host__ __device__ inline size_t gemv_x_bytes(size_t n, size_t tiles) { return n * (tiles * 256 + 64); }
 // Partial sums of a batch of row groups, and the room for what the other blocks of a cluster hand over.
 __host__ __device__ inline size_t gemv_sums_bytes(int wk, int split, size_t n, int batch) {
   const size_t out = (size_t)batch * (kGemvWarps / wk) * kW4Rows * n;
@@ -287,14 +192,11 @@ __host__ __device__ inline size_t gemv_sums_bytes(int wk, int split, size_t n, i
 template <typename T, int QG, bool ZEROS>
 __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs a) {
   constexpr uint32_t TILE = W4Tile<QG, ZEROS>::kBytes;
-  constexpr bool kScale = !std::is_same<T, __half>::value;
-  constexpr int G = 4 / QG, kWorkers = kGemvWarps * 32;
+  constexpr int kWorkers = kGemvWarps * 32;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) unsigned long long full_bars[kGemvWarps * kGemvMaxSlots], empty_bars[kGemvWarps * kGemvMaxSlots];
   __shared__ __align__(8) unsigned long long x_bar;
   __shared__ uint32_t abort_flag;
-  __shared__ uint32_t peak[8];
-  __shared__ float2 undo[8];
   const int split = 1 << a.split_log2, rank = blockIdx.x & (split - 1), first = blockIdx.x >> a.split_log2;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
   const int WK = 1 << a.wk_log2, WM = kGemvWarps >> a.wk_log2;
@@ -304,12 +206,11 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
   const int groups = (row_blocks + WM - 1) / WM;
   const int mine = first < groups ? (groups - first + a.clusters - 1) / a.clusters : 0;  // row groups of this cluster
 
-  // shared memory: rings | activations | their group sums | partial sums | sums from the cluster
+  // shared memory: rings | activations | partial sums | sums from the cluster
   const uint32_t slot_bytes = a.slot_tiles * TILE;
   unsigned char* xs = smem + (size_t)kGemvWarps * a.slots * slot_bytes;
   const uint32_t x_stride = a.x_tiles * 256 + 64;  // columns 64 bytes out of step: conflict-free 16-byte reads
-  float* xsums = reinterpret_cast<float*>(xs + (size_t)n * x_stride);
-  float* sums = xsums + a.x_tiles * G * 8;
+  float* sums = reinterpret_cast<float*>(xs + (size_t)n * x_stride);
   float* received = sums + (size_t)a.batch * kGemvWarps * kW4Rows * n;
 
   if (threadIdx.x == 0) {
@@ -347,7 +248,6 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
     const size_t k0 = (size_t)(t0 + chunk0) * kW4Cols;
     const int pieces = min(span - chunk0, a.x_tiles) * 16;  // of 16 bytes in a column
     const int whole = x_bulk ? (int)min((size_t)pieces, (a.k - min(a.k, k0)) / 8) : 0;
-    if (kScale && threadIdx.x < n) peak[threadIdx.x] = 0;
     if (x_bulk && threadIdx.x == 0) {
       mbar_expect_tx(smem_u32(&x_bar), n * whole * 16);
       for (int col = 0; col < n && whole > 0; ++col)
@@ -416,7 +316,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
 
   bool ok = true;
   // columns past n repeat the last one; their sums are not stored
-  const uint32_t x_lane = smem_u32(xs) + min(r, n - 1) * x_stride + t * 16, xsum_lane = smem_u32(xsums) + t * 8;
+  const uint32_t x_lane = smem_u32(xs) + min(r, n - 1) * x_stride + t * 16;
   for (int batch0 = 0; batch0 < mine; batch0 += a.batch) {
     const int batch_end = min(mine, batch0 + a.batch);
     for (int chunk0 = 0; chunk0 < span || chunk0 == 0; chunk0 += a.x_tiles) {
@@ -428,7 +328,6 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
         if (x_bulk && ok) ok = mbar_wait_asleep(smem_u32(&x_bar), x_phase, &abort_flag, kFaultWaitCLoad, 0x4b10u);
         x_phase ^= 1u;
         workers_sync();
-        w4_stage<T, QG>(n, min(span - chunk0, a.x_tiles), xs, x_stride, xsums, peak, undo);
       }
       const int w0 = part_of(chunk0, wk), w1 = part_of(chunk0, wk + 1);
       for (int g = batch0; g < batch_end; ++g) {
@@ -437,14 +336,11 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
           if (ok) ok = mbar_wait_asleep(full0 + slot * 8, phase, &abort_flag, kFaultWaitFull, 0x4b00u + warp);
           const int cnt = min(a.slot_tiles, w1 - tile);
           uint32_t at = ring_at + slot * slot_bytes, x = x_lane + (tile - chunk0) * 256;
-          uint32_t xsum = xsum_lane + (tile - chunk0) * (G * 32);
 #pragma unroll 2
           for (int i = 0; i < cnt; ++i) {
-            w4_tile_mma<T, QG>(at, [&](int q) { return lds128(x + q * 64); }, [&](int g) { return lds_f2(xsum + g * 32); },
-                               ZEROS, acc);
+            w4_tile_mma<T, T, QG>(at, [&](int, int q) { return lds128(x + q * 64); }, ZEROS, acc);
             at += TILE;
             x += 256;
-            xsum += G * 32;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(empty0 + slot * 8);
@@ -460,8 +356,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
           const int col = t * 2 + (i & 1), row = r + 8 * (i >> 1);
           if (col < n) {
             float* o = out + col * kW4Rows + row;
-            const float v = kScale ? acc[i] * undo[col].x * undo[col].y : acc[i] * 0x1p20f;
-            *o = chunk0 == 0 ? v : *o + v;
+            *o = chunk0 == 0 ? acc[i] : *o + acc[i];
           }
         }
       }
@@ -482,10 +377,8 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
       const int g = group_block >> (4 - a.wk_log2), b = group_block & (WM - 1);
       const size_t grow = ((size_t)(first + (batch0 + g) * a.clusters) * WM + b) * kW4Rows + row;
       if (grow >= a.m) return;
-      if (!(fabsf(v) < INFINITY))  // infinities or NaNs among the operands, which the split sums may have turned around
-        v = w4_slow_dot(a.packed, W4Format{32 * QG, ZEROS}, grow, a.k, static_cast<const T*>(a.B) + col * a.ldb);
       T* c = static_cast<T*>(a.C) + col * a.ldc + grow;
-      v *= a.alpha;
+      v = v * a.alpha * W4Operand<T>::kUnit;
       *c = from_f32<T>(a.beta != 0.f ? fmaf(a.beta, to_f32(*c), v) : v);
     };
     // thread i: row i % 16 of the units i / 16, i / 16 + 32, ...; unit = group_block * n + column, kept without divisions

@@ -341,9 +341,9 @@ int mmbo_w4_unpack(int dtype, size_t m, size_t k, int group, int zeros, const vo
                    size_t ldw, void* stream);
 
 /* C = alpha * W * B + beta * C with W packed, B k x n (ldb >= k), C m x n (ldc >= m), any n: one
- * token's vector, a decoding batch, a prompt.  Codes enter the products as exact integers and each
- * group's sum is scaled in fp32, so the result differs from the formula by fp32 summation and the
- * final rounding only.  C must not overlap B or packed. */
+ * token's vector, a decoding batch, a prompt.  Codes enter the products as exact differences q - z and
+ * each group's sum is scaled in fp32, so the result differs from the formula by fp32 summation (of the
+ * terms (q - z) s B, for any n) and the final rounding only.  C must not overlap B or packed. */
 int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, const float* alpha, const void* packed,
                  int group, int zeros, const void* B, size_t ldb, const float* beta, void* C, size_t ldc,
                  void* stream);

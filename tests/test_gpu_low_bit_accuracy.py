@@ -133,3 +133,97 @@ def test_packed_hidden_vectors_near_the_end_of_the_range(cuda, mm):
     y, want_ids, _, bound, _ = moe64(x.double(), router.double(), *in64(experts, group), 1, False)
     assert torch.equal(ids.long(), want_ids)
     check16(Y, y, bound, "bf16")
+
+
+LOUD = [("f16", 60000.0), ("bf16", 2.0 ** 17), ("bf16", 2.0 ** 30), ("bf16", 2.0 ** 120)]
+
+
+@pytest.mark.parametrize("dtype,loud", LOUD)
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_loud_activations_at_weights_of_zero(cuda, mm, dtype, loud, group, zeros):
+    """A weight whose code is its zero point is zero: what it meets drops out, however large.  The same columns give the same
+    accuracy alone, in a call of 8 and in one of 9, and rows of zeros give zeros."""
+    gen = torch.Generator().manual_seed(group)
+    m, k, dt = 150, 1100, TYPES[dtype]
+    codes, scales, zps = make_w4(gen, m, k, group, zeros, dt)
+    for j in (3, 700, k - 1):
+        codes[:, j] = 8 if zps is None else zps[:, j // group]
+    for i in (0, 77, m - 1):
+        codes[i] = 8 if zps is None else zps[i, torch.arange(k) // group]
+    packed = pack(mm, dtype, codes, scales, zps, group)
+    w = weights64(codes, scales, zps, group)
+    x = torch.randn(70, k, generator=gen).to(dt)
+    x[:, 3], x[::2, 700], x[1::2, k - 1] = loud, -loud, loud
+    for n in (1, 2, 8, 9, 33, 70):
+        C = torch.full((n, m), float("nan"), dtype=dt, device="cuda")
+        mm.gemm_w4(dtype, m, n, k, 1.0, packed, group, zeros, x.cuda(), k, 0.0, C, m)
+        check16(C.cpu(), x[:n].double() @ w.t(), chain(k) * (x[:n].double().abs() @ w.abs().t()), dtype)
+        assert (C[:, [0, 77, m - 1]] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1, 8, 9])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_small_results_beside_large_ones(cuda, mm, dtype, n):
+    """One large weight-activation pair in a column of B leaves the other rows' small sums alone."""
+    gen = torch.Generator().manual_seed(n)
+    m, k, group, dt = 64, 384, 128, TYPES[dtype]
+    codes, scales, zps = make_w4(gen, m, k, group, True, dt)
+    codes[1:, 5] = zps[1:, 0]  # only row 0 has a weight in column 5
+    packed = pack(mm, dtype, codes, scales, zps, group)
+    x = (torch.randn(n, k, generator=gen) * 2.0 ** -10).to(dt)
+    x[:, 5] = 2.0 ** 14
+    C = torch.empty(n, m, dtype=dt, device="cuda")
+    mm.gemm_w4(dtype, m, n, k, 1.0, packed, group, True, x.cuda(), k, 0.0, C, m)
+    w = weights64(codes, scales, zps, group)
+    check16(C.cpu(), x.double() @ w.t(), chain(k) * (x.double().abs() @ w.abs().t()), dtype)
+
+
+@pytest.mark.parametrize("dtype,loud", LOUD)
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_packed_layer_with_loud_activations_at_weights_of_zero(cuda, mm, dtype, loud, group, zeros):
+    gen = torch.Generator().manual_seed(group + 1)
+    tokens, d, f, E, topk, dt = 11, 300, 96, 4, 2, TYPES[dtype]
+    x = torch.randn(tokens, d, generator=gen).to(dt)
+    router = (torch.randn(E, d, generator=gen) / 8).to(dt)
+    experts = expert_weights(gen, E, d, f, group, zeros, dt)
+    for j in (1, 200, d - 1):
+        x[:, j] = loud if j != 200 else -loud
+        router[:, j] = 0
+        for n in ("gate", "up"):
+            for codes, scales, zps in experts[n]:
+                codes[:, j] = 8 if zps is None else zps[:, j // group]
+    Y, ids, _ = expert_layer(mm, dtype, x, router, experts, group, topk, renorm=True)
+    y, want_ids, _, bound, _ = moe64(x.double(), router.double(), *in64(experts, group), topk, True)
+    assert torch.equal(ids.long(), want_ids)
+    check16(Y, y, bound, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_a_spoilt_column_beside_others_costs_nothing(cuda, mm, dtype):
+    """A column with a NaN and one with an infinity among eight: they come out as NaN and infinities, and the call takes as
+    long as without them (it took some milliseconds when such columns were summed again element by element)."""
+    gen = torch.Generator().manual_seed(2)
+    m, k, n, group, dt = 512, 16384, 8, 128, TYPES[dtype]
+    codes, scales, zps = make_w4(gen, m, k, group, True, dt)
+    codes[:, 7] = (zps[:, 0] + 1) % 16
+    packed = pack(mm, dtype, codes, scales, zps, group)
+    x = torch.randn(n, k, generator=gen).to(dt)
+    times = []
+    for spoilt in (False, True):
+        if spoilt:
+            x[2, 9], x[5, 7] = float("nan"), float("inf")
+        X, C = x.cuda(), torch.empty(n, m, dtype=dt, device="cuda")
+        marks = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        best = float("inf")
+        for _ in range(8):  # the shortest of several: another process may take the host for a while
+            marks[0].record()
+            for _ in range(20):
+                mm.gemm_w4(dtype, m, n, k, 1.0, packed, group, True, X, k, 0.0, C, m)
+            marks[1].record()
+            torch.cuda.synchronize()
+            best = min(best, marks[0].elapsed_time(marks[1]))
+        times.append(best)
+    got = C.cpu()
+    assert torch.isnan(got[2]).all() and torch.isinf(got[5]).all()
+    assert torch.isfinite(got[[0, 1, 3, 4, 6, 7]]).all()
+    assert times[1] < 5 * times[0]
