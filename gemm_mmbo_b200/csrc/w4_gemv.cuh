@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
     for (int chunk0 = 0; chunk0 < span || chunk0 == 0; chunk0 += a.x_tiles) {
       if (span > a.x_tiles || batch0 == 0) {
         if (batch0 + chunk0 > 0) {
+          fence_proxy_async_smem();  // bulk copies will overwrite what plain stores left
           workers_sync();
           request_x(chunk0);
         }

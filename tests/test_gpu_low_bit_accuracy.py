@@ -227,3 +227,25 @@ def test_a_spoilt_column_beside_others_costs_nothing(cuda, mm, dtype):
     assert torch.isnan(got[2]).all() and torch.isinf(got[5]).all()
     assert torch.isfinite(got[[0, 1, 3, 4, 6, 7]]).all()
     assert times[1] < 5 * times[0]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("m,n,k,ldb", [(2600, 8, 6001, 6008), (2600, 8, 5500, 5504), (5000, 3, 20002, 20008)])
+def test_columns_staged_again_for_every_batch_of_rows(cuda, mm, dtype, m, n, k, ldb):
+    """Columns that do not fit a block's shared memory and rows of several rounds: what plain stores left of one staging (the
+    ragged end of a column) is overwritten by the bulk copies of the next."""
+    gen = torch.Generator().manual_seed(m + k)
+    group, dt = 128, TYPES[dtype]
+    codes, scales, zps = make_w4(gen, m, k, group, True, dt)
+    packed = pack(mm, dtype, codes, scales, zps, group)
+    x = torch.randn(n, k, generator=gen).to(dt)
+    B = torch.full((n, ldb), float("nan"), dtype=dt, device="cuda")
+    B[:, :k] = x.cuda()
+    out = [torch.empty(n, m, dtype=dt, device="cuda") for _ in range(30)]
+    for C in out:
+        mm.gemm_w4(dtype, m, n, k, 1.0, packed, group, True, B, ldb, 0.0, C, m)
+    torch.cuda.synchronize()
+    w = weights64(codes, scales, zps, group).cuda()
+    X = x.cuda().double()
+    check16(out[0].cpu(), (X @ w.t()).cpu(), (chain(k) * (X.abs() @ w.abs().t())).cpu(), dtype)
+    assert all(torch.equal(out[0], C) for C in out[1:])
