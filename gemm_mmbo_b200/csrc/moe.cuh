@@ -576,6 +576,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_up4_kernel(const MoeArgs a
     }
     float* ours = sums + ((n & 1) * kMoeWarps + (team << a.team_log2)) * 256;
     moe_keep_sums(ours + wk * 256, gate, up);
+    __syncwarp();
     asm volatile("bar.sync %0, %1;" ::"r"(2 + team), "r"(WK * 32) : "memory");
     moe_finish_unit<__nv_bfloat16>(a, ours, WK, (wk * 32 + lane + 384 * (n & 3)) & (WK * 32 - 1), cols, unit.rows,
                                    plan.order + p0, W4Operand<T>::kUnit);

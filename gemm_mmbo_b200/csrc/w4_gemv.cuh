@@ -116,8 +116,11 @@ __device__ __forceinline__ void w4_tile_mma(uint32_t tile, Columns column, bool 
 constexpr int kGemvWarps = 16;                       // that multiply
 constexpr int kGemvThreads = (kGemvWarps + 1) * 32;  // and one that feeds them
 constexpr int kGemvMaxSlots = 4;
-// Barrier of the multiplying warps.
-__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kGemvWarps * 32) : "memory"); }
+// Barrier of the multiplying warps.  Loops in front of it may have split a warp, which has to arrive as one.
+__device__ __forceinline__ void workers_sync() {
+  __syncwarp();
+  asm volatile("bar.sync 1, %0;" ::"n"(kGemvWarps * 32) : "memory");
+}
 
 // Untiled bulk copy, completion on an mbarrier of this CTA (addresses and size multiples of 16 bytes), and the request
 // to have the bytes brought into L2.
@@ -156,9 +159,16 @@ __device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, 
   return false;
 }
 
-// Cluster barrier in its two halves, and a store to the same place in another block's shared memory.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Cluster barrier in its two halves, which a warp passes as one, and a store to the same place in another block's shared
+// memory.
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(addr, rank)), "f"(v) : "memory");
 }

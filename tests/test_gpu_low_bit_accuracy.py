@@ -249,3 +249,22 @@ def test_columns_staged_again_for_every_batch_of_rows(cuda, mm, dtype, m, n, k, 
     X = x.cuda().double()
     check16(out[0].cpu(), (X @ w.t()).cpu(), (chain(k) * (X.abs() @ w.abs().t())).cpu(), dtype)
     assert all(torch.equal(out[0], C) for C in out[1:])
+
+
+@pytest.mark.parametrize("n", [1, 3, 5, 7, 8])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_joins_whose_units_do_not_fill_a_warp(cuda, mm, dtype, n):
+    """Few rows and a long contraction: clusters cut k, and the halves of a warp have different numbers of sums to hand over."""
+    gen = torch.Generator().manual_seed(n)
+    group, dt = 64, TYPES[dtype]
+    for m, k in ((16, 8192), (17, 16384), (144, 12288), (1000, 8200), (4112, 4096)):
+        codes, scales, zps = make_w4(gen, m, k, group, True, dt)
+        packed = pack(mm, dtype, codes, scales, zps, group)
+        x = torch.randn(n, k, generator=gen).to(dt)
+        C = torch.empty(n, m, dtype=dt, device="cuda")
+        mm.gemm_w4(dtype, m, n, k, 1.0, packed, group, True, x.cuda(), k, 0.0, C, m)
+        torch.cuda.synchronize()
+        assert mm.device_status() == 0
+        w = weights64(codes, scales, zps, group).cuda()
+        X = x.cuda().double()
+        check16(C.cpu(), (X @ w.t()).cpu(), (chain(k) * (X.abs() @ w.abs().t())).cpu(), dtype)
