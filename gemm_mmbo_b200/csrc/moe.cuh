@@ -78,9 +78,8 @@ struct MoePlan {
   }
 };
 
-// Order of the scores as unsigned integers: larger score, larger key; -0 equals +0; NaN comes first.
+// Order of the scores as unsigned integers: larger score, larger key; -0 equals +0.
 __device__ __forceinline__ uint32_t moe_score_key(float v) {
-  if (v != v) return 0xffffffffu;
   if (v == 0.f) v = 0.f;
   const uint32_t b = __float_as_uint(v);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
@@ -146,13 +145,15 @@ __device__ __forceinline__ void moe_select(const MoeArgs& a, const float* from, 
   for (int e = lane; e < a.experts; e += 32) sum += expf(scores[e] - top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  // A NaN or +inf among the scores, or nothing but -inf: every p is a NaN, so all are equal.
+  const bool lost = sum != sum;
   uint32_t last_key = 0xffffffffu;
   int last = -1;  // the expert taken before
   for (int s = 0; s < a.topk; ++s) {
     uint32_t key = 0;
     int best = 0;
     for (int e = lane; e < a.experts; e += 32) {
-      const uint32_t k = moe_score_key(scores[e]);
+      const uint32_t k = lost ? 1u : moe_score_key(scores[e]);
       if ((k < last_key || (k == last_key && e > last)) && k > key) {
         key = k;
         best = e;

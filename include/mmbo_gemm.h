@@ -350,8 +350,9 @@ int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, const float* alpha, co
 
 /* A whole mixture-of-experts layer for a few tokens.  X is d x tokens, Y d x tokens, router d x
  * experts (ldr >= d: expert e's vector is contiguous).  Per token t:
- *   p = softmax(router^T x);  the topk experts of largest p, the lower number first among equals
- *   (a NaN counts as largest);  g_e = p_e, divided by the sum over the chosen ones if renorm = 1;
+ *   p = softmax(router^T x);  the topk experts of largest p, the lower number first among equals (a
+ *   NaN among the scores makes every p a NaN: experts 0 .. topk - 1);  g_e = p_e, divided by the sum
+ *   over the chosen ones if renorm = 1;
  *   y = sum g_e * down_e * (silu(gate_e x) o (up_e x)) + beta * y.
  * gate_e and up_e are f x d, down_e is d x f, stored like W above.  group = 0: 16-bit experts, row i
  * of gate_e at gate + e * strideG + i * ldg elements (ldg >= d; up the same), of down_e at

@@ -268,3 +268,29 @@ def test_joins_whose_units_do_not_fill_a_warp(cuda, mm, dtype, n):
         w = weights64(codes, scales, zps, group).cuda()
         X = x.cuda().double()
         check16(C.cpu(), (X @ w.t()).cpu(), (chain(k) * (X.abs() @ w.abs().t())).cpu(), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("experts,topk", [(5, 2), (70, 32), (300, 7)])
+def test_choices_without_a_number(cuda, mm, dtype, experts, topk):
+    """A NaN or +inf among a token's scores makes all its probabilities NaN: equal ones, so the lowest experts.  One -inf is a
+    probability of zero."""
+    gen = torch.Generator().manual_seed(experts)
+    tokens, d, f, group, dt = 6, 64, 32, 32, TYPES[dtype]
+    x = torch.randn(tokens, d, generator=gen).to(dt)
+    x[:, 0] = torch.tensor([1.0, -1.0, 1.0, -1.0, 0.0, -1.0])
+    x[3, 9] = float("nan")
+    router = torch.randn(experts, d, generator=gen).to(dt)
+    router[3, 0] = float("inf")  # scores of +inf, -inf, +inf, NaN, NaN, -inf
+    one = expert_weights(gen, 1, d, f, group, False, dt)
+    packs = {n: v * experts for n, v in one.items()}
+    Y, ids, gates = expert_layer(mm, dtype, x, router, packs, group, topk)
+    lowest = torch.arange(topk, dtype=torch.int32)
+    for t in (0, 2, 3, 4):
+        assert torch.equal(ids[t], lowest), t
+        assert torch.isnan(gates[t]).all() and torch.isnan(Y[t]).all()
+    scores = x.double() @ router.double().t()
+    for t in (1, 5):
+        p = torch.softmax(scores[t], 0)
+        assert 3 not in ids[t].tolist() and torch.isfinite(gates[t]).all() and torch.isfinite(Y[t]).all()
+        assert ((gates[t].double() - p[ids[t].long()]).abs() <= 2.0 ** -12 * p[ids[t].long()]).all()
