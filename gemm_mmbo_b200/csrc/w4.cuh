@@ -283,7 +283,16 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(size_t m, size_t k, co
     const float2 range = widen2<T>(ends[0]);
     const float l = range.x, h = -range.y;
     // halves first: the span of two bfloat16 values may pass the largest float
-    const float wide = ZEROS ? (0.5f * h - 0.5f * l) / 7.5f : fmaxf(-l, h) / 7.f;
+    float span = 0.5f * h - 0.5f * l;
+    if (ZEROS && std::is_same<T, __half>::value) {
+      // Two half-precision ends may need 27 bits together (bfloat16 ones that do are too far apart to matter).  Rounded to nearest, a
+      // span beside 15 times a tie of the scale became that tie; rounded to the odd neighbour it stays beside it, and so does the
+      // quotient.
+      const float part = span - 0.5f * h, lost = (0.5f * h - (span - part)) + (-0.5f * l - part);
+      const uint32_t bits = __float_as_uint(span);
+      if (lost != 0.f && (bits & 1u) == 0) span = __uint_as_float(lost > 0.f ? bits + 1 : bits - 1);
+    }
+    const float wide = ZEROS ? span / 7.5f : fmaxf(-l, h) / 7.f;
     float s = to_f32(from_f32<T>(wide));
     if (!(s <= 3.4e38f)) s = __int_as_float(0x7fc00000);
     // A group's multiplier; -s for a scale whose reciprocal might overflow (bfloat16 only): these divide.

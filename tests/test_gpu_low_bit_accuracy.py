@@ -294,3 +294,58 @@ def test_choices_without_a_number(cuda, mm, dtype, experts, topk):
         p = torch.softmax(scores[t], 0)
         assert 3 not in ids[t].tolist() and torch.isfinite(gates[t]).all() and torch.isfinite(Y[t]).all()
         assert ((gates[t].double() - p[ids[t].long()]).abs() <= 2.0 ** -12 * p[ids[t].long()]).all()
+
+
+def to_bits(value, bits):
+    """A positive Fraction rounded to that many significant bits, ties to even."""
+    from fractions import Fraction
+    e = value.numerator.bit_length() - value.denominator.bit_length()
+    if Fraction(2) ** e > value:
+        e -= 1
+    unit = Fraction(2) ** (e - bits + 1)
+    q = value / unit
+    n, rest = divmod(q.numerator, q.denominator)
+    twice = 2 * rest - q.denominator
+    return (n + (twice > 0 or (twice == 0 and n % 2))) * unit
+
+
+def spans_beside_ties():
+    """(h, -l) of half precision whose span in 32 bits is 15 times a tie between two half-precision scales although the
+    span itself is not."""
+    from fractions import Fraction
+    found = []
+    for h in range(1024, 2048):
+        x = Fraction(h, 15)
+        unit = to_bits(x, 1) / 2 ** 11 if to_bits(x, 1) <= x else to_bits(x, 1) / 2 ** 12
+        for n in range(int(x / unit), int(x / unit) + 3):
+            gap = 15 * n * unit - h
+            if n % 2 == 0 or gap <= 0:
+                continue
+            low = to_bits(gap, 11)
+            ulp = to_bits(low, 1) / 2 ** 10 if to_bits(low, 1) <= low else to_bits(low, 1) / 2 ** 11
+            for j in range(-8, 9):
+                l = low + j * ulp
+                if l > 0 and to_bits(l, 11) == l and to_bits(to_bits(h + l, 24) / 15, 11) != to_bits((h + l) / 15, 11):
+                    found.append((h, l))
+    return found
+
+
+def test_scales_of_spans_beside_a_tie(cuda, mm):
+    """Groups whose ends need more than 24 bits together: the scale is the rounded quotient of the exact span."""
+    pairs = spans_beside_ties()
+    assert len(pairs) > 50
+    k, m = 32, len(pairs)
+    for exponent in (0, 4):
+        w = torch.zeros(m, k, dtype=torch.float64)
+        for i, (h, l) in enumerate(pairs):
+            w[i, 3], w[i, 17] = float(h) * 2.0 ** exponent, -float(l) * 2.0 ** exponent
+        W = w.half()
+        assert torch.equal(W.double(), w)
+        packed = torch.empty(mm.w4_bytes(m, k, 32, True), dtype=torch.uint8, device="cuda")
+        mm.w4_quantize("f16", m, k, 32, True, W.cuda(), k, packed)
+        back = torch.empty(m, k, dtype=torch.float16, device="cuda")
+        mm.w4_unpack("f16", m, k, 32, True, packed, back, k)
+        # the small end rounds to no step at all, so that the zero point is 0 and the large end 15 steps
+        want = torch.tensor([float(to_bits(15 * to_bits((h + l) / 15, 11), 11)) for h, l in pairs], dtype=torch.float64)
+        assert torch.equal(back[:, 3].cpu().double(), want * 2.0 ** exponent)
+        assert (back[:, 17] == 0).all()
