@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(UmmaShape<NT>::kThreads, 1)
     const int block = first / a.col_tiles * 8 + (lane & 7), cnt = min(span, a.stages);
     if (lane < 8 && block < row_blocks && cnt > 0)
       bulk_prefetch(a.packed + ((size_t)block * k_tiles + t0) * TILE, cnt * TILE);
-    if (lane == 8) prefetch_tensormap(&w_map);
+    if (lane == 8 && span > 0) prefetch_tensormap(&w_map);  // (no map where k is 0)
     if (lane == 9 && a.x_tma) prefetch_tensormap(&x_map);
   }
   tcgen05_fence_before();
