@@ -349,3 +349,40 @@ def test_scales_of_spans_beside_a_tie(cuda, mm):
         want = torch.tensor([float(to_bits(15 * to_bits((h + l) / 15, 11), 11)) for h, l in pairs], dtype=torch.float64)
         assert torch.equal(back[:, 3].cpu().double(), want * 2.0 ** exponent)
         assert (back[:, 17] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("group", [0, 64])
+def test_hidden_vectors_keep_what_a_16_bit_rounding_leaves(cuda, mm, dtype, group):
+    """Tokens with one element each, so that scores, gates and hidden values come from single exact products; Y holds the
+    negative of the rounded result and beta is one, so that what is left shows the sums to 32 bits.  A hidden value may be off
+    by 2^-17 of itself (two bfloat16) or 2^-22 and 2^-30 (two halves), and by 2^-21 for exp, division and product; dropping
+    the second half would be off by more than the bound."""
+    from test_gpu_moe import Layer
+    tokens, d, f, E, topk, dt = 6, 64, 40, 4, 2, TYPES[dtype]
+    gen = torch.Generator().manual_seed(77)
+    x = torch.zeros(tokens, d)
+    x[torch.arange(tokens), torch.arange(tokens) * 9] = 1 + torch.rand(tokens, generator=gen)
+    layer = Layer(mm, dtype, tokens, d, f, E, topk, renorm=True, group=group, x=x, seed=5)
+    halves = dtype == "f16" and group == 0
+    rel, floor = (2.0 ** -22, 2.0 ** -30) if halves else (2.0 ** -17, 0.0)
+    scores = layer.x.double() @ layer.router.double().t()
+    p, order = torch.sort(torch.softmax(scores, 1), dim=1, descending=True)
+    assert ((p[:, :-1] - p[:, 1:]) > 1e-4).all(), "the inputs leave the choice of experts open"
+    gates = p[:, :topk] / p[:, :topk].sum(1, keepdim=True)
+    y, lost, bound = (torch.zeros(tokens, d, dtype=torch.float64) for _ in range(3))
+    for t in range(tokens):
+        for j in range(topk):
+            e = int(order[t, j])
+            g, u = layer.ref["gate"][e] @ layer.x[t].double(), layer.ref["up"][e] @ layer.x[t].double()
+            h, down = g * torch.sigmoid(g) * u, layer.ref["down"][e]
+            y[t] += gates[t, j] * (down @ h)
+            lost[t] += gates[t, j] * (down @ h.to(dt if group == 0 else torch.bfloat16).double())
+            bound[t] += gates[t, j] * (down.abs() @ (h.abs() * (rel + 2.0 ** -21 + chain(f)) + floor) + 2.0 ** -19 * (down @ h).abs())
+    assert ((lost - y).abs() / bound).max() > 3, "the bound would not notice"
+    Y = -y.to(dt)
+    rest = y + Y.double()
+    Y = Y.cuda()
+    layer.call(Y, beta=1.0)
+    torch.cuda.synchronize()
+    check16(Y.cpu(), rest, bound, dtype)
