@@ -294,18 +294,21 @@ __global__ void __launch_bounds__(kGemvThreads, 1) w4_gemv_kernel(const GemvArgs
   if (warp == kGemvWarps) {
     // For each batch of row groups, for each chunk of k, for each row group: the served warp's part of the chunk in
     // pieces of slot_tiles.  This warp takes no part in the barriers of the others.
-    uint32_t idle = 0;
-    for (int batch0 = 0; batch0 < mine && lane < kGemvWarps; batch0 += a.batch) {
-      for (int chunk0 = 0; chunk0 < span; chunk0 += a.x_tiles) {
+    uint32_t idle = 0;  // tries of the present wait
+    bool more = lane < kGemvWarps;
+    for (int batch0 = 0; more && batch0 < mine; batch0 += a.batch) {
+      for (int chunk0 = 0; more && chunk0 < span; chunk0 += a.x_tiles) {
         const int begin = part_of(chunk0, wk), end = part_of(chunk0, wk + 1);
-        for (int g = batch0; g < min(mine, batch0 + a.batch); ++g) {
+        for (int g = batch0; more && g < min(mine, batch0 + a.batch); ++g) {
           const bool have = (first + g * a.clusters) * WM + wm < row_blocks;
           const unsigned char* src = weights_of(g, wm, begin);
           for (int tile = begin; tile < end;) {
             if (!mbar_try_wait(empty0 + slot * 8, phase ^ 1u)) {
-              if (*(volatile uint32_t*)&abort_flag || ++idle > (1u << 24)) break;  // the others report
+              more = !*(volatile uint32_t*)&abort_flag && ++idle <= (1u << 24);
+              if (!more) break;  // the others report
               continue;
             }
+            idle = 0;
             const int cnt = min(a.slot_tiles, end - tile);
             mbar_expect_tx(full0 + slot * 8, have ? cnt * TILE : 0);
             if (have) bulk_load(ring_at + slot * slot_bytes, src, cnt * TILE, full0 + slot * 8);

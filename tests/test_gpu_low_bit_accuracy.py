@@ -386,3 +386,28 @@ def test_hidden_vectors_keep_what_a_16_bit_rounding_leaves(cuda, mm, dtype, grou
     layer.call(Y, beta=1.0)
     torch.cuda.synchronize()
     check16(Y.cpu(), rest, bound, dtype)
+
+
+@pytest.mark.parametrize("n,ldb_pad", [(1, 0), (8, 0), (8, 3)])
+def test_long_contractions_of_few_rows(cuda, mm, n, ldb_pad):
+    """Two rows of 6e8 weights: more than a million tiles for each of a few blocks, whose feeding warps' waits add up.  B is zero but for 150 places, so that the other additions are exact."""
+    k, m, group = 600_000_000, 2, 128
+    if torch.cuda.mem_get_info()[0] < 40 * 2 ** 30:
+        pytest.skip("needs 40 GB")
+    g, gen = k // group, torch.Generator().manual_seed(3)
+    at = torch.cat([torch.arange(a, a + 50) * 5 for a in (0, k // 11, k // 5 - 50)])
+    codes = torch.randint(0, 256, (m, k // 2), dtype=torch.uint8, device="cuda")
+    scales = (0.002 + 0.01 * torch.rand(m, g, device="cuda")).bfloat16()
+    packed = torch.empty(mm.w4_bytes(m, k, group, False), dtype=torch.uint8, device="cuda")
+    mm.w4_pack("bf16", m, k, group, codes, k // 2, scales, g, None, 0, packed)
+    x = torch.randn(n, at.numel(), generator=gen).bfloat16()
+    B = torch.zeros(n, k + ldb_pad, dtype=torch.bfloat16, device="cuda")
+    B[:, at.cuda()] = x.cuda()
+    C = torch.empty(n, m, dtype=torch.bfloat16, device="cuda")
+    mm.gemm_w4("bf16", m, n, k, 1.0, packed, group, False, B, k + ldb_pad, 0.0, C, m)
+    torch.cuda.synchronize()
+    assert mm.device_status() == 0
+    both = codes[:, at.cuda() // 2].cpu()
+    q = torch.where(at % 2 == 0, both & 15, both >> 4).double()
+    w = (q - 8) * scales[:, (at // group).cuda()].cpu().double()
+    check16(C.cpu(), x.double() @ w.t(), chain(200 * 128) * (x.double().abs() @ w.abs().t()), "bf16")
