@@ -106,8 +106,8 @@ static int launch_clustered(K kernel, unsigned grid, unsigned threads, size_t sm
 
 // How w4_gemv_kernel cuts a problem: the cheapest of all (warps along k, blocks along k), by a sum of what was measured
 // (B200, us): 0.022 a tile of the busiest SM, 0.3 a slot of a warp's ring, 0.05 a KB of activations staged, 1.8 / 2.5 to join
-// clusters of two / four, 1 a batch of row groups.  8192 x 28672, one column: 28.4 us with the chosen 16 x 2, 30.7 with
-// 16 x 1, 49 with 1 x 2; 4096 x 4096: 5.3 with 8 x 1, 7.9 with 8 x 2.
+// clusters of two / four, 1 a batch of row groups.  8192 x 28672, one column: 29.2 us with the chosen 16 x 2, 30.8 with
+// 16 x 1, 52 with 1 x 2; 4096 x 4096: 5.5 with 8 x 1, 8.1 with 8 x 2 (times of a call in a graph).
 static bool plan_gemv(GemvArgs& a, uint32_t tile_bytes, const int (&clusters)[3], size_t* smem) {
   const size_t k_tiles = w4_k_tiles(a.k), blocks = w4_row_blocks(a.m);
   double best = 1e30;
@@ -329,8 +329,8 @@ static int launch_moe(const MoeArgs& args, cudaStream_t st) {
     auto down = moe_down4_kernel<T, QG>;
     if ((rc = allow_smem(up, kGemvSmem, up_ready[0])) || (rc = allow_smem(down, kGemvSmem, down_ready[0]))) return rc;
     // Teams of `up`: small ones (fewer sums to join, fewer barriers) as long as most of them have a unit.  8 tokens, 4 of 32
-    // experts, 4096 to 1800 (some 2200 units): 89 us with teams of four, 96 with sixteen; 1 token, 2 experts, 2048 to 1408 (176
-    // units): 16.4 and 16.1.
+    // experts, 4096 to 1800 (some 2200 units): 83 us with teams of four, 90 with sixteen; 1 token, 2 experts, 2048 to 1408 (176
+    // units): 14.7 with four, 14.4 with eight, 15.1 with sixteen (the rule's).
     const size_t experts = pairs < (size_t)a.experts ? pairs : (size_t)a.experts, units = experts * ((a.f + 15) / 16);
     a.team_log2 = 4;
     while (a.team_log2 > 2 && units >= (size_t)sm_count() * (kMoeWarps >> (a.team_log2 - 1)) * 3 / 4) --a.team_log2;

@@ -4,10 +4,13 @@
 //   g(t, e) = p(t, e)                 (or p(t, e) / sum of p over S(t))
 //   y_t     = sum over e in S(t) of g(t, e) * down_e * (silu(gate_e * x_t) o (up_e * x_t))  +  beta * y_t
 //
-// with silu(v) = v / (1 + exp(-v)).  All sums, the softmax and the products in between are held in 32 bits.
+// with silu(v) = v / (1 + exp(-v)).  Scores, softmax, gates and all sums are held in 32 bits; a hidden value in a pair of 16-bit
+// numbers, see MoeHidden.
 //
 // What bounds it: the bytes of the experts that the tokens choose, and for one token the chain of three kernels.  They run in
-// one stream, each started while the one in front drains (programmatic dependent launch):
+// one stream, each launched while the one in front drains (programmatic dependent launch).  That hides the launch and what a block
+// sets up, no more: a block of `down` has no room beside one of `up` on an SM, so it asks for its first weights when all of
+// `up` has finished.
 //   scores   one warp per (token, expert); also an aligned, zero-padded copy of the activations
 //   up       every block repeats the selection for itself (one to eight microseconds, cheaper than another kernel and its
 //            launch), then its share of the units (expert, 16 rows of gate and up, group of up to eight tokens)
@@ -18,11 +21,12 @@
 // 16 bytes' worth of k of a lane's token), come straight from L2.  Tokens are the eight columns of the instruction; an expert
 // with more tokens is taken in groups of eight, the later ones finding its weights in L2.
 //
-// Measured (whole layer, B200): 48 tokens, 8 of 64 fp16 experts, 2048 to 1408: 231 us, up 131 us (740 MB, 5.6 TB/s), down 100 us
-// (371 MB on 128 of 148 SMs; 76 us without its arithmetic); one token, 6 of 64 bf16 experts of that size: 36 us, of which
-// scores 8, up 22, down 13 one by one; 8 tokens, 4 of 32 packed experts, 4096 to 1800: 86 us, up 45 us and down 43 us (3.9 and
-// 2.2 TB/s: instructions, about 170 a tile in up and 230 in down).  Asking for packed experts' columns a tile ahead made both
-// slower (97 us): the added instructions cost more than the wait.
+// Measured (whole layer, B200): 48 tokens, 8 of 64 fp16 experts, 2048 to 1408: 230 to 242 us, up 131 us (740 MB, 5.6 TB/s), down 100 us
+// (371 MB on 128 of 148 SMs; 76 us without its arithmetic); one token, 6 of 64 bf16 experts of that size: 35 us, of which
+// scores 8, up 22, down 13 one by one; 8 tokens, 4 of 32 packed experts, 4096 to 1800: 84 to 93 us (by the experts that the tokens
+// choose), up 50 us and down 46 us (3.6 and 2.1 TB/s: instructions, about 150 a tile in up and 215 in down).  Asking for packed
+// experts' columns a tile ahead made both slower (97 us where 89 were taken): the added instructions cost more than the wait.
+// More than a pass's tokens read the experts again: 64 tokens 260 us, 128 tokens 522, 256 tokens 1056 (8 of 64 fp16).
 #pragma once
 
 #include "w4_umma.cuh"
@@ -173,8 +177,9 @@ __device__ __forceinline__ void moe_select(const MoeArgs& a, const float* from, 
 
 // ---------------------------------------------------------------- hidden vectors ------
 // Hidden vectors as products take them: a 16-bit value and what its rounding left, so that 16 bits and more survive.
-// bfloat16 has the range of a float.  Half precision holds h / 64 and 2^11 times the remainder: magnitudes up to 4.19e6,
-// steps of 2^-30 near zero (results in half precision have steps of 2^-24).
+// bfloat16 has the range of a float: off by 2^-17 of the value at most.  Half precision holds h / 64 and 2^11 times the
+// remainder: off by 2^-22 of the value, near zero by 2^-30 (results in half precision have steps of 2^-24), up to magnitudes of
+// 4.19e6.  32 bits would take a third product, or one in a type that the weights do not have.
 template <typename U>
 struct MoeHidden;
 template <>
@@ -186,8 +191,8 @@ struct MoeHidden<__half> {
   static constexpr float kScale = 0x1p-6f, kRest = 0x1p11f;
 };
 
-// The selection and its plan, by every block for itself; `scores`: kMoeUpSums bytes of shared memory.  The block's first
-// kMoeThreads threads take part, all of them pass the barriers.
+// The selection and its plan, by every block for itself; `scores`: kMoeUpSums bytes of shared memory.  All threads of
+// the block take part (the first kMoeWarps warps in the selection).
 constexpr size_t kMoeUpSums = (size_t)2 * kMoeWarps * 256 * 4;
 template <typename A>
 __device__ __forceinline__ void moe_make_plan(const A& a, MoePlan& plan, int* ids, int* count, float* scores) {
@@ -358,7 +363,8 @@ __device__ __forceinline__ uint4 moe_piece(uint32_t stage, int row, int column, 
   return WHOLE || column < columns ? lds128(stage + row * kMoeRowBytes + column * 2) : make_uint4(0, 0, 0, 0);
 }
 
-// FED: rows that bulk copies can address; others are read by the multiplying warps themselves.
+// FED: rows that bulk copies can address; others are read by the multiplying warps themselves, four times as slow (48 tokens, 8 of
+// 64 fp16 experts: 230 us at 2048 to 1408, 960 at 2047 to 1407).
 template <typename T, bool FED>
 __global__ void __launch_bounds__(kMoeFed16Threads, 1) moe_up16_kernel(const MoeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];

@@ -343,7 +343,8 @@ int mmbo_w4_unpack(int dtype, size_t m, size_t k, int group, int zeros, const vo
 /* C = alpha * W * B + beta * C with W packed, B k x n (ldb >= k), C m x n (ldc >= m), any n: one
  * token's vector, a decoding batch, a prompt.  Codes enter the products as exact differences q - z and
  * each group's sum is scaled in fp32, so the result differs from the formula by fp32 summation (of the
- * terms (q - z) s B, for any n) and the final rounding only.  C must not overlap B or packed. */
+ * terms (q - z) s B, for any n) and the final rounding only; an infinite scale makes its row infinite
+ * or NaN.  C must not overlap B or packed. */
 int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, const float* alpha, const void* packed,
                  int group, int zeros, const void* B, size_t ldb, const float* beta, void* C, size_t ldc,
                  void* stream);
@@ -359,7 +360,8 @@ int mmbo_gemm_w4(int dtype, size_t m, size_t n, size_t k, const float* alpha, co
  * down + e * strideD + i * ldd (ldd >= f).  group != 0: packed experts (the format above), expert e
  * at e * strideG (strideD) BYTES, multiples of 16; ldg and ldd are not used.
  * Sums, scores and gates are fp32; a hidden value (silu(gate) o up) keeps 16 bits and more, with 16-bit
- * fp16 experts up to a magnitude of 4.19e6 (larger ones become infinite).
+ * fp16 experts between magnitudes of 2^-14 and 4.19e6 (smaller ones are held to 2^-30 absolutely,
+ * larger ones become infinite).
  * ids (tokens x topk, int) and gates (tokens x topk, float) receive the choice and may be NULL.
  * tokens <= MMBO_MOE_MAX_TOKENS, topk <= MMBO_MOE_MAX_TOPK, experts <= MMBO_MOE_MAX_EXPERTS, d and f
  * <= MMBO_MOE_MAX_WIDTH.  workspace: 256-byte aligned device memory of at least
