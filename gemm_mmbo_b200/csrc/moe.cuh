@@ -21,7 +21,7 @@
 // 16 bytes' worth of k of a lane's token), come straight from L2.  Tokens are the eight columns of the instruction; an expert
 // with more tokens is taken in groups of eight, the later ones finding its weights in L2.
 //
-// Measured (whole layer, B200): 48 tokens, 8 of 64 fp16 experts, 2048 to 1408: 230 to 242 us, up 131 us (740 MB, 5.6 TB/s), down 100 us
+// Measured (whole layer, B200): 48 tokens, 8 of 64 fp16 experts, 2048 to 1408: 228 to 242 us, up 131 us (740 MB, 5.6 TB/s), down 100 us
 // (371 MB on 128 of 148 SMs; 76 us without its arithmetic); one token, 6 of 64 bf16 experts of that size: 35 us, of which
 // scores 8, up 22, down 13 one by one; 8 tokens, 4 of 32 packed experts, 4096 to 1800: 84 to 93 us (by the experts that the tokens
 // choose), up 50 us and down 46 us (3.6 and 2.1 TB/s: instructions, about 150 a tile in up and 215 in down).  Asking for packed
